@@ -356,6 +356,54 @@ size_t silcu_sgemv_workspace_bytes(uint32_t N, uint32_t K);
 silcu_status silcu_sgemv(const float *x, const float *W, float *y, const float *bias, uint32_t N,
                          uint32_t K, void *workspace, size_t workspace_bytes, silcu_stream stream);
 
+/* ------------------------------------------------------------ training ops
+ * No counterpart in the reference, whose backward pass has gpu::sigmoid_backward
+ * only: the gradient of layer_norm, the loss of a vocabulary projection with its
+ * gradients, and the norm of a list of gradients. */
+typedef enum silcu_dtype { SILCU_F32 = 0, SILCU_BF16 = 1 } silcu_dtype;
+
+/* layer_norm of a contiguous [rows, cols] matrix of `dtype` that also keeps
+ * each row's statistics for the backward pass (fp32, NULL = not wanted):
+ * mean, and rstd = 1 / sqrt(var + eps).  gamma and beta are fp32 for either
+ * dtype; all arithmetic is fp32, and the output is rounded once.  out may be
+ * `in` itself. */
+silcu_status silcu_layer_norm_forward(const void *in, void *out, float *mean, float *rstd, const float *gamma,
+                                      const float *beta, size_t rows, size_t cols, float eps, int dtype,
+                                      silcu_stream stream);
+/* Its gradients.  With xh = (in - mean) * rstd and a = dout * gamma, per row
+ *   din = rstd * (a - avg(a) - xh * avg(a * xh)) (+ dresidual),
+ * and over all rows dgamma = sum(dout * xh), dbeta = sum(dout) (fp32).
+ * dresidual (NULL = none) is the gradient that reaches `in` past the norm, as in
+ * a pre-norm block.  din may be dout, in or dresidual itself.  dgamma and dbeta
+ * are written, not added to; rows = 0 writes zeros.  The sums' order depends on
+ * the shape and the GPU only, so results repeat bit for bit.  The workspace
+ * holds per-CTA partial sums. */
+size_t silcu_layer_norm_backward_workspace_bytes(size_t rows, size_t cols, int dtype);
+silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const float *mean, const float *rstd,
+                                       const float *gamma, const void *dresidual, void *din, float *dgamma,
+                                       float *dbeta, size_t rows, size_t cols, int dtype, void *workspace,
+                                       size_t workspace_bytes, silcu_stream stream);
+
+/* The 2-norm over a list of tensors: norm = sqrt(sum of x^2 over all of them),
+ * a device scalar.  Squares are added in fp32 in groups of 16 bytes, where they neither
+ * overflow nor vanish, and in fp64 everywhere else.  The list is read on the
+ * host at call time.  clip multiplies every element by
+ * min(1, max_norm / (norm + eps)), a factor rounded to fp32: in place when outputs_host is
+ * NULL, else into outputs_host[i], a tensor of the same size and dtype that
+ * either is tensors[i] or overlaps none of the list.  A norm that is NaN makes
+ * every element NaN; an infinite one makes finite elements 0. */
+typedef struct silcu_tensor {
+  void *data;
+  uint64_t n;
+  int32_t dtype; /* silcu_dtype */
+} silcu_tensor;
+size_t silcu_grad_norm_workspace_bytes(const silcu_tensor *tensors_host, size_t count);
+silcu_status silcu_grad_norm(const silcu_tensor *tensors_host, size_t count, float *norm, void *workspace,
+                             size_t workspace_bytes, silcu_stream stream);
+silcu_status silcu_clip_grad_norm(const silcu_tensor *tensors_host, void *const *outputs_host, size_t count,
+                                  float max_norm, float eps, float *norm, void *workspace, size_t workspace_bytes,
+                                  silcu_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

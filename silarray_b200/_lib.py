@@ -69,6 +69,18 @@ class AttnArgs(C.Structure):
                 ("scale", f32), ("V_hi", vp), ("V_lo", vp)]
 
 
+class CrossEntropyArgs(C.Structure):
+    _fields_ = [("H", vp), ("W", vp), ("targets", vp),
+                ("rows", i64), ("V", i64), ("D", i64), ("ldh", i64), ("ldw", i64),
+                ("dtype", i32), ("reduction", i32),
+                ("loss", vp), ("lse", vp), ("dloss", vp), ("dH", vp), ("dW", vp),
+                ("lddh", i64), ("lddw", i64)]
+
+
+class Tensor(C.Structure):
+    _fields_ = [("data", vp), ("n", u64), ("dtype", i32)]
+
+
 _SIGS = {
     "silcu_last_error": ([], C.c_char_p),
     "silcu_abi_version": ([], C.c_int),
@@ -115,6 +127,12 @@ _SIGS = {
     "silcu_sgemm_bias": ([vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, vp, sz, vp], C.c_int),
     "silcu_sgemm_bias_sigmoid": ([vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, vp, sz, vp], C.c_int),
     "silcu_sgemv_workspace_bytes": ([u32, u32], sz),
+    "silcu_layer_norm_forward": ([vp, vp, vp, vp, vp, vp, sz, sz, f32, C.c_int, vp], C.c_int),
+    "silcu_layer_norm_backward_workspace_bytes": ([sz, sz, C.c_int], sz),
+    "silcu_layer_norm_backward": ([vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, C.c_int, vp, sz, vp], C.c_int),
+    "silcu_grad_norm_workspace_bytes": ([C.POINTER(Tensor), sz], sz),
+    "silcu_grad_norm": ([C.POINTER(Tensor), sz, vp, vp, sz, vp], C.c_int),
+    "silcu_clip_grad_norm": ([C.POINTER(Tensor), C.POINTER(vp), sz, f32, f32, vp, vp, sz, vp], C.c_int),
     "silcu_sgemv": ([vp, vp, vp, vp, u32, u32, vp, sz, vp], C.c_int),
 }
 for _op in ("add", "sub", "mul", "div", "pow"):

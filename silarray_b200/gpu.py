@@ -460,3 +460,169 @@ def sgemv(x, W, y, N, K, bias=None):
     wp, wn = _ws_args(lib().silcu_sgemv_workspace_bytes(N, K), x.device)
     check(lib().silcu_sgemv(_p(x), _p(W), _p(y), _p(bias), N, K, wp, wn, _stream()))
     return y
+
+
+# ------------------------------------------------------------------- training
+DTYPE = {_F32: 0, torch.bfloat16: 1}
+
+
+def _floats(*ts):
+    """Contiguous CUDA tensors of one dtype (fp32 or bf16) and device."""
+    first = None
+    for t in ts:
+        if t is None:
+            continue
+        _dev(t)
+        if t.dtype not in DTYPE:
+            raise TypeError(f"silarray_b200.gpu: expected float32 or bfloat16, got {t.dtype}")
+        if first is None:
+            first = t
+        elif t.dtype != first.dtype:
+            raise TypeError(f"silarray_b200.gpu: {first.dtype} and {t.dtype} operands mixed")
+    return DTYPE[first.dtype]
+
+
+def _same_device(first, *ts):
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"silarray_b200.gpu: operands on {first.device} and {t.device}")
+
+
+def _sized(name, t, n):
+    if t is not None and t.numel() != n:
+        raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
+    return t
+
+
+class _on:
+    """Runs a call on its operands' device: (stream of that device, scratch of
+    nbytes).  The scratch comes from torch's caching allocator for each call,
+    so calls on several streams or in several captured graphs never share it."""
+
+    def __init__(self, device, nbytes=0):
+        self.device, self.nbytes = device, nbytes
+        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device) if self.nbytes else None
+        return _p(self.ws), self.nbytes, _stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows_cols(IN, rows, cols):
+    if rows is None:
+        cols = IN.shape[-1]
+        rows = IN.numel() // cols if cols else 0
+    if rows * cols != IN.numel():
+        raise ValueError(f"layer_norm: {rows} x {cols} rows in {IN.numel()} elements")
+    return rows, cols
+
+
+def layer_norm_forward(IN, OUT=None, gamma=None, beta=None, rows=None, cols=None, eps=1e-5):
+    """layer_norm (fp32 or bf16 rows, fp32 gamma and beta) that also returns the
+    statistics its backward pass needs: (OUT, mean[rows], rstd[rows])."""
+    dt = _floats(IN, OUT)
+    rows, cols = _rows_cols(IN, rows, cols)
+    _sized("layer_norm gamma", _dev(gamma, _F32), cols), _sized("layer_norm beta", _dev(beta, _F32), cols)
+    OUT = torch.empty_like(IN) if OUT is None else _sized("layer_norm OUT", OUT, rows * cols)
+    _same_device(IN, OUT, gamma, beta)
+    stats = torch.empty(2, rows, dtype=_F32, device=IN.device)
+    mean, rstd = stats[0], stats[1]
+    with _on(IN.device) as (_, _, stream):
+        check(lib().silcu_layer_norm_forward(_p(IN), _p(OUT), _p(mean), _p(rstd), _p(gamma), _p(beta), rows, cols,
+                                             float(eps), dt, stream))
+    return OUT, mean, rstd
+
+
+def layer_norm_backward(dout, IN, mean, rstd, gamma, dresidual=None, din=None, dgamma=None, dbeta=None,
+                        rows=None, cols=None):
+    """Gradients of layer_norm_forward: (din, dgamma, dbeta).  dresidual, when
+    given, is added to din (the gradient that bypasses the norm)."""
+    dt = _floats(IN, dout, dresidual, din)
+    rows, cols = _rows_cols(IN, rows, cols)
+    n = rows * cols
+    _sized("layer_norm dout", dout, n), _sized("layer_norm dresidual", dresidual, n)
+    _sized("layer_norm mean", _dev(mean, _F32), rows), _sized("layer_norm rstd", _dev(rstd, _F32), rows)
+    _sized("layer_norm gamma", _dev(gamma, _F32), cols)
+    din = torch.empty_like(IN) if din is None else _sized("layer_norm din", din, n)
+    if dgamma is None:
+        dgamma = torch.empty(cols, dtype=_F32, device=IN.device)
+    if dbeta is None:
+        dbeta = torch.empty(cols, dtype=_F32, device=IN.device)
+    _sized("layer_norm dgamma", _dev(dgamma, _F32), cols), _sized("layer_norm dbeta", _dev(dbeta, _F32), cols)
+    _same_device(IN, dout, mean, rstd, gamma, dresidual, din, dgamma, dbeta)
+    with _on(IN.device, lib().silcu_layer_norm_backward_workspace_bytes(rows, cols, dt)) as (wp, wn, stream):
+        check(lib().silcu_layer_norm_backward(_p(dout), _p(IN), _p(mean), _p(rstd), _p(gamma), _p(dresidual),
+                                              _p(din), _p(dgamma), _p(dbeta), rows, cols, dt, wp, wn, stream))
+    return din, dgamma, dbeta
+
+
+class TensorList:
+    """The gradients of a model as grad_norm and clip_grad_norm take them: a
+    list of fp32 / bf16 CUDA tensors, laid out once for the C call (and again
+    when a tensor's storage has moved)."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise ValueError("TensorList: no tensors")
+        self.device = self.tensors[0].device
+        self._addresses = None
+        self._layout()
+
+    def _layout(self):
+        """Checks the tensors and fills the C arrays, unless no address changed."""
+        addresses = [t.data_ptr() for t in self.tensors]
+        if addresses == self._addresses:
+            return self
+        n = len(self.tensors)
+        self.array = (_lib.Tensor * n)()
+        self.pointers = (ct.c_void_p * n)(*addresses)
+        for i, t in enumerate(self.tensors):
+            _floats(t)
+            _same_device(self.tensors[0], t)
+            self.array[i] = _lib.Tensor(addresses[i], t.numel(), DTYPE[t.dtype])
+        self._addresses = addresses
+        return self
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def _matches(self, other):
+        return len(self) == len(other) and self.device == other.device and all(
+            a.dtype == b.dtype and a.n == b.n for a, b in zip(self.array, other.array))
+
+
+def _list(tensors):
+    return tensors._layout() if isinstance(tensors, TensorList) else TensorList(tensors)
+
+
+def grad_norm(tensors):
+    """2-norm over a list of tensors (or a TensorList) as a 0-d device tensor."""
+    tl = _list(tensors)
+    norm = torch.empty((), dtype=_F32, device=tl.device)
+    with _on(tl.device, lib().silcu_grad_norm_workspace_bytes(tl.array, len(tl))) as (wp, wn, stream):
+        check(lib().silcu_grad_norm(tl.array, len(tl), _p(norm), wp, wn, stream))
+    return norm
+
+
+def clip_grad_norm(tensors, max_norm, OUT=None, eps=1e-6):
+    """Multiplies the tensors by min(1, max_norm / (norm + eps)), in place or
+    into OUT (a list or TensorList of the same shapes); returns the norm before
+    clipping as a 0-d device tensor."""
+    tl = _list(tensors)
+    out = None
+    if OUT is not None:
+        out = _list(OUT)
+        if not tl._matches(out):
+            raise ValueError("clip_grad_norm: OUT must match the tensors in number, size, dtype and device")
+    norm = torch.empty((), dtype=_F32, device=tl.device)
+    with _on(tl.device, lib().silcu_grad_norm_workspace_bytes(tl.array, len(tl))) as (wp, wn, stream):
+        check(lib().silcu_clip_grad_norm(tl.array, out.pointers if out is not None else None, len(tl),
+                                         float(max_norm), float(eps), _p(norm), wp, wn, stream))
+    return norm

@@ -1,0 +1,103 @@
+"""The training operators without a GPU: their formulas (the references of the
+GPU tests) against torch's autograd in fp64, and what the C entry points and the
+Python mirror refuse before they touch a device."""
+import ctypes as C
+
+import pytest
+import torch
+
+from silarray_b200 import _build, _lib
+
+
+# ----------------------------------------------------------------- references
+def ln_forward_ref(x, gamma, beta, eps):
+    mean = x.mean(1)
+    var = (x - mean[:, None]).square().mean(1)
+    rstd = 1.0 / (var + eps).sqrt()
+    return (x - mean[:, None]) * rstd[:, None] * gamma + beta, mean, rstd
+
+
+def ln_backward_ref(dy, x, mean, rstd, gamma, dres=None):
+    xh = (x - mean[:, None]) * rstd[:, None]
+    a = dy * gamma
+    dx = rstd[:, None] * (a - a.mean(1, keepdim=True) - xh * (a * xh).mean(1, keepdim=True))
+    return dx if dres is None else dx + dres, (dy * xh).sum(0), dy.sum(0)
+
+
+def test_layer_norm_reference_is_the_gradient():
+    g = torch.Generator().manual_seed(0)
+    x, gamma, beta = (torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((5, 33), 33, 33))
+    dy = torch.randn(5, 33, generator=g, dtype=torch.float64)
+    out, mean, rstd = ln_forward_ref(x, gamma, beta, 1e-5)
+    grads = torch.autograd.grad((out * dy).sum(), (x, gamma, beta))
+    for p, q in zip(ln_backward_ref(dy, x, mean, rstd, gamma), grads):
+        assert torch.allclose(p, q, rtol=1e-10, atol=1e-12)
+
+
+# ------------------------------------------------------------------- refusals
+@pytest.fixture(scope="module")
+def lib():
+    _build.build()
+    return _lib.lib()
+
+
+P = C.c_void_p(1 << 20)  # never dereferenced: every call below fails its checks first
+
+
+def test_layer_norm_refusals(lib):
+    f, b = lib.silcu_layer_norm_forward, lib.silcu_layer_norm_backward
+    assert f(None, None, None, None, None, None, 0, 5, 1e-5, 0, None) == 0  # no rows: nothing to do
+    assert f(P, P, None, None, P, None, 4, 8, 1e-5, 0, None) == 1  # no beta
+    assert f(P, P, None, None, P, P, 4, 0, 1e-5, 0, None) == 1  # no columns
+    assert f(P, P, None, None, P, P, 4, 8, 1e-5, 2, None) == 1 and b"dtype" in lib.silcu_last_error()
+    assert f(P, P, None, None, P, P, 4, (1 << 24) + 1, 1e-5, 0, None) == 5
+    assert f(P, P, None, None, P, P, 1 << 31, 8, 1e-5, 0, None) == 5
+    need = lib.silcu_layer_norm_backward_workspace_bytes(100, 768, 0)
+    assert need >= 2 * 768 * 4
+    args = (P, P, P, P, P, None, P, P, P, 100, 768, 0)
+    assert b(*args, P, need - 1, None) == 4
+    assert b(*args, None, need, None) == 4
+    assert b(*args, C.c_void_p((1 << 20) + 2), need, None) == 1
+    assert b(P, P, None, P, P, None, P, P, P, 100, 768, 0, P, need, None) == 1
+    assert b(P, P, P, P, P, None, P, None, P, 100, 768, 0, P, need, None) == 1
+    assert lib.silcu_layer_norm_backward_workspace_bytes(0, 768, 0) == 0
+
+
+def test_gradient_list_refusals(lib):
+    norm, clip = lib.silcu_grad_norm, lib.silcu_clip_grad_norm
+    two = (_lib.Tensor * 2)(_lib.Tensor(1 << 20, 100, 0), _lib.Tensor(1 << 21, 50, 1))
+    need = lib.silcu_grad_norm_workspace_bytes(two, 2)
+    assert need >= 8
+    assert norm(two, 2, None, P, need, None) == 1
+    assert norm(two, 2, P, P, need - 1, None) == 4
+    assert norm(None, 2, P, P, 64, None) == 1
+    assert norm(two, 2, P, C.c_void_p((1 << 20) + 4), need, None) == 1
+    for bad in (_lib.Tensor(1 << 20, 100, 7), _lib.Tensor(0, 100, 0), _lib.Tensor((1 << 20) + 2, 100, 0),
+                _lib.Tensor((1 << 20) + 1, 100, 1)):
+        lst = (_lib.Tensor * 2)(two[0], bad)
+        assert norm(lst, 2, P, P, 1 << 20, None) == 1 and b"tensor 1" in lib.silcu_last_error()
+    assert norm((_lib.Tensor * 1)(_lib.Tensor(1 << 20, 1 << 48, 0)), 1, P, P, 1 << 20, None) == 5
+    assert clip(two, None, 2, -1.0, 1e-6, P, P, need, None) == 1
+    assert clip(two, None, 2, float("nan"), 1e-6, P, P, need, None) == 1
+    assert clip(two, None, 2, 1.0, -1.0, P, P, need, None) == 1
+    outs = (C.c_void_p * 2)(1 << 20, 0)
+    assert clip(two, outs, 2, 1.0, 1e-6, P, P, need, None) == 1 and b"output 1" in lib.silcu_last_error()
+
+
+def test_workspace_of_many_tensors(lib):
+    """One fp64 partial per CTA, whatever the list's length; empty tensors ask for none."""
+    many = (_lib.Tensor * 3000)(*[_lib.Tensor(1 << 20, 10, 0)] * 3000)
+    assert 8 <= lib.silcu_grad_norm_workspace_bytes(many, 3000) <= 8 * 3 * 148 * 8
+    none = (_lib.Tensor * 2)(_lib.Tensor(0, 0, 0), _lib.Tensor(0, 0, 1))
+    assert lib.silcu_grad_norm_workspace_bytes(none, 2) == 0
+
+
+def test_python_refuses_cpu_tensors():
+    from silarray_b200 import gpu
+    x = torch.ones(4, 8)
+    with pytest.raises(TypeError):
+        gpu.layer_norm_forward(x, gamma=x[0], beta=x[0])
+    with pytest.raises(TypeError):
+        gpu.grad_norm([x])
+    with pytest.raises(ValueError):
+        gpu.TensorList([])
