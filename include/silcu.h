@@ -384,6 +384,41 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
                                        float *dbeta, size_t rows, size_t cols, int dtype, void *workspace,
                                        size_t workspace_bytes, silcu_stream stream);
 
+/* Softmax cross entropy of a vocabulary projection, without its logits in
+ * memory: s = H . W^T, lse_t = log(sum_v exp(s_tv)), loss_t = lse_t - s_t,y(t).
+ * H is [rows, D] (row stride ldh), W [V, D] (ldw), both of `dtype`; sums,
+ * softmax and loss are fp32.  A target outside [0, V) leaves its row out: loss
+ * 0, zero gradients, not counted, whatever H holds in it.
+ * reduction: NONE writes loss[rows]; SUM and MEAN write the scalar loss[0],
+ * MEAN divided by the number of rows that count (0 when there are none).
+ * lse (forward output, backward input) is [rows], for every row.
+ * The backward pass recomputes the scores in pieces of the vocabulary:
+ *   ds_tv = dloss_t * (exp(s_tv - lse_t) - [v = y(t)]),  dH = ds . W,  dW = ds^T . H
+ * dloss: [rows] for NONE, a device scalar for SUM and MEAN (there dloss_t =
+ * dloss, or dloss / count); NULL = 1.  dH / dW may be NULL when not wanted;
+ * they are written, not added to.  f32 products are 3xTF32; with bf16, ds is
+ * rounded to bf16 once (the products' operand type) and sums are fp32.
+ * dH may not overlap H, nor dW W. */
+typedef enum silcu_reduction { SILCU_REDUCE_MEAN = 0, SILCU_REDUCE_SUM = 1, SILCU_REDUCE_NONE = 2 } silcu_reduction;
+typedef struct silcu_cross_entropy_args {
+  const void *H, *W;
+  const int32_t *targets;
+  int64_t rows, V, D, ldh, ldw;
+  int32_t dtype, reduction;
+  float *loss;         /* forward */
+  float *lse;          /* forward: written; backward: read */
+  const float *dloss;  /* backward */
+  void *dH, *dW;       /* backward */
+  int64_t lddh, lddw;
+} silcu_cross_entropy_args;
+/* Workspace for both directions, or (backward = 0) for the forward pass alone.
+ * Queried with the dH and dW (NULL or not) of the call. */
+size_t silcu_linear_cross_entropy_workspace_bytes(const silcu_cross_entropy_args *args_host, int backward);
+silcu_status silcu_linear_cross_entropy(const silcu_cross_entropy_args *args_host, void *workspace,
+                                        size_t workspace_bytes, silcu_stream stream);
+silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args *args_host, void *workspace,
+                                                 size_t workspace_bytes, silcu_stream stream);
+
 /* The 2-norm over a list of tensors: norm = sqrt(sum of x^2 over all of them),
  * a device scalar.  Squares are added in fp32 in groups of 16 bytes, where they neither
  * overflow nor vanish, and in fp64 everywhere else.  The list is read on the

@@ -130,6 +130,9 @@ _SIGS = {
     "silcu_layer_norm_forward": ([vp, vp, vp, vp, vp, vp, sz, sz, f32, C.c_int, vp], C.c_int),
     "silcu_layer_norm_backward_workspace_bytes": ([sz, sz, C.c_int], sz),
     "silcu_layer_norm_backward": ([vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, C.c_int, vp, sz, vp], C.c_int),
+    "silcu_linear_cross_entropy_workspace_bytes": ([C.POINTER(CrossEntropyArgs), C.c_int], sz),
+    "silcu_linear_cross_entropy": ([C.POINTER(CrossEntropyArgs), vp, sz, vp], C.c_int),
+    "silcu_linear_cross_entropy_backward": ([C.POINTER(CrossEntropyArgs), vp, sz, vp], C.c_int),
     "silcu_grad_norm_workspace_bytes": ([C.POINTER(Tensor), sz], sz),
     "silcu_grad_norm": ([C.POINTER(Tensor), sz, vp, vp, sz, vp], C.c_int),
     "silcu_clip_grad_norm": ([C.POINTER(Tensor), C.POINTER(vp), sz, f32, f32, vp, vp, sz, vp], C.c_int),

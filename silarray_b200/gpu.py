@@ -562,6 +562,78 @@ def layer_norm_backward(dout, IN, mean, rstd, gamma, dresidual=None, din=None, d
     return din, dgamma, dbeta
 
 
+REDUCTION = {"mean": 0, "sum": 1, "none": 2}
+
+
+def _matrix(name, t, rows=None, cols=None, dtype=None):
+    """A 2-D fp32 / bf16 CUDA tensor with contiguous rows; its row stride."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError("silarray_b200.gpu: operands must be CUDA tensors (no CPU fallback)")
+    if t.dtype not in DTYPE or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name}: expected {dtype or 'float32 or bfloat16'}, got {t.dtype}")
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name}: bad shape {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows must be contiguous and apart")
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _cross_entropy_args(H, W, targets, lse, reduction):
+    if reduction not in REDUCTION:
+        raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    a = _lib.CrossEntropyArgs()
+    a.ldh = _matrix("linear_cross_entropy H", H)
+    a.ldw = _matrix("linear_cross_entropy W", W, cols=H.shape[1], dtype=H.dtype)
+    _sized("linear_cross_entropy targets", _dev(targets, _I32), H.shape[0])
+    _sized("linear_cross_entropy lse", _dev(lse, _F32), H.shape[0])
+    a.H, a.W, a.targets, a.lse = H.data_ptr(), W.data_ptr(), targets.data_ptr(), lse.data_ptr()
+    a.rows, a.V, a.D = H.shape[0], W.shape[0], H.shape[1]
+    a.dtype, a.reduction = DTYPE[H.dtype], REDUCTION[reduction]
+    return a
+
+
+def linear_cross_entropy(H, W, targets, reduction="mean", loss=None, lse=None):
+    """Softmax cross entropy of the scores H . W^T without the scores in memory:
+    H [rows, D] and W [V, D] fp32 or bf16, targets [rows] int32; a target
+    outside [0, V) leaves its row out.  Returns (loss, lse): the fp32 mean (over
+    the rows that count) or sum as a 0-d tensor, or [rows] for "none"; lse
+    [rows] is what the backward pass needs."""
+    n = H.shape[0]
+    if lse is None:
+        lse = torch.empty(n, dtype=_F32, device=H.device)
+    a = _cross_entropy_args(H, W, targets, lse, reduction)
+    if loss is None:
+        loss = torch.empty(n if reduction == "none" else (), dtype=_F32, device=H.device)
+    a.loss = _sized("linear_cross_entropy loss", _dev(loss, _F32), n if reduction == "none" else 1).data_ptr()
+    _same_device(H, W, targets, loss, lse)
+    with _on(H.device, lib().silcu_linear_cross_entropy_workspace_bytes(ct.byref(a), 0)) as (wp, wn, stream):
+        check(lib().silcu_linear_cross_entropy(ct.byref(a), wp, wn, stream))
+    return loss, lse
+
+
+def linear_cross_entropy_backward(H, W, targets, lse, dloss=None, reduction="mean", dH=None, dW=None,
+                                  need_dH=True, need_dW=True):
+    """Gradients (dH, dW) of linear_cross_entropy in the operands' type, for the
+    gradient dloss of its result (a 0-d tensor, [rows] for "none"; None = 1);
+    None in place of one that is not needed."""
+    a = _cross_entropy_args(H, W, targets, lse, reduction)
+    if dloss is not None:
+        a.dloss = _sized("linear_cross_entropy dloss", _dev(dloss, _F32),
+                         H.shape[0] if reduction == "none" else 1).data_ptr()
+    if need_dH:
+        dH = torch.empty(H.shape, dtype=H.dtype, device=H.device) if dH is None else dH
+        a.lddh = _matrix("linear_cross_entropy dH", dH, *H.shape, dtype=H.dtype)
+        a.dH = dH.data_ptr()
+    if need_dW:
+        dW = torch.empty(W.shape, dtype=W.dtype, device=W.device) if dW is None else dW
+        a.lddw = _matrix("linear_cross_entropy dW", dW, *W.shape, dtype=W.dtype)
+        a.dW = dW.data_ptr()
+    _same_device(H, W, targets, lse, dloss, dH, dW)
+    with _on(H.device, lib().silcu_linear_cross_entropy_workspace_bytes(ct.byref(a), 1)) as (wp, wn, stream):
+        check(lib().silcu_linear_cross_entropy_backward(ct.byref(a), wp, wn, stream))
+    return dH if need_dH else None, dW if need_dW else None
+
+
 class TensorList:
     """The gradients of a model as grad_norm and clip_grad_norm take them: a
     list of fp32 / bf16 CUDA tensors, laid out once for the C call (and again

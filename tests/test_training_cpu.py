@@ -24,6 +24,40 @@ def ln_backward_ref(dy, x, mean, rstd, gamma, dres=None):
     return dx if dres is None else dx + dres, (dy * xh).sum(0), dy.sum(0)
 
 
+def cross_entropy_ref(H, W, y, reduction, dloss):
+    V = W.shape[0]
+    used = (y >= 0) & (y < V)
+    H = torch.where(used[:, None], H, H.nan_to_num(0.0, 0.0, 0.0))
+    s = H @ W.T
+    lse = torch.logsumexp(s, 1)
+    at = torch.where(used, y, torch.zeros_like(y))
+    row = torch.where(used, lse - s.gather(1, at[:, None])[:, 0], torch.zeros_like(lse))
+    n = max(1, int(used.sum()))
+    loss = {"none": row, "sum": row.sum(), "mean": row.sum() / n}[reduction]
+    d = torch.ones((), dtype=H.dtype, device=H.device) if dloss is None else dloss
+    scale = torch.where(used, (d / n if reduction == "mean" else d).expand_as(row), torch.zeros_like(row))
+    p = torch.exp(s - lse[:, None])
+    ds = p.clone()
+    ds[torch.arange(len(y), device=H.device), at] -= 1.0
+    ds = ds * scale[:, None]
+    hz = torch.where(used[:, None], H, torch.zeros_like(H))
+    return {"loss": loss, "lse": lse, "row_loss": row, "scale": scale, "p": p, "ds": ds, "dH": ds @ W, "dW": ds.T @ hz}
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_cross_entropy_reference_is_the_gradient(reduction):
+    g = torch.Generator().manual_seed(0)
+    H, W = (torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((6, 9), (13, 9)))
+    y = torch.tensor([0, 12, -100, 13, 5, 5])
+    dloss = torch.randn(6 if reduction == "none" else (), generator=g, dtype=torch.float64)
+    target = torch.where(y < 13, y, torch.full_like(y, -100))
+    loss = torch.nn.functional.cross_entropy(H @ W.T, target, ignore_index=-100, reduction=reduction)
+    r = cross_entropy_ref(H.detach(), W.detach(), y, reduction, dloss)
+    assert torch.allclose(r["loss"], loss.detach())
+    for p, q in zip((r["dH"], r["dW"]), torch.autograd.grad((loss * dloss).sum(), (H, W))):
+        assert torch.allclose(p, q, rtol=1e-10, atol=1e-12)
+
+
 def test_layer_norm_reference_is_the_gradient():
     g = torch.Generator().manual_seed(0)
     x, gamma, beta = (torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((5, 33), 33, 33))
@@ -82,6 +116,53 @@ def test_gradient_list_refusals(lib):
     assert clip(two, None, 2, 1.0, -1.0, P, P, need, None) == 1
     outs = (C.c_void_p * 2)(1 << 20, 0)
     assert clip(two, outs, 2, 1.0, 1e-6, P, P, need, None) == 1 and b"output 1" in lib.silcu_last_error()
+
+
+def _loss_args(**kw):
+    a = _lib.CrossEntropyArgs()
+    for k in ("H", "W", "targets", "loss", "lse", "dH", "dW"):
+        setattr(a, k, 1 << 20)
+    a.rows, a.V, a.D, a.ldh, a.ldw, a.lddh, a.lddw = 10, 100, 64, 64, 64, 64, 64
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_cross_entropy_refusals(lib):
+    size, fwd, bwd = (lib.silcu_linear_cross_entropy_workspace_bytes, lib.silcu_linear_cross_entropy,
+                      lib.silcu_linear_cross_entropy_backward)
+    big = 1 << 30
+    for status, kw in [(1, dict(dtype=2)), (1, dict(reduction=3)), (1, dict(rows=-1)), (1, dict(V=0)), (1, dict(D=0)),
+                       (1, dict(ldh=63)), (1, dict(ldw=10)), (5, dict(rows=(1 << 20) + 1)), (5, dict(V=(1 << 24) + 1)),
+                       (5, dict(ldh=(1 << 32) + 1)), (1, dict(H=0)), (1, dict(W=0)), (1, dict(targets=0)),
+                       (1, dict(lse=0)), (1, dict(H=(1 << 20) + 2)), (1, dict(W=(1 << 20) + 1, dtype=1))]:
+        a = _loss_args(**kw)
+        assert fwd(C.byref(a), P, big, None) == status, kw
+        assert bwd(C.byref(a), P, big, None) == status, kw
+    assert fwd(None, P, big, None) == 1 and bwd(None, P, big, None) == 1
+    a = _loss_args(loss=0)
+    assert fwd(C.byref(a), P, big, None) == 1
+    for kw in (dict(lddh=63), dict(lddw=1), dict(dH=(1 << 20) + 1)):
+        a = _loss_args(**kw)
+        assert bwd(C.byref(a), P, big, None) == 1, kw
+    for dtype in (0, 1):
+        a = _loss_args(dtype=dtype)
+        need = size(C.byref(a), 1)
+        assert need >= size(C.byref(a), 0) > 0
+        assert bwd(C.byref(a), P, need - 1, None) == 4 and bwd(C.byref(a), None, need, None) == 4
+        assert fwd(C.byref(a), P, 10, None) == 4
+    a = _loss_args(dH=0, dW=0)
+    assert bwd(C.byref(a), None, 0, None) == 0  # nothing wanted
+    a = _loss_args(rows=0, reduction=2, loss=0)
+    assert fwd(C.byref(a), None, 0, None) == 0 and size(C.byref(a), 1) == 0
+
+
+def test_cross_entropy_workspace_stays_in_pieces(lib):
+    """The workspace of a large vocabulary does not grow with it: a piece of the
+    score gradients, not the logits."""
+    a = _loss_args(rows=8192, V=1 << 17, D=2048, ldh=2048, ldw=2048, lddh=2048, lddw=2048, dtype=1)
+    logits = 2 * 8192 * (1 << 17)
+    assert lib.silcu_linear_cross_entropy_workspace_bytes(C.byref(a), 1) < logits / 4
 
 
 def test_workspace_of_many_tensors(lib):
