@@ -420,7 +420,7 @@ silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args 
                                                  size_t workspace_bytes, silcu_stream stream);
 
 /* The 2-norm over a list of tensors: norm = sqrt(sum of x^2 over all of them),
- * a device scalar.  Squares are added in fp32 in groups of 16 bytes, where they neither
+ * a device scalar.  Squares are added in fp32 in groups of up to 64 bytes, where they neither
  * overflow nor vanish, and in fp64 everywhere else.  The list is read on the
  * host at call time.  clip multiplies every element by
  * min(1, max_norm / (norm + eps)), a factor rounded to fp32: in place when outputs_host is

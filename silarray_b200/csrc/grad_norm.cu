@@ -10,8 +10,8 @@
 // The clipping pass walks its spans from the last to the first, as the norm
 // pass's most recent reads are what the L2 still holds.
 //
-// Squares add in fp32 in groups of 16 bytes' elements, and the groups in fp64.
-// A group whose fp32 sum may have overflowed or lost denormal squares adds
+// Squares add in fp32 over four 16-byte vectors of a thread, and those sums in fp64.
+// Vectors whose fp32 sum may have overflowed or lost denormal squares add
 // again in fp64.  Every CTA writes one fp64 partial; all of them add in CTA
 // order, so results repeat bit for bit.
 #include <math.h>
@@ -41,22 +41,28 @@ struct ListArgs {
   float max_norm, eps;
 };
 
-// Sum of the squares of N values in fp64 from fp32 products.
+// Whether a fp32 sum of squares stands: nothing overflowed, and no square
+// small enough to have vanished matters in it.
+__device__ __forceinline__ bool in_range(float s) { return s > 1e-28f && s < 1e37f; }
+
 template <int N>
-__device__ __forceinline__ double squares(const float (&f)[N]) {
+__device__ __forceinline__ float squares32(const float (&f)[N]) {
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < N; k++) s = fmaf(f[k], f[k], s);
-  if (s > 1e-28f && s < 1e38f) return double(s);
+  return s;
+}
+template <int N>
+__device__ __forceinline__ double squares64(const float (&f)[N]) {
   double d = 0.0;
 #pragma unroll
   for (int k = 0; k < N; k++) d = fma(double(f[k]), double(f[k]), d);
   return d;
 }
 
-// A warp's part of one tensor: f.vec for whole aligned 16-byte vectors, f.one
-// for the elements before and after them.  `skew` = the operands' common
-// offset from a 16-byte boundary, in elements, or < 0 when they have none.
+// A warp's part of one tensor: f.vec4 / f.vec for whole 16-byte vectors from a
+// 128-byte line on, f.one for the elements before and after them.  `head` =
+// elements before the first line, or < 0 where the operands have no common one.
 template <typename T, typename F>
 __device__ __forceinline__ void walk(uint64_t n, int head, F &&f) {
   constexpr int V = 16 / sizeof(T);
@@ -66,7 +72,7 @@ __device__ __forceinline__ void walk(uint64_t n, int head, F &&f) {
     return;
   }
   if (uint64_t(head) > n) head = int(n);
-  if (lane < uint32_t(head)) f.one(lane);
+  for (int i = lane; i < head; i += 32) f.one(i);
   const uint64_t nv = (n - head) / V;
   uint64_t i = lane;
   for (; i + 96 < nv; i += 128) f.vec4(head + i * V);
@@ -75,10 +81,10 @@ __device__ __forceinline__ void walk(uint64_t n, int head, F &&f) {
   if (done + lane < n) f.one(done + lane);
 }
 
-// Elements of T from p to the next 16-byte boundary.
+// Elements of T from p to the next 128-byte line.
 template <typename T>
 __device__ __forceinline__ int head_of(const void *p) {
-  return int(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+  return int(((128 - (reinterpret_cast<uintptr_t>(p) & 127)) & 127) / sizeof(T));
 }
 
 template <typename T>
@@ -89,22 +95,36 @@ struct SumSquares {
   __device__ __forceinline__ void one(uint64_t i) {
     float f[1];
     unpack(raw_ld<1>(i), f);
-    acc += squares(f);
+    acc += squares64(f);
   }
   __device__ __forceinline__ void vec(uint64_t i) {
     float f[V];
     unpack(raw_ld<V>(i), f);
-    acc += squares(f);
+    const float s = squares32(f);
+    acc += in_range(s) ? double(s) : squares64(f);
   }
   __device__ __forceinline__ void vec4(uint64_t i) {
     Raw<T, V> r[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) r[u] = raw_ld<V>(i + u * 32 * V);
+    float s[4];
+    bool all = true;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       float f[V];
       unpack(r[u], f);
-      acc += squares(f);
+      s[u] = squares32(f);
+      all = all && in_range(s[u]);
+    }
+    if (all) {
+      acc += double((s[0] + s[1]) + (s[2] + s[3]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        float f[V];
+        unpack(r[u], f);
+        acc += squares64(f);
+      }
     }
   }
   // plain loads: the clipping pass finds the newest of them in the L2

@@ -7,15 +7,28 @@
 //
 // Both are bound by HBM: the forward reads x and writes y, the backward reads
 // dy, x (and the residual gradient) and writes dx, each once.  A row lives in
-// registers: a warp per row up to 1024 columns, a CTA per row up to 16384, a
-// re-reading loop beyond.  Elements move as 16-byte vectors where the columns
-// and pointers allow (VEC = 4 fp32 / 8 bf16), else one by one (VEC = 1).
+// the registers of a warp (short rows) or of a CTA, 4 to 32 elements a thread;
+// beyond 16384 columns a CTA re-reads its row.  Elements move as 16-byte
+// vectors where columns and pointers allow (4 fp32 / 8 bf16), else one by one.
 //
-// Backward: a persistent grid; each group of threads walks its rows and adds
-// its columns' dgamma / dbeta terms as it goes (in registers for a warp per
-// row, in the thread's own shared-memory slots for a CTA per row), writes one
-// partial row per CTA, and ln_finish adds the partials in CTA order.  All sums
-// are fp32 in an order fixed by the shape and the SM count.
+// Three kernels, by what keeps the memory busy (measured, rows rotating
+// through more than the L2):
+//   ln_forward         a group of threads per row, many short-lived CTAs: fp32
+//                      rows, 8192 x 4096 in 43.3 us (6.2 TB/s; persistent with
+//                      prefetch 47.4).
+//   ln_forward_stream  bf16 vectors: persistent, the next row's loads in flight
+//                      during this row's sums, gamma and beta in shared memory.
+//                      At 8 elements a vector the parameters weigh twice the
+//                      row, and read from global memory with a 32-byte lane
+//                      stride they keep the L1 77 % busy: 4096 x 8192 39.2 us
+//                      with ln_forward, 31.4 persistent, 28.5 with shared memory.
+//   ln_backward        persistent, prefetching; each thread adds its columns'
+//                      dgamma / dbeta terms in registers over all rows of its CTA,
+//                      one partial row per CTA, added in CTA order by ln_finish.
+//                      16384 x 768 fp32 with residual: 34 us (5.9 TB/s), 48 with a
+//                      warp per row (151 registers, one CTA per SM); 8190 x 4096
+//                      bf16: 72 us with the sums in shared memory instead.
+// All sums are fp32 in an order fixed by the shape and the SM count.
 #include "elem.cuh"
 
 namespace silcu {
@@ -85,7 +98,7 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_forward(const LnArgs a) {
       }
     }
   }
-  const float rstd = 1.0f / sqrtf(group_sum<NT>(ss, sm[1]) * inv_n + a.eps);
+  const float rstd = rsqrtf(group_sum<NT>(ss, sm[1]) * inv_n + a.eps);
   if (t == 0) {
     if (a.mean_out) a.mean_out[row] = mu;
     if (a.rstd_out) a.rstd_out[row] = rstd;
@@ -103,6 +116,102 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_forward(const LnArgs a) {
       Raw<T, VEC> o;
       pack(v, o);
       raw_store<T, VEC>(dst + c, o);
+    }
+  }
+}
+
+// Parameters in shared memory, laid out so that the float4 h of a thread's
+// vectors are NT apart: conflict-free for VEC = 8, where global loads would
+// step 32 bytes per lane.
+template <int VEC, int VPT, int NT>
+__device__ __forceinline__ void params_to_smem(float4 *s, const float *g, uint32_t cols, uint32_t t) {
+#pragma unroll
+  for (int j = 0; j < VPT; j++) {
+    const uint32_t i = t + j * NT, c = i * VEC;
+    if (c < cols) {
+#pragma unroll
+      for (int h = 0; h < VEC / 4; h++) s[h * VPT * NT + i] = *reinterpret_cast<const float4 *>(g + c + 4 * h);
+    }
+  }
+}
+template <int VEC, int VPT, int NT>
+__device__ __forceinline__ void params_from_smem(const float4 *s, int j, uint32_t t, float (&f)[VEC]) {
+#pragma unroll
+  for (int h = 0; h < VEC / 4; h++) {
+    const float4 v = s[h * VPT * NT + t + j * NT];
+    f[4 * h] = v.x, f[4 * h + 1] = v.y, f[4 * h + 2] = v.z, f[4 * h + 3] = v.w;
+  }
+}
+
+// One CTA per row at a time, persistent, the next row in flight.
+template <typename T, int VEC, int VPT, int NT, int MIN_CTAS>
+__global__ void __launch_bounds__(NT, MIN_CTAS) ln_forward_stream(const LnArgs a) {
+  constexpr int NW = NT / 32;
+  extern __shared__ __align__(16) float4 ps[];  // gamma, beta
+  __shared__ float sm[2][2][NW];
+  const float4 *gs = ps, *bs = ps + VPT * NT * VEC / 4;
+  const uint32_t t = threadIdx.x;
+  params_to_smem<VEC, VPT, NT>(ps, a.gamma, a.cols, t);  // each thread reads back what it wrote
+  params_to_smem<VEC, VPT, NT>(ps + VPT * NT * VEC / 4, a.beta, a.cols, t);
+  const float inv_n = 1.0f / float(a.cols);
+  Raw<T, VEC> raw[VPT], next[VPT];
+  auto load = [&](uint64_t r) {
+    const T *src = static_cast<const T *>(a.in) + r * a.cols;
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      const uint32_t c = (t + j * NT) * VEC;
+      next[j] = c < a.cols ? raw_load<T, VEC>(src + c) : raw_zero<T, VEC>();
+    }
+  };
+  uint64_t row = blockIdx.x;
+  if (row < a.rows) load(row);
+  for (int b = 0; row < a.rows; row += gridDim.x, b ^= 1) {
+#pragma unroll
+    for (int j = 0; j < VPT; j++) raw[j] = next[j];
+    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      float v[VEC];
+      unpack(raw[j], v);
+#pragma unroll
+      for (int k = 0; k < VEC; k++) s += v[k];
+    }
+    // buffer b: its last readers have passed the two barriers of the row between
+    const float mu = group_sum<NT>(s, sm[b][0]) * inv_n;
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      if ((t + j * NT) * VEC < a.cols) {
+        float v[VEC];
+        unpack(raw[j], v);
+#pragma unroll
+        for (int k = 0; k < VEC; k++) {
+          const float d = v[k] - mu;
+          ss = fmaf(d, d, ss);
+        }
+      }
+    }
+    const float rstd = rsqrtf(group_sum<NT>(ss, sm[b][1]) * inv_n + a.eps);
+    if (t == 0) {
+      if (a.mean_out) a.mean_out[row] = mu;
+      if (a.rstd_out) a.rstd_out[row] = rstd;
+    }
+    T *dst = static_cast<T *>(a.out) + row * a.cols;
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      const uint32_t c = (t + j * NT) * VEC;
+      if (c < a.cols) {
+        float v[VEC], gm[VEC], bt[VEC];
+        unpack(raw[j], v);
+        params_from_smem<VEC, VPT, NT>(gs, j, t, gm);
+        params_from_smem<VEC, VPT, NT>(bs, j, t, bt);
+#pragma unroll
+        for (int k = 0; k < VEC; k++) v[k] = fmaf((v[k] - mu) * rstd, gm[k], bt[k]);
+        Raw<T, VEC> o;
+        pack(v, o);
+        raw_store<T, VEC>(dst + c, o);
+      }
     }
   }
 }
@@ -130,7 +239,7 @@ __global__ void __launch_bounds__(512) ln_forward_long(const LnArgs a) {
     const float d = at(c) - mu;
     ss = fmaf(d, d, ss);
   }
-  const float rstd = 1.0f / sqrtf(group_sum<512>(ss, sm[1]) * inv_n + a.eps);
+  const float rstd = rsqrtf(group_sum<512>(ss, sm[1]) * inv_n + a.eps);
   if (threadIdx.x == 0) {
     if (a.mean_out) a.mean_out[row] = mu;
     if (a.rstd_out) a.rstd_out[row] = rstd;
@@ -166,17 +275,37 @@ struct LnRow {
   }
 };
 
+// Rows of more than 8192 columns (32 elements a thread) have no registers for
+// the sums and the next row: the sums then live in shared memory.
+template <int VEC, int VPT, int NT, int GROUPS>
+struct BwdCfg {
+  static constexpr int E = VEC * VPT;
+  static constexpr bool WIDE = E == 32;
+  static constexpr bool PARAMS = VEC == 8;  // gamma in shared memory
+  static constexpr int PARAM_FLOATS = PARAMS ? E * NT : 0;
+  static constexpr bool ACC_S = WIDE || GROUPS > 1;
+  static uint32_t smem(uint32_t cols) { return (PARAM_FLOATS + (ACC_S ? 2 * cols : 0)) * sizeof(float); }
+};
+
 template <typename T, int VEC, int VPT, int NT, int GROUPS, bool RES>
 __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
+  using Cfg = BwdCfg<VEC, VPT, NT, GROUPS>;
   constexpr int NW = NT / 32, E = VPT * VEC;
-  constexpr bool WARP = NT == 32;
-  extern __shared__ __align__(16) float acc_s[];  // dgamma[cols], dbeta[cols] of this CTA
+  constexpr bool WARP = NT == 32, ACCREG = !Cfg::WIDE, PF = !Cfg::WIDE;
+  extern __shared__ __align__(16) float dyn[];
+  float *acc_s = dyn + Cfg::PARAM_FLOATS;  // dgamma[cols], dbeta[cols] of this CTA
+  const float4 *gs = reinterpret_cast<const float4 *>(dyn);
   __shared__ float2 sm[2][NW];
   const uint32_t t = threadIdx.x % NT, g = threadIdx.x / NT;
-  float ag[WARP ? E : 1], ab[WARP ? E : 1];
-  if (WARP) {
+  auto gamma_at = [&](int j, float(&f)[VEC]) {
+    if constexpr (Cfg::PARAMS) params_from_smem<VEC, VPT, NT>(gs, j, t, f);
+    else load_f32<VEC>(a.gamma + (t + j * NT) * VEC, f);
+  };
+  if constexpr (Cfg::PARAMS) params_to_smem<VEC, VPT, NT>(reinterpret_cast<float4 *>(dyn), a.gamma, a.cols, t);
+  float ag[ACCREG ? E : 1], ab[ACCREG ? E : 1];
+  if (ACCREG) {
 #pragma unroll
-    for (int i = 0; i < E; i++) ag[i] = ab[i] = 0.f;
+    for (int i = 0; i < E; i++) ag[ACCREG ? i : 0] = ab[ACCREG ? i : 0] = 0.f;
   } else {
     for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NT * GROUPS) acc_s[c] = 0.f;
     __syncthreads();
@@ -184,9 +313,16 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
   const float inv_n = 1.0f / float(a.cols);
   const uint64_t step = uint64_t(gridDim.x) * GROUPS;
   int buf = 0;
-  for (uint64_t row = uint64_t(blockIdx.x) * GROUPS + g; row < a.rows; row += step) {
-    LnRow<T, VEC, VPT, NT, RES> r;
-    r.load(a, row, t);
+  LnRow<T, VEC, VPT, NT, RES> r, next;
+  uint64_t row = uint64_t(blockIdx.x) * GROUPS + g;
+  if (PF && row < a.rows) next.load(a, row, t);
+  for (; row < a.rows; row += step) {
+    if (PF) {
+      r = next;
+      if (row + step < a.rows) next.load(a, row + step, t);
+    } else {
+      r.load(a, row, t);
+    }
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
@@ -195,8 +331,8 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
         float x[VEC], dy[VEC], gm[VEC], sg[VEC], sb[VEC];
         unpack(r.x[j], x);
         unpack(r.dy[j], dy);
-        load_f32<VEC>(a.gamma + c, gm);
-        if (!WARP) {
+        gamma_at(j, gm);
+        if (!ACCREG) {
           load_f32<VEC>(acc_s + c, sg);
           load_f32<VEC>(acc_s + a.cols + c, sb);
         }
@@ -206,15 +342,16 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
           const float w = dy[k] * gm[k];
           c1 += w;
           c2 = fmaf(w, xh, c2);
-          if (WARP) {
-            ag[j * VEC + k] = fmaf(dy[k], xh, ag[j * VEC + k]);
-            ab[j * VEC + k] += dy[k];
+          if (ACCREG) {
+            const int i = ACCREG ? j * VEC + k : 0;
+            ag[i] = fmaf(dy[k], xh, ag[i]);
+            ab[i] += dy[k];
           } else {
             sg[k] = fmaf(dy[k], xh, sg[k]);
             sb[k] += dy[k];
           }
         }
-        if (!WARP) {
+        if (!ACCREG) {
           store_f32<VEC>(acc_s + c, sg);
           store_f32<VEC>(acc_s + a.cols + c, sb);
         }
@@ -243,7 +380,7 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
         float x[VEC], dy[VEC], gm[VEC], res[VEC];
         unpack(r.x[j], x);
         unpack(r.dy[j], dy);
-        load_f32<VEC>(a.gamma + c, gm);
+        gamma_at(j, gm);
         if (RES) unpack(r.res[RES ? j : 0], res);
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
@@ -258,7 +395,26 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
       }
     }
   }
-  if (WARP) {  // the CTA's warps add their sums in warp order
+  float *part = a.part + uint64_t(blockIdx.x) * 2 * a.cols;
+  if (ACCREG && GROUPS == 1) {
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      const uint32_t c = (t + j * NT) * VEC;
+      if (c < a.cols) {
+        float sg[VEC], sb[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; k++) {
+          const int i = ACCREG ? j * VEC + k : 0;
+          sg[k] = ag[i];
+          sb[k] = ab[i];
+        }
+        store_f32<VEC>(part + c, sg);
+        store_f32<VEC>(part + a.cols + c, sb);
+      }
+    }
+    return;
+  }
+  if (ACCREG) {  // the CTA's groups add their sums in order
 #pragma unroll 1
     for (int w = 0; w < GROUPS; w++) {
       if (int(g) == w) {
@@ -268,7 +424,7 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
           if (c < a.cols) {
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
-              const int i = j * VEC + k;
+              const int i = ACCREG ? j * VEC + k : 0;
               acc_s[c + k] = w ? acc_s[c + k] + ag[i] : ag[i];
               acc_s[a.cols + c + k] = w ? acc_s[a.cols + c + k] + ab[i] : ab[i];
             }
@@ -280,7 +436,6 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
   } else {
     __syncthreads();
   }
-  float *part = a.part + uint64_t(blockIdx.x) * 2 * a.cols;
   for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NT * GROUPS) part[c] = acc_s[c];
 }
 
@@ -336,42 +491,73 @@ __global__ void __launch_bounds__(512) ln_backward_long(const LnArgs a) {
   }
 }
 
-// dgamma / dbeta: the partial rows added in CTA order, in 8 interleaved
-// slices per column that then add in slice order.
-__global__ void __launch_bounds__(256) ln_finish(const float *__restrict__ part, uint32_t nparts, uint32_t cols,
-                                                 float *__restrict__ dgamma, float *__restrict__ dbeta) {
-  __shared__ float sm[8][33];
+// dgamma / dbeta: the partial rows added in CTA order, in 32 interleaved
+// slices per column (one warp each) that then add in slice order.
+__global__ void __launch_bounds__(1024) ln_finish(const float *__restrict__ part, uint32_t nparts, uint32_t cols,
+                                                  float *__restrict__ dgamma, float *__restrict__ dbeta) {
+  __shared__ float sm[32][33];
   const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const uint32_t c = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (c < 2 * cols) {
 #pragma unroll 8
-    for (uint32_t i = slice; i < nparts; i += 8) s += __ldcs(part + uint64_t(i) * 2 * cols + c);
+    for (uint32_t i = slice; i < nparts; i += 32) s += __ldcs(part + uint64_t(i) * 2 * cols + c);
   }
   sm[slice][lane] = s;
   __syncthreads();
   if (slice == 0 && c < 2 * cols) {
 #pragma unroll
-    for (int i = 1; i < 8; i++) s += sm[i][lane];
+    for (int i = 1; i < 32; i++) s += sm[i][lane];
     if (c < cols) dgamma[c] = s;
     else dbeta[c - cols] = s;
   }
 }
 
 // --------------------------------------------------------------------- host
-// Calls f.run<VEC, VPT, NT, GROUPS>() for a row of `cols`: the fewest
-// registers that hold it.  VEC is the vector width, 1 for unaligned rows.
+// Calls f.run<VEC, VPT, NT, GROUPS>() with NT threads of VEC * VPT elements for
+// a row of `cols`.
 template <int VEC, typename F>
-silcu_status by_cols(uint32_t cols, F &&f) {
-  constexpr int V = VEC == 1 ? 1 : VEC;
-  if (cols <= 32 * 8) return f.template run<V, 8 / V, 32, 8>();
-  if (cols <= 32 * 16) return f.template run<V, 16 / V, 32, 8>();
-  if (cols <= 32 * 24) return f.template run<V, 24 / V, 32, 8>();
-  if (cols <= 32 * 32) return f.template run<V, 32 / V, 32, 8>();
-  if (cols <= 128 * 16) return f.template run<V, 16 / V, 128, 1>();
-  if (cols <= 256 * 16) return f.template run<V, 16 / V, 256, 1>();
-  if (cols <= 512 * 16) return f.template run<V, 16 / V, 512, 1>();
-  return f.template run<V, 32 / V, 512, 1>();
+silcu_status by_cols_forward(uint32_t cols, F &&f) {
+  if (cols <= 32 * 8) return f.template run<VEC, 8 / VEC, 32, 8>();
+  if (cols <= 64 * 8) return f.template run<VEC, 8 / VEC, 64, 1>();
+  if (cols <= 96 * 8) return f.template run<VEC, 8 / VEC, 96, 1>();
+  if (cols <= 128 * 8) return f.template run<VEC, 8 / VEC, 128, 1>();
+  if (cols <= 128 * 16) return f.template run<VEC, 16 / VEC, 128, 1>();
+  if (cols <= 256 * 16) return f.template run<VEC, 16 / VEC, 256, 1>();
+  if (cols <= 512 * 16) return f.template run<VEC, 16 / VEC, 512, 1>();
+  return f.template run<VEC, 32 / VEC, 512, 1>();
+}
+
+// Measured for 16384 x 768: 192 threads of 4 fp32 elements 34 us, 96 of 8 35;
+// bf16 96 of 8 21 us, a warp of 24 33.
+template <int VEC, typename F>
+auto by_cols_backward(uint32_t cols, F &&f) {
+  if (cols <= 32 * 8) return f.template run<VEC, 8 / VEC, 32, 8>();
+  if constexpr (VEC <= 4) {
+    if (cols <= 128 * 4) return f.template run<VEC, 4 / VEC, 128, 1>();
+    if (cols <= 192 * 4) return f.template run<VEC, 4 / VEC, 192, 1>();
+    if (cols <= 128 * 8) return f.template run<VEC, 8 / VEC, 128, 1>();
+    if (cols <= 256 * 8) return f.template run<VEC, 8 / VEC, 256, 1>();
+  } else {
+    if (cols <= 64 * 8) return f.template run<VEC, 1, 64, 1>();
+    if (cols <= 96 * 8) return f.template run<VEC, 1, 96, 1>();
+    if (cols <= 64 * 16) return f.template run<VEC, 2, 64, 1>();
+    if (cols <= 128 * 16) return f.template run<VEC, 2, 128, 1>();
+  }
+  if (cols <= 256 * 16) return f.template run<VEC, 16 / VEC, 256, 1>();
+  if (cols <= 512 * 16) return f.template run<VEC, 16 / VEC, 512, 1>();
+  return f.template run<VEC, 32 / VEC, 512, 1>();
+}
+
+template <typename K>
+silcu_status allow_smem(K kernel, uint32_t bytes, bool (&configured)[64], const char *what) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && configured[dev]) return SILCU_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+  if (dev >= 0 && dev < 64) configured[dev] = true;
+  return SILCU_OK;
 }
 
 template <typename T>
@@ -384,38 +570,54 @@ struct Forward {
     ln_forward<T, VEC, VPT, NT, GROUPS><<<uint32_t(grid), NT * GROUPS, 0, s>>>(a);
     return check_launch("layer_norm_forward");
   }
+  // CTAS per SM fill the registers (64 to 94 a thread).
+  template <int VPT, int NT, int CTAS>
+  silcu_status stream() {
+    constexpr uint32_t smem = VPT * NT * 8 * 2 * sizeof(float);
+    static bool configured[64] = {false};
+    const silcu_status st =
+        allow_smem(ln_forward_stream<T, 8, VPT, NT, CTAS>, smem, configured, "layer_norm_forward");
+    if (st != SILCU_OK) return st;
+    const uint64_t cap = uint64_t(sm_count()) * CTAS;
+    ln_forward_stream<T, 8, VPT, NT, CTAS><<<uint32_t(a.rows < cap ? a.rows : cap), NT, smem, s>>>(a);
+    return check_launch("layer_norm_forward");
+  }
 };
 
-// CTAs of the persistent backward grid: enough to fill the SMs, never more
-// than the groups of rows there are.  The workspace holds one partial row pair
-// for each.
-constexpr int kBwdCtasPerSm = 4;
-uint32_t bwd_ctas(uint64_t rows, uint32_t cols) {
-  const uint64_t groups = cols <= 1024 ? (rows + 7) / 8 : rows;
-  const uint64_t cap = uint64_t(sm_count()) * (cols <= kMaxRegCols ? kBwdCtasPerSm : 1);
-  return uint32_t(groups < cap ? groups : cap);
+// CTAs of the persistent backward grid: as many as the registers hold, two
+// rows or more for each where that still fills the SMs (every CTA's partial
+// row is written and read again).  The workspace holds one for each.
+struct BackwardGrid {
+  uint64_t rows;
+  template <int VEC, int VPT, int NT, int GROUPS>
+  uint32_t run() const {
+    constexpr int E = VEC * VPT, threads = E == 4 ? 1152 : E == 8 ? 768 : E == 16 ? (NT <= 128 ? 640 : 512) : 512;
+    constexpr int per_sm = threads / (NT * GROUPS);
+    const uint64_t sms = uint64_t(sm_count()), groups = (rows + GROUPS - 1) / GROUPS;
+    uint64_t g = groups / 2 > sms ? groups / 2 : sms;
+    if (g > groups) g = groups;
+    return uint32_t(g < sms * per_sm ? g : sms * per_sm);
+  }
+};
+uint32_t long_grid(uint64_t rows) {
+  const uint64_t sms = uint64_t(sm_count());
+  return uint32_t(rows < sms ? rows : sms);
 }
 
 template <typename T, bool RES>
 struct Backward {
   LnArgs a;
-  uint32_t grid;
   cudaStream_t s;
+  uint32_t *grid;  // its number of partial rows
   template <int VEC, int VPT, int NT, int GROUPS>
   silcu_status run() {
-    const uint32_t smem = 2 * a.cols * sizeof(float);
+    using Cfg = BwdCfg<VEC, VPT, NT, GROUPS>;
     static bool configured[64] = {false};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (smem > 48 * 1024 - 1024 && dev >= 0 && dev < 64 && !configured[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(ln_backward<T, VEC, VPT, NT, GROUPS, RES>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 int(2 * kMaxRegCols * sizeof(float)));
-      if (e != cudaSuccess)
-        return fail(SILCU_CUDA_ERROR, "layer_norm_backward: smem attribute: %s", cudaGetErrorString(e));
-      configured[dev] = true;
-    }
-    ln_backward<T, VEC, VPT, NT, GROUPS, RES><<<grid, NT * GROUPS, smem, s>>>(a);
+    const auto kernel = ln_backward<T, VEC, VPT, NT, GROUPS, RES>;
+    const silcu_status st = allow_smem(kernel, Cfg::smem(Cfg::E * NT), configured, "layer_norm_backward");
+    if (st != SILCU_OK) return st;
+    *grid = BackwardGrid{a.rows}.run<VEC, VPT, NT, GROUPS>();
+    kernel<<<*grid, NT * GROUPS, Cfg::smem(a.cols), s>>>(a);
     return check_launch("layer_norm_backward");
   }
 };
@@ -427,23 +629,39 @@ silcu_status forward(const LnArgs &a, cudaStream_t s) {
     ln_forward_long<T><<<uint32_t(a.rows), 512, 0, s>>>(a);
     return check_launch("layer_norm_forward");
   }
-  if (a.cols % V == 0 && aligned16(a.in) && aligned16(a.out) && aligned16(a.gamma) && aligned16(a.beta))
-    return by_cols<V>(a.cols, Forward<T>{a, s});
-  return by_cols<1>(a.cols, Forward<T>{a, s});
+  Forward<T> f{a, s};
+  const bool vec = a.cols % V == 0 && aligned16(a.in) && aligned16(a.out) && aligned16(a.gamma) && aligned16(a.beta);
+  if constexpr (V == 8) {
+    if (vec) {
+      if (a.cols <= 256) return f.template stream<1, 32, 28>();
+      if (a.cols <= 512) return f.template stream<2, 32, 24>();
+      if (a.cols <= 768) return f.template stream<3, 32, 20>();
+      if (a.cols <= 1024) return f.template stream<4, 32, 16>();
+      if (a.cols <= 2048) return f.template stream<4, 64, 10>();
+      if (a.cols <= 4096) return f.template stream<4, 128, 5>();
+      if (a.cols <= 8192) return f.template stream<4, 256, 3>();
+      return f.template stream<4, 512, 1>();
+    }
+  } else {
+    if (vec) return by_cols_forward<V>(a.cols, f);
+  }
+  return by_cols_forward<1>(a.cols, f);
 }
 
 template <typename T, bool RES>
-silcu_status backward(const LnArgs &a, uint32_t grid, cudaStream_t s) {
+silcu_status backward(const LnArgs &a, cudaStream_t s, uint32_t *grid) {
   constexpr int V = 16 / sizeof(T);
   if (a.cols > kMaxRegCols) {
-    ln_backward_cols<T><<<dim3((a.cols + 255) / 256, grid), 256, 0, s>>>(a);
+    *grid = long_grid(a.rows);
+    ln_backward_cols<T><<<dim3((a.cols + 255) / 256, *grid), 256, 0, s>>>(a);
     ln_backward_long<T, RES><<<uint32_t(a.rows), 512, 0, s>>>(a);
     return check_launch("layer_norm_backward", 2);
   }
+  Backward<T, RES> f{a, s, grid};
   if (a.cols % V == 0 && aligned16(a.in) && aligned16(a.dout) && aligned16(a.out) && aligned16(a.gamma) &&
-      (!RES || aligned16(a.dres)))
-    return by_cols<V>(a.cols, Backward<T, RES>{a, grid, s});
-  return by_cols<1>(a.cols, Backward<T, RES>{a, grid, s});
+      aligned16(a.part) && (!RES || aligned16(a.dres)))
+    return by_cols_backward<V>(a.cols, f);
+  return by_cols_backward<1>(a.cols, f);
 }
 
 silcu_status check_extent(const char *what, size_t rows, size_t cols, int dtype) {
@@ -479,10 +697,20 @@ silcu_status silcu_layer_norm_forward(const void *in, void *out, float *mean, fl
   return dtype == SILCU_BF16 ? forward<__nv_bfloat16>(a, as_stream(stream)) : forward<float>(a, as_stream(stream));
 }
 
-size_t silcu_layer_norm_backward_workspace_bytes(size_t rows, size_t cols, int) {
+size_t silcu_layer_norm_backward_workspace_bytes(size_t rows, size_t cols, int dtype) {
   using namespace silcu;
   if (rows == 0 || cols == 0 || rows > 0x7FFFFFFFull || cols > (1u << 24)) return 0;
-  return size_t(bwd_ctas(rows, uint32_t(cols))) * 2 * cols * sizeof(float);
+  const uint32_t c = uint32_t(cols);
+  uint32_t grid;
+  if (c > kMaxRegCols) {
+    grid = long_grid(rows);
+  } else {  // the larger of the vector and the element-wise variant: alignment is known at the call
+    const BackwardGrid g{rows};
+    const uint32_t v = dtype == SILCU_BF16 ? by_cols_backward<8>(c, g) : by_cols_backward<4>(c, g);
+    const uint32_t e = by_cols_backward<1>(c, g);
+    grid = v > e ? v : e;
+  }
+  return size_t(grid) * 2 * cols * sizeof(float);
 }
 
 silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const float *mean, const float *rstd,
@@ -494,7 +722,7 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
   if (st != SILCU_OK) return st;
   if (!dgamma || !dbeta) return fail(SILCU_INVALID_ARGUMENT, "layer_norm_backward: null pointer");
   cudaStream_t s = as_stream(stream);
-  const uint32_t grid = rows ? bwd_ctas(rows, uint32_t(cols)) : 0;
+  uint32_t grid = 0;
   if (rows) {
     if (!dout || !in || !mean || !rstd || !gamma || !din)
       return fail(SILCU_INVALID_ARGUMENT, "layer_norm_backward: null pointer");
@@ -515,12 +743,12 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
     a.rows = rows;
     a.cols = uint32_t(cols);
     if (dtype == SILCU_BF16)
-      st = dresidual ? backward<__nv_bfloat16, true>(a, grid, s) : backward<__nv_bfloat16, false>(a, grid, s);
+      st = dresidual ? backward<__nv_bfloat16, true>(a, s, &grid) : backward<__nv_bfloat16, false>(a, s, &grid);
     else
-      st = dresidual ? backward<float, true>(a, grid, s) : backward<float, false>(a, grid, s);
+      st = dresidual ? backward<float, true>(a, s, &grid) : backward<float, false>(a, s, &grid);
     if (st != SILCU_OK) return st;
   }
-  ln_finish<<<uint32_t((2 * cols + 31) / 32), 256, 0, s>>>(static_cast<const float *>(workspace), grid,
+  ln_finish<<<uint32_t((2 * cols + 31) / 32), 1024, 0, s>>>(static_cast<const float *>(workspace), grid,
                                                            uint32_t(cols), dgamma, dbeta);
   return check_launch("layer_norm_backward finish");
 }

@@ -463,79 +463,72 @@ def sgemv(x, W, y, N, K, bias=None):
 
 
 # ------------------------------------------------------------------- training
+# These calls are short next to a Python call's own cost, so operands are
+# checked and turned into addresses in one step each.
 DTYPE = {_F32: 0, torch.bfloat16: 1}
+REDUCTION = {"mean": 0, "sum": 1, "none": 2}
 
 
-def _floats(*ts):
-    """Contiguous CUDA tensors of one dtype (fp32 or bf16) and device."""
-    first = None
-    for t in ts:
-        if t is None:
-            continue
+def _kind(t):
+    """The silcu_dtype of a CUDA tensor."""
+    k = DTYPE.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if k is None or not t.is_cuda:
         _dev(t)
-        if t.dtype not in DTYPE:
-            raise TypeError(f"silarray_b200.gpu: expected float32 or bfloat16, got {t.dtype}")
-        if first is None:
-            first = t
-        elif t.dtype != first.dtype:
-            raise TypeError(f"silarray_b200.gpu: {first.dtype} and {t.dtype} operands mixed")
-    return DTYPE[first.dtype]
+        raise TypeError(f"silarray_b200.gpu: expected float32 or bfloat16, got {t.dtype}")
+    return k
 
 
-def _same_device(first, *ts):
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"silarray_b200.gpu: operands on {first.device} and {t.device}")
+def _at(what, t, dtype, n, index):
+    """Address of a contiguous tensor of n elements of dtype on GPU `index`."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.numel() == n \
+            and t.is_contiguous():
+        return t.data_ptr()
+    _dev(t, dtype)
+    if t.get_device() != index:
+        raise ValueError(f"{what}: on cuda:{t.get_device()}, expected cuda:{index}")
+    raise ValueError(f"{what}: expected {n} elements, got {t.numel()}")
 
 
-def _sized(name, t, n):
-    if t is not None and t.numel() != n:
-        raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
-    return t
+def _scratch(nbytes, device):
+    """Scratch of one call (the tensor and its address).  It comes from torch's
+    caching allocator each time, so calls on several streams or in several
+    captured graphs never share it."""
+    if nbytes == 0:
+        return None, None
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return buf, buf.data_ptr()
 
 
-class _on:
-    """Runs a call on its operands' device: (stream of that device, scratch of
-    nbytes).  The scratch comes from torch's caching allocator for each call,
-    so calls on several streams or in several captured graphs never share it."""
-
-    def __init__(self, device, nbytes=0):
-        self.device, self.nbytes = device, nbytes
-        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device) if self.nbytes else None
-        return _p(self.ws), self.nbytes, _stream()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(fn, index, *args):
+    """fn(*args, stream) on GPU `index` and its current stream."""
+    if torch._C._cuda_getDevice() == index:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _rows_cols(IN, rows, cols):
     if rows is None:
         cols = IN.shape[-1]
         rows = IN.numel() // cols if cols else 0
-    if rows * cols != IN.numel():
-        raise ValueError(f"layer_norm: {rows} x {cols} rows in {IN.numel()} elements")
     return rows, cols
 
 
 def layer_norm_forward(IN, OUT=None, gamma=None, beta=None, rows=None, cols=None, eps=1e-5):
     """layer_norm (fp32 or bf16 rows, fp32 gamma and beta) that also returns the
     statistics its backward pass needs: (OUT, mean[rows], rstd[rows])."""
-    dt = _floats(IN, OUT)
+    dt = _kind(IN)
     rows, cols = _rows_cols(IN, rows, cols)
-    _sized("layer_norm gamma", _dev(gamma, _F32), cols), _sized("layer_norm beta", _dev(beta, _F32), cols)
-    OUT = torch.empty_like(IN) if OUT is None else _sized("layer_norm OUT", OUT, rows * cols)
-    _same_device(IN, OUT, gamma, beta)
-    stats = torch.empty(2, rows, dtype=_F32, device=IN.device)
-    mean, rstd = stats[0], stats[1]
-    with _on(IN.device) as (_, _, stream):
-        check(lib().silcu_layer_norm_forward(_p(IN), _p(OUT), _p(mean), _p(rstd), _p(gamma), _p(beta), rows, cols,
-                                             float(eps), dt, stream))
+    n, index = rows * cols, IN.get_device()
+    x = _at("layer_norm IN", IN, IN.dtype, n, index)
+    g = _at("layer_norm gamma", gamma, _F32, cols, index)
+    b = _at("layer_norm beta", beta, _F32, cols, index)
+    OUT = torch.empty_like(IN) if OUT is None else OUT
+    mean = torch.empty(rows, dtype=_F32, device=IN.device)
+    rstd = torch.empty(rows, dtype=_F32, device=IN.device)
+    _launch(lib().silcu_layer_norm_forward, index, x, _at("layer_norm OUT", OUT, IN.dtype, n, index),
+            mean.data_ptr(), rstd.data_ptr(), g, b, rows, cols, eps, dt)
     return OUT, mean, rstd
 
 
@@ -543,53 +536,54 @@ def layer_norm_backward(dout, IN, mean, rstd, gamma, dresidual=None, din=None, d
                         rows=None, cols=None):
     """Gradients of layer_norm_forward: (din, dgamma, dbeta).  dresidual, when
     given, is added to din (the gradient that bypasses the norm)."""
-    dt = _floats(IN, dout, dresidual, din)
+    dt = _kind(IN)
     rows, cols = _rows_cols(IN, rows, cols)
-    n = rows * cols
-    _sized("layer_norm dout", dout, n), _sized("layer_norm dresidual", dresidual, n)
-    _sized("layer_norm mean", _dev(mean, _F32), rows), _sized("layer_norm rstd", _dev(rstd, _F32), rows)
-    _sized("layer_norm gamma", _dev(gamma, _F32), cols)
-    din = torch.empty_like(IN) if din is None else _sized("layer_norm din", din, n)
-    if dgamma is None:
-        dgamma = torch.empty(cols, dtype=_F32, device=IN.device)
-    if dbeta is None:
-        dbeta = torch.empty(cols, dtype=_F32, device=IN.device)
-    _sized("layer_norm dgamma", _dev(dgamma, _F32), cols), _sized("layer_norm dbeta", _dev(dbeta, _F32), cols)
-    _same_device(IN, dout, mean, rstd, gamma, dresidual, din, dgamma, dbeta)
-    with _on(IN.device, lib().silcu_layer_norm_backward_workspace_bytes(rows, cols, dt)) as (wp, wn, stream):
-        check(lib().silcu_layer_norm_backward(_p(dout), _p(IN), _p(mean), _p(rstd), _p(gamma), _p(dresidual),
-                                              _p(din), _p(dgamma), _p(dbeta), rows, cols, dt, wp, wn, stream))
+    n, index, t = rows * cols, IN.get_device(), IN.dtype
+    ops = (_at("layer_norm dout", dout, t, n, index), _at("layer_norm IN", IN, t, n, index),
+           _at("layer_norm mean", mean, _F32, rows, index), _at("layer_norm rstd", rstd, _F32, rows, index),
+           _at("layer_norm gamma", gamma, _F32, cols, index),
+           None if dresidual is None else _at("layer_norm dresidual", dresidual, t, n, index))
+    din = torch.empty_like(IN) if din is None else din
+    dgamma = torch.empty(cols, dtype=_F32, device=IN.device) if dgamma is None else dgamma
+    dbeta = torch.empty(cols, dtype=_F32, device=IN.device) if dbeta is None else dbeta
+    nbytes = lib().silcu_layer_norm_backward_workspace_bytes(rows, cols, dt)
+    buf, ws = _scratch(nbytes, IN.device)
+    _launch(lib().silcu_layer_norm_backward, index, *ops, _at("layer_norm din", din, t, n, index),
+            _at("layer_norm dgamma", dgamma, _F32, cols, index), _at("layer_norm dbeta", dbeta, _F32, cols, index),
+            rows, cols, dt, ws, nbytes)
     return din, dgamma, dbeta
 
 
-REDUCTION = {"mean": 0, "sum": 1, "none": 2}
-
-
-def _matrix(name, t, rows=None, cols=None, dtype=None):
-    """A 2-D fp32 / bf16 CUDA tensor with contiguous rows; its row stride."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError("silarray_b200.gpu: operands must be CUDA tensors (no CPU fallback)")
-    if t.dtype not in DTYPE or (dtype is not None and t.dtype != dtype):
-        raise TypeError(f"{name}: expected {dtype or 'float32 or bfloat16'}, got {t.dtype}")
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{name}: bad shape {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}: rows must be contiguous and apart")
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+def _matrix(what, t, rows, cols, dtype, index):
+    """Address and row stride of a 2-D tensor with contiguous rows."""
+    if t.dtype is not dtype or not t.is_cuda:
+        if not t.is_cuda:
+            _dev(t)
+        raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{what}: on cuda:{t.get_device()}, expected cuda:{index}")
+    if t.dim() != 2 or t.shape != (rows, cols):
+        raise ValueError(f"{what}: expected shape {(rows, cols)}, got {tuple(t.shape)}")
+    ld = t.stride(0) if rows > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise ValueError(f"{what}: rows must be contiguous and apart")
+    return t.data_ptr(), ld
 
 
 def _cross_entropy_args(H, W, targets, lse, reduction):
     if reduction not in REDUCTION:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
     a = _lib.CrossEntropyArgs()
-    a.ldh = _matrix("linear_cross_entropy H", H)
-    a.ldw = _matrix("linear_cross_entropy W", W, cols=H.shape[1], dtype=H.dtype)
-    _sized("linear_cross_entropy targets", _dev(targets, _I32), H.shape[0])
-    _sized("linear_cross_entropy lse", _dev(lse, _F32), H.shape[0])
-    a.H, a.W, a.targets, a.lse = H.data_ptr(), W.data_ptr(), targets.data_ptr(), lse.data_ptr()
-    a.rows, a.V, a.D = H.shape[0], W.shape[0], H.shape[1]
-    a.dtype, a.reduction = DTYPE[H.dtype], REDUCTION[reduction]
-    return a
+    a.dtype, a.reduction = _kind(H), REDUCTION[reduction]
+    if H.dim() != 2 or W.dim() != 2:
+        raise ValueError("linear_cross_entropy: H and W must be matrices")
+    (rows, D), V, index = H.shape, W.shape[0], H.get_device()
+    a.rows, a.V, a.D = rows, V, D
+    a.H, a.ldh = _matrix("linear_cross_entropy H", H, rows, D, H.dtype, index)
+    a.W, a.ldw = _matrix("linear_cross_entropy W", W, V, D, H.dtype, index)
+    a.targets = _at("linear_cross_entropy targets", targets, _I32, rows, index)
+    a.lse = _at("linear_cross_entropy lse", lse, _F32, rows, index)
+    return a, index
 
 
 def linear_cross_entropy(H, W, targets, reduction="mean", loss=None, lse=None):
@@ -599,15 +593,14 @@ def linear_cross_entropy(H, W, targets, reduction="mean", loss=None, lse=None):
     the rows that count) or sum as a 0-d tensor, or [rows] for "none"; lse
     [rows] is what the backward pass needs."""
     n = H.shape[0]
-    if lse is None:
-        lse = torch.empty(n, dtype=_F32, device=H.device)
-    a = _cross_entropy_args(H, W, targets, lse, reduction)
-    if loss is None:
-        loss = torch.empty(n if reduction == "none" else (), dtype=_F32, device=H.device)
-    a.loss = _sized("linear_cross_entropy loss", _dev(loss, _F32), n if reduction == "none" else 1).data_ptr()
-    _same_device(H, W, targets, loss, lse)
-    with _on(H.device, lib().silcu_linear_cross_entropy_workspace_bytes(ct.byref(a), 0)) as (wp, wn, stream):
-        check(lib().silcu_linear_cross_entropy(ct.byref(a), wp, wn, stream))
+    lse = torch.empty(n, dtype=_F32, device=H.device) if lse is None else lse
+    a, index = _cross_entropy_args(H, W, targets, lse, reduction)
+    each = reduction == "none"
+    loss = torch.empty(n if each else (), dtype=_F32, device=H.device) if loss is None else loss
+    a.loss = _at("linear_cross_entropy loss", loss, _F32, n if each else 1, index)
+    nbytes = lib().silcu_linear_cross_entropy_workspace_bytes(a, 0)
+    buf, ws = _scratch(nbytes, H.device)
+    _launch(lib().silcu_linear_cross_entropy, index, a, ws, nbytes)
     return loss, lse
 
 
@@ -616,21 +609,18 @@ def linear_cross_entropy_backward(H, W, targets, lse, dloss=None, reduction="mea
     """Gradients (dH, dW) of linear_cross_entropy in the operands' type, for the
     gradient dloss of its result (a 0-d tensor, [rows] for "none"; None = 1);
     None in place of one that is not needed."""
-    a = _cross_entropy_args(H, W, targets, lse, reduction)
+    a, index = _cross_entropy_args(H, W, targets, lse, reduction)
     if dloss is not None:
-        a.dloss = _sized("linear_cross_entropy dloss", _dev(dloss, _F32),
-                         H.shape[0] if reduction == "none" else 1).data_ptr()
+        a.dloss = _at("linear_cross_entropy dloss", dloss, _F32, H.shape[0] if reduction == "none" else 1, index)
     if need_dH:
         dH = torch.empty(H.shape, dtype=H.dtype, device=H.device) if dH is None else dH
-        a.lddh = _matrix("linear_cross_entropy dH", dH, *H.shape, dtype=H.dtype)
-        a.dH = dH.data_ptr()
+        a.dH, a.lddh = _matrix("linear_cross_entropy dH", dH, *H.shape, H.dtype, index)
     if need_dW:
         dW = torch.empty(W.shape, dtype=W.dtype, device=W.device) if dW is None else dW
-        a.lddw = _matrix("linear_cross_entropy dW", dW, *W.shape, dtype=W.dtype)
-        a.dW = dW.data_ptr()
-    _same_device(H, W, targets, lse, dloss, dH, dW)
-    with _on(H.device, lib().silcu_linear_cross_entropy_workspace_bytes(ct.byref(a), 1)) as (wp, wn, stream):
-        check(lib().silcu_linear_cross_entropy_backward(ct.byref(a), wp, wn, stream))
+        a.dW, a.lddw = _matrix("linear_cross_entropy dW", dW, *W.shape, W.dtype, index)
+    nbytes = lib().silcu_linear_cross_entropy_workspace_bytes(a, 1)
+    buf, ws = _scratch(nbytes, H.device)
+    _launch(lib().silcu_linear_cross_entropy_backward, index, a, ws, nbytes)
     return dH if need_dH else None, dW if need_dW else None
 
 
@@ -643,7 +633,6 @@ class TensorList:
         self.tensors = list(tensors)
         if not self.tensors:
             raise ValueError("TensorList: no tensors")
-        self.device = self.tensors[0].device
         self._addresses = None
         self._layout()
 
@@ -656,18 +645,18 @@ class TensorList:
         self.array = (_lib.Tensor * n)()
         self.pointers = (ct.c_void_p * n)(*addresses)
         for i, t in enumerate(self.tensors):
-            _floats(t)
-            _same_device(self.tensors[0], t)
-            self.array[i] = _lib.Tensor(addresses[i], t.numel(), DTYPE[t.dtype])
+            k = _kind(t)
+            if i == 0:
+                self.device, self.index = t.device, t.get_device()
+            _at(f"TensorList tensor {i}", t, t.dtype, t.numel(), self.index)
+            self.array[i] = _lib.Tensor(addresses[i], t.numel(), k)
+        self.shapes = [(t.dtype, t.numel()) for t in self.tensors]
+        self.nbytes = lib().silcu_grad_norm_workspace_bytes(self.array, n)
         self._addresses = addresses
         return self
 
     def __len__(self):
         return len(self.tensors)
-
-    def _matches(self, other):
-        return len(self) == len(other) and self.device == other.device and all(
-            a.dtype == b.dtype and a.n == b.n for a, b in zip(self.array, other.array))
 
 
 def _list(tensors):
@@ -678,8 +667,8 @@ def grad_norm(tensors):
     """2-norm over a list of tensors (or a TensorList) as a 0-d device tensor."""
     tl = _list(tensors)
     norm = torch.empty((), dtype=_F32, device=tl.device)
-    with _on(tl.device, lib().silcu_grad_norm_workspace_bytes(tl.array, len(tl))) as (wp, wn, stream):
-        check(lib().silcu_grad_norm(tl.array, len(tl), _p(norm), wp, wn, stream))
+    buf, ws = _scratch(tl.nbytes, tl.device)
+    _launch(lib().silcu_grad_norm, tl.index, tl.array, len(tl), norm.data_ptr(), ws, tl.nbytes)
     return norm
 
 
@@ -688,13 +677,14 @@ def clip_grad_norm(tensors, max_norm, OUT=None, eps=1e-6):
     into OUT (a list or TensorList of the same shapes); returns the norm before
     clipping as a 0-d device tensor."""
     tl = _list(tensors)
-    out = None
+    pointers = None
     if OUT is not None:
         out = _list(OUT)
-        if not tl._matches(out):
+        if tl.shapes != out.shapes or tl.index != out.index:
             raise ValueError("clip_grad_norm: OUT must match the tensors in number, size, dtype and device")
+        pointers = out.pointers
     norm = torch.empty((), dtype=_F32, device=tl.device)
-    with _on(tl.device, lib().silcu_grad_norm_workspace_bytes(tl.array, len(tl))) as (wp, wn, stream):
-        check(lib().silcu_clip_grad_norm(tl.array, out.pointers if out is not None else None, len(tl),
-                                         float(max_norm), float(eps), _p(norm), wp, wn, stream))
+    buf, ws = _scratch(tl.nbytes, tl.device)
+    _launch(lib().silcu_clip_grad_norm, tl.index, tl.array, pointers, len(tl), max_norm, eps, norm.data_ptr(), ws,
+            tl.nbytes)
     return norm

@@ -75,8 +75,8 @@ def check_backward(x, dy, dres, gamma, mean, rstd, din, dgamma, dbeta):
     if dres is not None:
         tol = tol + U * (r_dx.abs() + dres.double().abs())
     check(din, r_dx, tol + (2 * U + half_step(din.dtype)) * r_dx.abs() + 1e-30, "din")
-    # a thread's rows, 8 warps, then 8 slices of at most 4 * 148 partials
-    chain = rows // 148 + 8 + 4 * 148 // 8 + 8 + 6
+    # a thread's rows (over 148 CTAs or more), 8 groups, then 32 slices of at most 12 * 148 partials
+    chain = rows // 148 + 8 + 12 * 148 // 32 + 32 + 6
     check(dgamma, r_dg, chain * U * (dy.double().abs() * xh).sum(0) + 1e-30, "dgamma")
     check(dbeta, r_db, chain * U * dy.double().abs().sum(0) + 1e-30, "dbeta")
 
@@ -204,7 +204,8 @@ def test_norm_and_clip(cuda, sizes, kinds, shift):
     ts = make_list(sizes, kinds, len(sizes) + shift, 0.3, shift)
     ref = norm64(ts)
     norm = float(gpu.grad_norm(ts))
-    # groups of at most 8 squares add in fp32 (8 u of a sum of positive terms), halved by the root; stored in fp32
+    # at most 8 squares of a vector and 3 of its neighbours add in fp32: 10 u of a sum of positive
+    # terms, halved by the root; stored in fp32
     assert abs(norm - ref) <= 6 * U * ref
     for max_norm in (0.37 * ref, 10 * ref):
         c = min(1.0, max_norm / (ref + 1e-6))
