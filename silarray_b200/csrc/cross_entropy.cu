@@ -14,10 +14,11 @@
 // keeping them would take T V values.
 // Bound by the tensor cores except for few rows, where reading W is all.
 //
-// fp32 operands go through the 3xTF32 GEMM (tc_gemm.cu), bf16 ones through
-// bf16_gemm.cuh; there ds is rounded to bf16, the operand type of its two
-// products, once per element (2^-9 relative, the rounding that the gradients
-// themselves take when they are stored).
+// The products run on loss_gemm.cuh: bf16 operands as they are, fp32 ones as
+// exact tf32 pairs (3xTF32), split once per call (H) and per piece (W).  With
+// bf16, ds is rounded to bf16, the operand type of its two products, once per
+// element; the factor that all rows share (the gradient of the mean or the
+// sum) multiplies the results instead, so that its own rounding does not.
 //
 // Rows whose target lies outside [0, V) are left out: the backward pass works
 // on a copy of H with those rows zero and gives them ds = 0 by selection, so
@@ -27,8 +28,7 @@
 
 #include <utility>
 
-#include "bf16_gemm.cuh"
-#include "gemm_internal.cuh"
+#include "loss_gemm.cuh"
 
 namespace silcu {
 namespace {
@@ -37,12 +37,12 @@ using Args = silcu_cross_entropy_args;
 
 // ------------------------------------------------------------ small kernels
 // Joins a row's parts: lse = M + log sum l_i exp(m_i - M).  A CTA takes 32
-// rows, 8 warps the parts in 8 interleaved slices.
-__global__ void __launch_bounds__(256) loss_finish(const float2 *__restrict__ part, int nparts, int64_t rows,
-                                                   const int32_t *__restrict__ targets, int V,
-                                                   const float *__restrict__ target_score, float *__restrict__ lse,
-                                                   float *__restrict__ loss) {
-  __shared__ float2 sm[8][32];
+// rows, 32 warps the parts in 32 interleaved slices.
+__global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ part, int nparts, int64_t rows,
+                                                    const int32_t *__restrict__ targets, int V,
+                                                    const float *__restrict__ target_score, float *__restrict__ lse,
+                                                    float *__restrict__ loss) {
+  __shared__ float2 sm[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int64_t row = int64_t(blockIdx.x) * 32 + lane;
   float m = -INFINITY, l = 0.f;
@@ -54,13 +54,13 @@ __global__ void __launch_bounds__(256) loss_finish(const float2 *__restrict__ pa
   };
   if (row < rows) {
 #pragma unroll 4
-    for (int i = slice; i < nparts; i += 8) join(__ldcs(part + int64_t(i) * rows + row));
+    for (int i = slice; i < nparts; i += 32) join(__ldcs(part + int64_t(i) * rows + row));
   }
   sm[slice][lane] = make_float2(m, l);
   __syncthreads();
   if (slice == 0 && row < rows) {
 #pragma unroll
-    for (int i = 1; i < 8; i++) join(sm[i][lane]);
+    for (int i = 1; i < 32; i++) join(sm[i][lane]);
     const float v = m + logf(l);
     lse[row] = v;
     const int y = targets[row];
@@ -121,10 +121,12 @@ __global__ void __launch_bounds__(1024) row_scales(const float *__restrict__ dlo
 }
 
 // dst [rows, dp] = src [rows, D] (row stride ld), columns D.. zero; with
-// targets, rows that are left out are zero as well.
+// targets, rows that are left out are zero as well.  With `lo`, dst and lo
+// take the exact tf32 pair.
 template <typename T>
 __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int64_t ld, int64_t rows, int D, int dp,
-                                                 const int32_t *__restrict__ targets, int V, T *__restrict__ dst) {
+                                                 const int32_t *__restrict__ targets, int V, T *__restrict__ dst,
+                                                 float *__restrict__ lo) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = dp / W;
   const bool vec = ld % W == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
@@ -142,41 +144,61 @@ __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int6
       if (vec && c + W <= D) {
         v = raw_load<T, W>(src + r * ld + c);
       } else {
-        T *e = reinterpret_cast<T *>(&v);
+        T e[W] = {};
 #pragma unroll
         for (int k = 0; k < W; k++)
           if (c + k < D) e[k] = src[r * ld + c + k];
+        memcpy(&v, e, sizeof(v));
       }
+    }
+    if constexpr (sizeof(T) == 4) {
+      float x[4], l[4];
+      unpack(v, x);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float h = tc::tf32_rna(x[k]);
+        l[k] = __fsub_rn(x[k], h);
+        x[k] = h;
+      }
+      pack(x, v);
+      store_f32<4>(lo + r * dp + c, l);
     }
     *reinterpret_cast<decltype(v.r) *>(dst + r * dp + c) = v.r;
   }
 }
 
-// out [rows, D] bf16 = the sum of the fp32 planes [rows, ldp], in plane order.
+// out [rows, D] = alpha times the sum of the fp32 planes [rows, ldp], in plane order.
+template <typename T>
 __global__ void __launch_bounds__(256) planes_finish(const float *__restrict__ planes, int nplanes, int64_t plane,
-                                                     int64_t rows, int D, int ldp, __nv_bfloat16 *__restrict__ out,
-                                                     int64_t ldo, int vec) {
-  const int per_row = (D + 7) / 8;
+                                                     int64_t rows, int D, int ldp, const float *__restrict__ alpha,
+                                                     T *__restrict__ out, int64_t ldo, int vec) {
+  constexpr int W = 16 / sizeof(T);
+  const int per_row = (D + W - 1) / W;
   const int64_t n = rows * per_row;
+  const float k0 = alpha ? *alpha : 1.0f;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
     const int64_t r = i / per_row;
-    const int c = int(i - r * per_row) * 8;
-    float f[8] = {};
-    for (int p = 0; p < nplanes; p++) {  // ldp is a multiple of 8: the last vectors stay inside the row
-      float v[8];
-      load_f32<8>(planes + p * plane + r * ldp + c, v);
+    const int c = int(i - r * per_row) * W;
+    float f[W] = {};
+    for (int p = 0; p < nplanes; p++) {  // ldp is a multiple of W: the last vectors stay inside the row
+      float v[W];
+      load_f32<W>(planes + p * plane + r * ldp + c, v);
 #pragma unroll
-      for (int k = 0; k < 8; k++) f[k] += v[k];
+      for (int k = 0; k < W; k++) f[k] += v[k];
     }
-    __nv_bfloat16 *dst = out + r * ldo + c;
-    if (vec && c + 8 <= D) {
-      Raw<__nv_bfloat16, 8> o;
-      pack(f, o);
-      *reinterpret_cast<uint4 *>(dst) = o.r;
-    } else {
 #pragma unroll
-      for (int k = 0; k < 8; k++)
-        if (c + k < D) dst[k] = __float2bfloat16_rn(f[k]);
+    for (int k = 0; k < W; k++) f[k] *= k0;
+    T *dst = out + r * ldo + c;
+    Raw<T, W> o;
+    pack(f, o);
+    if (vec && c + W <= D) {
+      *reinterpret_cast<decltype(o.r) *>(dst) = o.r;
+    } else {
+      T e[W];
+      memcpy(e, &o, sizeof(o));
+#pragma unroll
+      for (int k = 0; k < W; k++)
+        if (c + k < D) dst[k] = e[k];
     }
   }
 }
@@ -187,23 +209,37 @@ uint32_t stream_grid(int64_t items) {
 }
 
 // --------------------------------------------------------------------- plan
-constexpr int64_t kPieceBytes = int64_t(256) << 20;  // of ds, and of a piece's copied weights
+using lossmm::Bf16;
+using lossmm::Operand;
+using lossmm::Tf32;
+
+// Of a piece's ds (and of its copied weights).
+constexpr int64_t kPieceBytes[2] = {int64_t(512) << 20, int64_t(256) << 20};  // by silcu_dtype
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 
 // Vocabulary columns per piece: a multiple of 256 whose `bytes` per column
-// stay within kPieceBytes, and pieces of about equal size.
-int64_t piece_of(int64_t V, int64_t bytes) {
-  int64_t p = kPieceBytes / bytes / 256 * 256;
+// stay within the limit, and pieces of about equal size.
+int64_t piece_of(int64_t V, int64_t bytes, int dtype) {
+  int64_t p = kPieceBytes[dtype] / bytes / 256 * 256;
   if (p < 256) p = 256;
-  if (p > (1 << 20)) p = 1 << 20;  // the packing passes' grids
   if (const char *e = getenv("SILCU_LOSS_PIECE")) {  // columns per piece at most (tests, tuning)
     const int64_t want = up(atoll(e) > 0 ? atoll(e) : 256, 256);
     if (want < p) p = want;
   }
   if (p >= V) return V;
-  const int64_t n = (V + p - 1) / p;
-  return up((V + n - 1) / n, 256);
+  return up(ceil_div(V, ceil_div(V, p)), 256);
+}
+
+// Tile columns of the scores.  More than 128 rows: CTA pairs, 256.  Else one
+// CTA per tile, as wide as spreads n columns evenly over rounds of all SMs
+// (32768 columns: 147 tiles of 224 on 148 SMs instead of 128 of 256), in steps
+// of an MMA's 16 columns, or of the 64 that a store of score gradients writes.
+int score_columns(int64_t rows, int64_t n, int step) {
+  if (rows > lossmm::BM) return lossmm::BN;
+  const int64_t sms = sm_count(), rounds = ceil_div(n, sms * lossmm::BN);
+  return int(up(ceil_div(n, sms * rounds), step));
 }
 
 bool rows16(const void *p, int64_t ld, int dtype) {
@@ -223,348 +259,247 @@ struct Space {
   }
 };
 
+// An operand's copy in the workspace: aligned rows (bf16), or the tf32 pair.
+template <typename Ty>
+struct Copy {
+  typename Ty::T *p = nullptr;
+  float *lo = nullptr;
+  int64_t dp = 0;
+  void take(Space &sp, int64_t rows, int64_t D) {
+    dp = up(D, 16 / int64_t(sizeof(typename Ty::T)));
+    p = sp.take<typename Ty::T>(rows * dp);
+    if (Ty::PARTS == 2) lo = sp.take<float>(rows * dp);
+  }
+  silcu_status fill(const void *src, int64_t ld, int64_t rows, int64_t D, const int32_t *targets, int64_t V,
+                    cudaStream_t s) const {
+    using T = typename Ty::T;
+    copy_rows<T><<<stream_grid(rows * dp * int64_t(sizeof(T)) / 16), 256, 0, s>>>(
+        static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo);
+    return check_launch("cross_entropy copy");
+  }
+  Operand operand(bool mn) const { return Operand{p, lo, dp, mn}; }
+};
+
+template <typename Ty>
 struct Forward {
-  int64_t piece, dp;
-  bool copy_h, copy_w;  // operands whose rows TMA cannot read in place (bf16)
+  int64_t piece;
+  int bn, nparts;
+  bool copy_h, copy_w;  // operands that are not read in place
+  Copy<Ty> h, w;
   float2 *part;
   float *target_score, *row_loss;
-  __nv_bfloat16 *h, *w;
-  float *h_hi, *h_lo;
-  void *gemm;
-  size_t gemm_bytes;
+
+  Forward(const Args &a, Space &sp) {
+    copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
+    copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
+    piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype) : a.V;
+    bn = score_columns(a.rows, piece, 16);
+    nparts = 0;
+    for (int64_t v0 = 0; v0 < a.V; v0 += piece) nparts += parts(a, v0);
+    part = sp.take<float2>(int64_t(nparts) * a.rows);
+    target_score = sp.take<float>(a.rows);
+    row_loss = a.reduction == SILCU_REDUCE_NONE ? a.loss : sp.take<float>(a.rows);
+    if (copy_h) h.take(sp, a.rows, a.D);
+    if (copy_w) w.take(sp, piece, a.D);
+  }
+  int64_t columns(const Args &a, int64_t v0) const { return a.V - v0 < piece ? a.V - v0 : piece; }
+  int parts(const Args &a, int64_t v0) const { return 2 * int(ceil_div(columns(a, v0), bn)); }
 };
 
-silcu_gemm_args f32_args(int64_t M, int64_t N, int64_t K) {
-  silcu_gemm_args g;
-  memset(&g, 0, sizeof(g));
-  g.M = M;
-  g.N = N;
-  g.K = K;
-  g.batch = 1;
-  g.alpha = 1.0f;
-  g.algo = SILCU_GEMM_TC3XTF32;
-  return g;
-}
+// One of the two products of ds, with M x N results from sums of K: its K is
+// cut into `split` parts whose sums are fp32 planes, and `direct` results
+// need no planes at all.
+struct Gradient {
+  int64_t M, N, K;
+  int split = 1;
+  bool wanted, direct;
+  float *planes = nullptr;
+  int64_t tiles() const { return ceil_div(M, 2 * lossmm::BM) * ceil_div(N, lossmm::BN); }
+};
 
-// Scores of a vocabulary piece (fp32): A = the split H, B = W's rows, plain.
-silcu_gemm_args score_args(const Args &a, const float *hi, const float *lo, int64_t dp, int64_t v0, int64_t n) {
-  silcu_gemm_args g = f32_args(a.rows, n, a.D);
-  g.A_hi = hi;
-  g.A_lo = lo;
-  g.lda = dp;
-  g.B = static_cast<const float *>(a.W) + v0 * a.ldw;
-  g.ldb = a.ldw;
-  g.trans_b = 1;
-  g.ldc = n;
-  return g;
-}
-
-// Not null, for workspace sizes: only whether an operand is given matters.
-float *given() { return reinterpret_cast<float *>(uintptr_t(256)); }
-
-template <typename F>
-size_t most_over_pieces(int64_t V, int64_t piece, F &&f) {
-  size_t most = f(piece);
-  if (V % piece) {
-    const size_t last = f(V % piece);
-    if (last > most) most = last;
-  }
-  return most;
-}
-
-Forward plan_forward(const Args &a, Space &sp) {
-  Forward f = {};
-  f.part = sp.take<float2>((a.V + 127) / 128 * a.rows);
-  f.target_score = sp.take<float>(a.rows);
-  f.row_loss = a.reduction == SILCU_REDUCE_NONE ? a.loss : sp.take<float>(a.rows);
-  if (a.dtype == SILCU_BF16) {
-    f.dp = up(a.D, 8);
-    f.copy_h = !rows16(a.H, a.ldh, a.dtype);
-    f.copy_w = !rows16(a.W, a.ldw, a.dtype);
-    f.piece = f.copy_w ? piece_of(a.V, 2 * f.dp) : a.V;
-    if (f.copy_h) f.h = sp.take<__nv_bfloat16>(a.rows * f.dp);
-    if (f.copy_w) f.w = sp.take<__nv_bfloat16>(f.piece * f.dp);
-  } else {
-    f.dp = up(a.D, 4);
-    f.piece = piece_of(a.V, 8 * f.dp);
-    f.h_hi = sp.take<float>(a.rows * f.dp);
-    f.h_lo = sp.take<float>(a.rows * f.dp);
-    f.gemm_bytes = most_over_pieces(a.V, f.piece, [&](int64_t n) {
-      return tc_loss_workspace_bytes(score_args(a, given(), given(), f.dp, 0, n));
-    });
-    f.gemm = sp.take<char>(int64_t(f.gemm_bytes));
-  }
-  return f;
-}
-
-// A bf16 product's split of K: parts for idle SMs when the tiles are few, at
-// least 8 stages of 64 k in each.
-int split_k(int64_t M, int64_t N, int64_t K) {
-  const bool pair = M > bf16::BM;
-  const int64_t units = pair ? sm_count() / 2 : sm_count();
-  const int64_t tiles = (M + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((N + 255) / 256);
-  int64_t ks = units / tiles;
-  const int64_t most = (K + 64 * 8 - 1) / (64 * 8);
-  if (ks > most) ks = most;
-  return int(ks < 1 ? 1 : ks);
-}
-
+template <typename Ty>
 struct Backward {
-  int64_t piece, dp, lds;  // lds: row stride of ds
-  float *scale;
-  void *h;                  // masked copy of H [rows, dp]
-  __nv_bfloat16 *w;         // a piece of W [piece, dp], when its rows are not aligned
-  void *ds;                 // [rows, lds]
+  int64_t piece, lds;  // lds: row stride of ds
+  int bn;
   bool copy_w;
-  float *dh_planes, *dw_planes;
-  int dh_split, dw_split;
-  bool dh_direct, dw_direct;
-  float *h_hi, *h_lo;
-  void *gemm;
-  size_t gemm_bytes;
+  float *scale;
+  Copy<Ty> h, w;       // H with left-out rows zero; a piece of W
+  Copy<Ty> ds;
+  Gradient dh, dw;
+
+  Backward(const Args &a, Space &sp) {
+    const int64_t e = int64_t(Ty::PARTS) * sizeof(typename Ty::T);
+    copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
+    const int64_t of_ds = e * a.rows, of_w = copy_w ? e * up(a.D, 8) : 0;
+    piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype);
+    bn = score_columns(a.rows, piece, 64);
+    scale = sp.take<float>(a.rows);
+    h.take(sp, a.rows, a.D);
+    if (copy_w) w.take(sp, piece, a.D);
+    ds.take(sp, a.rows, up(piece, 64));
+    lds = ds.dp;
+    dh.M = a.rows, dh.N = a.D, dh.K = piece, dh.wanted = a.dH;
+    dw.M = piece, dw.N = a.D, dw.K = a.rows, dw.wanted = a.dW;
+    // Parts of K where a single item would be more than half of what each SM
+    // pair has to do altogether; at least 512 k in each.
+    const double units = sm_count() / 2;
+    const double load = ((dh.wanted ? double(dh.tiles()) * dh.K : 0.0) + (dw.wanted ? double(dw.tiles()) * dw.K : 0.0)) / units;
+    for (Gradient *g : {&dh, &dw}) {
+      const double item = load / 2 > 512.0 ? load / 2 : 512.0;
+      const int64_t want = int64_t(double(g->K) / item) + (double(g->K) > item * double(int64_t(double(g->K) / item)));
+      g->split = int(want < 1 ? 1 : want > 32 ? 32 : want);
+    }
+    dh.direct = dh.split == 1 && piece == a.V;  // else pieces add up in the planes
+    dw.direct = dw.split == 1;
+    for (Gradient *g : {&dh, &dw})
+      if (g->wanted && !g->direct) g->planes = sp.take<float>(int64_t(g->split) * g->M * up(a.D, 8));
+  }
 };
-
-silcu_gemm_args dh_args(const Args &a, const float *ds, int64_t lds, int64_t v0, int64_t n) {
-  silcu_gemm_args g = f32_args(a.rows, a.D, n);
-  g.A = ds;
-  g.lda = lds;
-  g.B = static_cast<const float *>(a.W) + v0 * a.ldw;
-  g.ldb = a.ldw;
-  g.C = static_cast<float *>(a.dH);
-  g.ldc = a.lddh;
-  if (v0) {  // earlier pieces' sum
-    g.residual = g.C;
-    g.ldr = a.lddh;
-  }
-  return g;
-}
-
-silcu_gemm_args dw_args(const Args &a, const float *ds, int64_t lds, const float *h, int64_t dp, int64_t v0,
-                        int64_t n) {
-  silcu_gemm_args g = f32_args(n, a.D, a.rows);
-  g.A = ds;
-  g.lda = lds;
-  g.trans_a = 1;
-  g.B = h;
-  g.ldb = dp;
-  g.C = static_cast<float *>(a.dW) + v0 * a.lddw;
-  g.ldc = a.lddw;
-  return g;
-}
-
-Backward plan_backward(const Args &a, Space &sp) {
-  Backward b = {};
-  b.scale = sp.take<float>(a.rows);
-  if (a.dtype == SILCU_BF16) {
-    b.dp = up(a.D, 8);
-    b.copy_w = !rows16(a.W, a.ldw, a.dtype);
-    const int64_t per_col = 2 * a.rows > 2 * b.dp || !b.copy_w ? 2 * a.rows : 2 * b.dp;
-    b.piece = piece_of(a.V, per_col);
-    b.lds = up(b.piece, 64);
-    b.h = sp.take<__nv_bfloat16>(a.rows * b.dp);
-    if (b.copy_w) b.w = sp.take<__nv_bfloat16>(b.piece * b.dp);
-    b.ds = sp.take<__nv_bfloat16>(a.rows * b.lds);
-    if (a.dH) {
-      b.dh_split = split_k(a.rows, a.D, b.piece);
-      b.dh_direct = b.dh_split == 1 && b.piece == a.V;
-      if (!b.dh_direct) b.dh_planes = sp.take<float>(b.dh_split * a.rows * b.dp);
-    }
-    if (a.dW) {
-      b.dw_split = split_k(b.piece, a.D, a.rows);
-      b.dw_direct = b.dw_split == 1;
-      if (!b.dw_direct) b.dw_planes = sp.take<float>(b.dw_split * b.piece * b.dp);
-    }
-  } else {
-    b.dp = up(a.D, 4);
-    b.piece = piece_of(a.V, 4 * a.rows > 8 * b.dp ? 4 * a.rows : 8 * b.dp);
-    b.lds = up(b.piece, 4);
-    b.h = sp.take<float>(a.rows * b.dp);
-    b.h_hi = sp.take<float>(a.rows * b.dp);
-    b.h_lo = sp.take<float>(a.rows * b.dp);
-    b.ds = sp.take<float>(a.rows * b.lds);
-    b.gemm_bytes = most_over_pieces(a.V, b.piece, [&](int64_t n) {
-      silcu_gemm_args s = score_args(a, given(), given(), b.dp, 0, n);
-      s.C = given();
-      size_t most = tc_loss_workspace_bytes(s);
-      for (const bool first : {true, false}) {  // with and without an earlier sum to add
-        silcu_gemm_args g = dh_args(a, given(), b.lds, first ? 0 : 256, n);
-        g.C = given();
-        const size_t w = tc_workspace_bytes(g);
-        if (w > most) most = w;
-      }
-      silcu_gemm_args g = dw_args(a, given(), b.lds, given(), b.dp, 0, n);
-      g.C = given();
-      const size_t w = tc_workspace_bytes(g);
-      return w > most ? w : most;
-    });
-    b.gemm = sp.take<char>(int64_t(b.gemm_bytes));
-  }
-  return b;
-}
 
 // ---------------------------------------------------------------------- run
-silcu_status copy_bf16(const void *src, int64_t ld, int64_t rows, int64_t D, int64_t dp, const int32_t *targets,
-                       int64_t V, __nv_bfloat16 *dst, cudaStream_t s) {
-  copy_rows<__nv_bfloat16><<<stream_grid(rows * dp / 8), 256, 0, s>>>(
-      static_cast<const __nv_bfloat16 *>(src), ld, rows, int(D), int(dp), targets, int(V), dst);
-  return check_launch("cross_entropy copy");
-}
-
-template <int EPI>
-silcu_status bf16_scores(bf16::Params &p, bool pair, cudaStream_t s) {
-  return pair ? bf16::launch<false, false, EPI, true>(p, s) : bf16::launch<false, false, EPI, false>(p, s);
-}
-
 silcu_status map_error() { return fail(SILCU_CUDA_ERROR, "cross_entropy: cuTensorMapEncodeTiled failed"); }
 
-silcu_status forward(const Args &a, const Forward &f, cudaStream_t s) {
+template <typename Ty, int EPI>
+silcu_status scores(lossmm::Params &p, int64_t rows, cudaStream_t s) {
+  return rows > lossmm::BM ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
+}
+
+template <typename T>
+const T *row_of(const void *base, int64_t row, int64_t ld) {
+  return static_cast<const T *>(base) + row * ld;
+}
+
+template <typename Ty>
+silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
+  using T = typename Ty::T;
   silcu_status st;
-  LossArgs loss = {};
-  loss.targets = a.targets;
-  loss.V = int32_t(a.V);
-  loss.part = f.part;
-  loss.target_score = f.target_score;
-  if (a.dtype == SILCU_BF16) {
-    bf16::Operand h{a.H, a.ldh, false};
-    if (f.copy_h) {
-      if ((st = copy_bf16(a.H, a.ldh, a.rows, a.D, f.dp, nullptr, 0, f.h, s)) != SILCU_OK) return st;
-      h = {f.h, f.dp, false};
-    }
-    for (int64_t v0 = 0; v0 < a.V; v0 += f.piece) {
-      const int64_t n = a.V - v0 < f.piece ? a.V - v0 : f.piece;
-      const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.W) + v0 * a.ldw;
-      bf16::Operand w{src, a.ldw, false};
-      if (f.copy_w) {
-        if ((st = copy_bf16(src, a.ldw, n, a.D, f.dp, nullptr, 0, f.w, s)) != SILCU_OK) return st;
-        w = {f.w, f.dp, false};
-      }
-      bf16::Params p;
-      memset(&p, 0, sizeof(p));
-      const bool pair = a.rows > bf16::BM;
-      if (!bf16::set_operands(p, pair, a.rows, n, a.D, h, w)) return map_error();
-      p.loss = loss;
-      p.loss.v0 = int32_t(v0);
-      p.err = device_error_ptr();
-      if ((st = bf16_scores<bf16::kStats>(p, pair, s)) != SILCU_OK) return st;
-    }
-  } else {
-    st = split_rows(static_cast<const float *>(a.H), a.ldh, 1, a.rows, a.D, f.dp, f.h_hi, f.h_lo, s);
-    if (st != SILCU_OK) return st;
-    for (int64_t v0 = 0; v0 < a.V; v0 += f.piece) {
-      const int64_t n = a.V - v0 < f.piece ? a.V - v0 : f.piece;
-      loss.v0 = int32_t(v0);
-      st = tc_run_loss(score_args(a, f.h_hi, f.h_lo, f.dp, v0, n), kLossStats, loss, f.gemm, f.gemm_bytes, s);
-      if (st != SILCU_OK) return st;
-    }
+  Operand h{a.H, nullptr, a.ldh, false};
+  if (f.copy_h) {
+    if ((st = f.h.fill(a.H, a.ldh, a.rows, a.D, nullptr, 0, s)) != SILCU_OK) return st;
+    h = f.h.operand(false);
   }
-  loss_finish<<<uint32_t((a.rows + 31) / 32), 256, 0, s>>>(f.part, int((a.V + 127) / 128), a.rows, a.targets,
-                                                           int(a.V), f.target_score, a.lse, f.row_loss);
+  int part0 = 0;
+  for (int64_t v0 = 0; v0 < a.V; v0 += f.piece) {
+    const int64_t n = f.columns(a, v0);
+    const T *src = row_of<T>(a.W, v0, a.ldw);
+    Operand w{src, nullptr, a.ldw, false};
+    if (f.copy_w) {
+      if ((st = f.w.fill(src, a.ldw, n, a.D, nullptr, 0, s)) != SILCU_OK) return st;
+      w = f.w.operand(false);
+    }
+    lossmm::Params p;
+    memset(&p, 0, sizeof(p));
+    if (!lossmm::set_problem<Ty>(p.p[0], a.rows > lossmm::BM, f.bn, a.rows, n, a.D, h, w)) return map_error();
+    p.bn = f.bn;
+    p.part0 = part0;
+    p.err = device_error_ptr();
+    p.loss.targets = a.targets;
+    p.loss.V = int32_t(a.V);
+    p.loss.v0 = int32_t(v0);
+    p.loss.part = f.part;
+    p.loss.target_score = f.target_score;
+    if ((st = scores<Ty, lossmm::kStats>(p, a.rows, s)) != SILCU_OK) return st;
+    part0 += f.parts(a, v0);
+  }
+  loss_finish<<<uint32_t((a.rows + 31) / 32), 1024, 0, s>>>(f.part, f.nparts, a.rows, a.targets, int(a.V),
+                                                            f.target_score, a.lse, f.row_loss);
   if ((st = check_launch("cross_entropy finish")) != SILCU_OK || a.reduction == SILCU_REDUCE_NONE) return st;
   loss_reduce<<<1, 1024, 0, s>>>(f.row_loss, a.targets, a.rows, int(a.V), a.reduction == SILCU_REDUCE_MEAN, a.loss);
   return check_launch("cross_entropy reduce");
 }
 
-silcu_status backward_bf16(const Args &a, const Backward &b, cudaStream_t s) {
+// Where a product of ds goes: the result itself, or planes that earlier
+// pieces may have begun.
+void set_output(lossmm::Problem &q, const Gradient &g, bool add, void *out, int64_t ldo, int vec, const float *alpha,
+                int64_t D, int64_t nk) {
+  q.ksplit = int(g.split < nk ? g.split : nk);  // a short last piece adds to the first planes only
+  q.alpha = alpha;
+  if (g.direct) {
+    q.mode = lossmm::kDirect;
+    q.out = out;
+    q.ldo = ldo;
+    q.vec = vec;
+  } else {
+    q.mode = add ? lossmm::kPlaneAdd : lossmm::kPlane;
+    q.out = g.planes;
+    q.ldo = up(D, 8);
+    q.plane = g.M * q.ldo;
+  }
+}
+
+template <typename Ty>
+silcu_status finish_planes(const Gradient &g, int64_t rows, int64_t D, const float *alpha, void *out, int64_t ldo,
+                           int vec, cudaStream_t s) {
+  using T = typename Ty::T;
+  const int64_t ldp = up(D, 8);
+  planes_finish<T><<<stream_grid(rows * ceil_div(D * int64_t(sizeof(T)), 16)), 256, 0, s>>>(
+      g.planes, g.split, g.M * ldp, rows, int(D), int(ldp), alpha, static_cast<T *>(out), ldo, vec);
+  return check_launch("cross_entropy planes");
+}
+
+template <typename Ty>
+silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
+  using T = typename Ty::T;
+  constexpr int BK = lossmm::Cfg<Ty, lossmm::kOut, true>::BK;
   silcu_status st;
-  __nv_bfloat16 *hm = static_cast<__nv_bfloat16 *>(b.h), *ds = static_cast<__nv_bfloat16 *>(b.ds);
-  if ((st = copy_bf16(a.H, a.ldh, a.rows, a.D, b.dp, a.targets, a.V, hm, s)) != SILCU_OK) return st;
-  const bool dh_vec = rows16(a.dH, a.lddh, a.dtype), dw_vec = rows16(a.dW, a.lddw, a.dtype);
-  const bool pair = a.rows > bf16::BM;
+  row_scales<<<1, 1024, 0, s>>>(a.dloss, a.targets, a.rows, int(a.V), a.reduction, b.scale);
+  if ((st = check_launch("cross_entropy scales")) != SILCU_OK) return st;
+  if ((st = b.h.fill(a.H, a.ldh, a.rows, a.D, a.targets, a.V, s)) != SILCU_OK) return st;
+  // A factor that all rows share leaves ds alone where ds is rounded.
+  const bool shared = Ty::PARTS == 1 && a.reduction != SILCU_REDUCE_NONE;
+  const float *alpha = shared ? b.scale : nullptr;
+  const int dh_vec = rows16(a.dH, a.lddh, a.dtype), dw_vec = rows16(a.dW, a.lddw, a.dtype);
   for (int64_t v0 = 0; v0 < a.V; v0 += b.piece) {
     const int64_t n = a.V - v0 < b.piece ? a.V - v0 : b.piece;
-    const void *w = static_cast<const __nv_bfloat16 *>(a.W) + v0 * a.ldw;
-    int64_t ldw = a.ldw;
+    const T *src = row_of<T>(a.W, v0, a.ldw);
+    Operand w{src, nullptr, a.ldw, false};
     if (b.copy_w) {
-      if ((st = copy_bf16(w, a.ldw, n, a.D, b.dp, nullptr, 0, b.w, s)) != SILCU_OK) return st;
-      w = b.w;
-      ldw = b.dp;
+      if ((st = b.w.fill(src, a.ldw, n, a.D, nullptr, 0, s)) != SILCU_OK) return st;
+      w = b.w.operand(false);
     }
-    bf16::Params p;
+    lossmm::Params p;
     memset(&p, 0, sizeof(p));
     p.err = device_error_ptr();
-    if (!bf16::set_operands(p, pair, a.rows, n, a.D, {hm, b.dp, false}, {w, ldw, false}) ||
-        !tc::make_map2_bf16(&p.c, ds, n, a.rows, b.lds, 64, 32))
-      return map_error();
+    p.bn = b.bn;
+    bool ok = lossmm::set_problem<Ty>(p.p[0], a.rows > lossmm::BM, b.bn, a.rows, n, a.D, b.h.operand(false), w);
+    for (int h = 0; h < Ty::PARTS; h++)
+      ok = ok && tc::make_map2<T>(&p.c[h], h ? static_cast<const void *>(b.ds.lo) : b.ds.p, n, a.rows, b.lds, Ty::KROW,
+                                  32, false);
+    if (!ok) return map_error();
     p.loss.targets = a.targets;
     p.loss.V = int32_t(a.V);
     p.loss.v0 = int32_t(v0);
     p.loss.lse = a.lse;
-    p.loss.scale = b.scale;
-    if ((st = bf16_scores<bf16::kScoreGrad>(p, pair, s)) != SILCU_OK) return st;
-    if (a.dH) {
-      if (!bf16::set_operands(p, pair, a.rows, a.D, n, {ds, b.lds, false}, {w, ldw, true})) return map_error();
-      const int nk = int((n + bf16::BK - 1) / bf16::BK);
-      p.ksplit = b.dh_split < nk ? b.dh_split : nk;  // a short last piece adds to the first planes only
-      if (b.dh_direct) {
-        p.mode = bf16::kOutBf16;
-        p.out = a.dH;
-        p.ldo = a.lddh;
-        p.vec = dh_vec;
-      } else {
-        p.mode = v0 ? bf16::kOutPlaneAdd : bf16::kOutPlane;
-        p.out = b.dh_planes;
-        p.ldo = b.dp;
-        p.plane = a.rows * b.dp;
-      }
-      st = pair ? bf16::launch<false, true, bf16::kOut, true>(p, s) : bf16::launch<false, true, bf16::kOut, false>(p, s);
-      if (st != SILCU_OK) return st;
-    }
-    if (a.dW) {
-      const bool wide = n > bf16::BM;
-      if (!bf16::set_operands(p, wide, n, a.D, a.rows, {ds, b.lds, true}, {hm, b.dp, true})) return map_error();
-      __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.dW) + v0 * a.lddw;
-      p.ksplit = b.dw_split;
-      if (b.dw_direct) {
-        p.mode = bf16::kOutBf16;
-        p.out = out;
-        p.ldo = a.lddw;
-        p.vec = dw_vec;
-      } else {
-        p.mode = bf16::kOutPlane;
-        p.out = b.dw_planes;
-        p.ldo = b.dp;
-        p.plane = b.piece * b.dp;
-      }
-      st = wide ? bf16::launch<true, true, bf16::kOut, true>(p, s) : bf16::launch<true, true, bf16::kOut, false>(p, s);
-      if (st != SILCU_OK) return st;
-      if (!b.dw_direct) {
-        planes_finish<<<stream_grid(n * b.dp / 8), 256, 0, s>>>(b.dw_planes, b.dw_split, p.plane, n, int(a.D),
-                                                                int(b.dp), out, a.lddw, dw_vec);
-        if ((st = check_launch("cross_entropy planes")) != SILCU_OK) return st;
-      }
-    }
-  }
-  if (a.dH && !b.dh_direct) {
-    planes_finish<<<stream_grid(a.rows * b.dp / 8), 256, 0, s>>>(b.dh_planes, b.dh_split, a.rows * b.dp, a.rows,
-                                                                 int(a.D), int(b.dp),
-                                                                 static_cast<__nv_bfloat16 *>(a.dH), a.lddh, dh_vec);
-    return check_launch("cross_entropy planes");
-  }
-  return SILCU_OK;
-}
+    p.loss.scale = shared ? nullptr : b.scale;
+    if ((st = scores<Ty, lossmm::kScoreGrad>(p, a.rows, s)) != SILCU_OK) return st;
 
-silcu_status backward_f32(const Args &a, const Backward &b, cudaStream_t s) {
-  silcu_status st;
-  float *hm = static_cast<float *>(b.h), *ds = static_cast<float *>(b.ds);
-  copy_rows<float><<<stream_grid(a.rows * b.dp / 4), 256, 0, s>>>(static_cast<const float *>(a.H), a.ldh, a.rows,
-                                                                  int(a.D), int(b.dp), a.targets, int(a.V), hm);
-  if ((st = check_launch("cross_entropy copy")) != SILCU_OK) return st;
-  if ((st = split_rows(hm, b.dp, 1, a.rows, a.D, b.dp, b.h_hi, b.h_lo, s)) != SILCU_OK) return st;
-  LossArgs loss = {};
-  loss.targets = a.targets;
-  loss.V = int32_t(a.V);
-  loss.lse = a.lse;
-  loss.scale = b.scale;
-  for (int64_t v0 = 0; v0 < a.V; v0 += b.piece) {
-    const int64_t n = a.V - v0 < b.piece ? a.V - v0 : b.piece;
-    loss.v0 = int32_t(v0);
-    silcu_gemm_args g = score_args(a, b.h_hi, b.h_lo, b.dp, v0, n);
-    g.C = ds;
-    g.ldc = b.lds;
-    if ((st = tc_run_loss(g, kLossGrad, loss, b.gemm, b.gemm_bytes, s)) != SILCU_OK) return st;
-    if (a.dH && (st = tc_run(dh_args(a, ds, b.lds, v0, n), b.gemm, b.gemm_bytes, s)) != SILCU_OK) return st;
-    if (a.dW && (st = tc_run(dw_args(a, ds, b.lds, hm, b.dp, v0, n), b.gemm, b.gemm_bytes, s)) != SILCU_OK) return st;
+    // Both products of ds in one launch, the one with the longer items first.
+    memset(&p, 0, sizeof(p));
+    p.err = device_error_ptr();
+    p.bn = lossmm::BN;
+    int count = 0;
+    w.mn = true;
+    const bool dw_first = b.dw.K / b.dw.split > b.dh.K / b.dh.split;
+    for (const bool is_dw : {dw_first, !dw_first}) {
+      if (!(is_dw ? b.dw : b.dh).wanted) continue;
+      lossmm::Problem &q = p.p[count++];
+      if (is_dw) {
+        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
+          return map_error();
+        set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, alpha, a.D,
+                   ceil_div(a.rows, BK));
+      } else {
+        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
+        set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, alpha, a.D, ceil_div(n, BK));
+      }
+    }
+    if ((st = lossmm::launch<Ty, lossmm::kOut, true>(p, count, s)) != SILCU_OK) return st;
+    if (b.dw.wanted && !b.dw.direct) {
+      st = finish_planes<Ty>(b.dw, n, a.D, alpha, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, s);
+      if (st != SILCU_OK) return st;
+    }
   }
+  if (b.dh.wanted && !b.dh.direct) return finish_planes<Ty>(b.dh, a.rows, a.D, alpha, a.dH, a.lddh, dh_vec, s);
   return SILCU_OK;
 }
 
@@ -618,8 +553,13 @@ size_t silcu_linear_cross_entropy_workspace_bytes(const silcu_cross_entropy_args
   using namespace silcu;
   if (check_shape("linear_cross_entropy_workspace_bytes", ap) != SILCU_OK || ap->rows == 0) return 0;
   Space f{nullptr}, b{nullptr};
-  plan_forward(*ap, f);
-  if (backward) plan_backward(*ap, b);
+  if (ap->dtype == SILCU_BF16) {
+    Forward<Bf16> plan(*ap, f);
+    if (backward) Backward<Bf16> plan_b(*ap, b);
+  } else {
+    Forward<Tf32> plan(*ap, f);
+    if (backward) Backward<Tf32> plan_b(*ap, b);
+  }
   return (f.used > b.used ? f.used : b.used) + 256;  // the caller's pointer need not be aligned
 }
 
@@ -640,7 +580,7 @@ silcu_status silcu_linear_cross_entropy(const silcu_cross_entropy_args *ap, void
   if ((st = check_pointers("linear_cross_entropy", a)) != SILCU_OK) return st;
   if ((st = check_space("linear_cross_entropy", a, 0, workspace, workspace_bytes)) != SILCU_OK) return st;
   Space sp{align256(workspace)};
-  return forward(a, plan_forward(a, sp), s);
+  return a.dtype == SILCU_BF16 ? forward(a, Forward<Bf16>(a, sp), s) : forward(a, Forward<Tf32>(a, sp), s);
 }
 
 silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args *ap, void *workspace,
@@ -664,10 +604,7 @@ silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args 
   if ((st = check_pointers(what, a)) != SILCU_OK) return st;
   if ((st = check_space(what, a, 1, workspace, workspace_bytes)) != SILCU_OK) return st;
   Space sp{align256(workspace)};
-  const Backward b = plan_backward(a, sp);
-  row_scales<<<1, 1024, 0, s>>>(a.dloss, a.targets, a.rows, int(a.V), a.reduction, b.scale);
-  if ((st = check_launch(what)) != SILCU_OK) return st;
-  return a.dtype == SILCU_BF16 ? backward_bf16(a, b, s) : backward_f32(a, b, s);
+  return a.dtype == SILCU_BF16 ? backward(a, Backward<Bf16>(a, sp), s) : backward(a, Backward<Tf32>(a, sp), s);
 }
 
 }  // extern "C"

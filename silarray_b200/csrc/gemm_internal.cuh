@@ -3,7 +3,6 @@
 #pragma once
 
 #include "common.cuh"
-#include "loss_epilogue.cuh"
 
 namespace silcu {
 
@@ -43,18 +42,6 @@ struct TcConv {
 silcu_status split_contiguous(const float *src, uint64_t n, float *hi, float *lo, cudaStream_t s);
 silcu_status tc_run(const silcu_gemm_args &a, void *ws, size_t ws_bytes, cudaStream_t s,
                     const TcConv *conv = nullptr);
-// The product as the scores of a cross entropy (its columns [v0, v0 + N) of
-// the vocabulary): kLossStats writes only the parts and target scores, kLossGrad
-// writes the scores' gradient to C.  Split and batch-free arguments only;
-// the output tiles run whole (no split K).
-enum LossEpilogue { kLossNone = 0, kLossStats = 1, kLossGrad = 2 };
-silcu_status tc_run_loss(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs &loss, void *ws,
-                         size_t ws_bytes, cudaStream_t s);
-size_t tc_loss_workspace_bytes(const silcu_gemm_args &a);
-// hi / lo [rows, Kp] of src element (r, k) at r * rs + k * ks (one of them 1);
-// columns K..Kp - 1 are zero.  Kp % 4 == 0 keeps the rows 16-byte aligned.
-silcu_status split_rows(const float *src, int64_t rs, int64_t ks, int64_t rows, int64_t K, int64_t Kp, float *hi,
-                        float *lo, cudaStream_t s);
 // The 3xTF32 path's tiling and split-K choice for these arguments.
 void tc_describe(const silcu_gemm_args &a, silcu_gemm_plan *out);
 

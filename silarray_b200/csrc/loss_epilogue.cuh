@@ -1,9 +1,8 @@
 // What the vocabulary projections of the cross entropy do with their scores
-// in registers, shared by the fp32 (tc_gemm.cu) and bf16 (cross_entropy.cu)
-// tensor-core kernels: a thread holds N neighbouring scores of one row.
+// in registers: a thread holds up to 128 neighbouring scores of one row.
 //
-//   forward   running maximum m and l = sum exp(s - m) of the row over the
-//             thread's 128 columns (a "part"), and the target's score;
+//   forward   maximum m and l = sum exp(s - m) of the row over the thread's
+//             columns (a "part"), and the target's score;
 //   backward  ds = g (exp(s - lse) - [column = target]).
 #pragma once
 
@@ -22,41 +21,39 @@ __device__ __forceinline__ float ex2(float x) {
 struct LossArgs {
   const int32_t *targets;  // [rows]; outside [0, V) = the row is left out
   int32_t v0, V;           // vocabulary index of this launch's column 0; vocabulary size
-  float2 *part;            // forward: [ceil(V / 128)][rows] (m, l)
+  float2 *part;            // forward: [parts][rows] (m, l)
   float *target_score;     // forward: [rows], written for rows that count
   const float *lse;        // backward: [rows]
-  const float *scale;      // backward: [rows] gradient of each row's loss
+  const float *scale;      // backward: [rows] gradient of each row's loss, or null = 1
 };
 
-// Folds N scores, of which the first `valid` exist, into (m, l).  The terms
+// Folds 32 scores, of which the first `valid` exist, into (m, l).  The terms
 // are 2^(s log2 e - m log2 e): one multiply-add and one ex2 each.  A row of
 // -inf alone keeps l = 0; NaN and +inf make l NaN.
-template <int N>
-__device__ __forceinline__ void softmax_fold(const float (&v)[N], int base, int valid, float &m, float &l) {
+__device__ __forceinline__ void softmax_fold(const float (&v)[32], int valid, float &m, float &l) {
   float mx = m;
 #pragma unroll
   for (int i = 0; i < 32; i++)
-    if (i < valid) mx = fmaxf(mx, v[base + i]);
+    if (i < valid) mx = fmaxf(mx, v[i]);
   const float neg = mx == -INFINITY ? 0.f : -mx * kLog2e;
   l *= ex2(fmaf(m, kLog2e, neg));  // m = -inf: 0
   float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 32; i++)
-    if (i < valid) a[i & 3] += ex2(fmaf(v[base + i], kLog2e, neg));
+    if (i < valid) a[i & 3] += ex2(fmaf(v[i], kLog2e, neg));
   l += (a[0] + a[1]) + (a[2] + a[3]);
   m = mx;
 }
 
-// v[base + 0..31]: the scores' gradients in place of the scores.  `at` = the
-// target's column relative to the first of them, `counts` = the row is not
-// left out (a row that is gets exact zeros, whatever its scores are).
-template <int N>
-__device__ __forceinline__ void score_gradient(float (&v)[N], int base, float lse_log2e, float g, int at, bool counts) {
+// The scores' gradients in place of the scores.  `at` = the target's column
+// relative to the first of them, `counts` = the row is not left out (a row that
+// is gets exact zeros, whatever its scores are).
+__device__ __forceinline__ void score_gradient(float (&v)[32], float lse_log2e, float g, int at, bool counts) {
 #pragma unroll
   for (int i = 0; i < 32; i++) {
-    float p = ex2(fmaf(v[base + i], kLog2e, -lse_log2e));
+    float p = ex2(fmaf(v[i], kLog2e, -lse_log2e));
     if (i == at) p -= 1.0f;
-    v[base + i] = counts ? g * p : 0.f;
+    v[i] = counts ? g * p : 0.f;
   }
 }
 

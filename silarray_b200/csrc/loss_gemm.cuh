@@ -1,0 +1,634 @@
+// The tensor-core products of the cross entropy (sm_100a), for bf16 operands
+// and for fp32 ones given as exact tf32 pairs (x = hi + lo).
+//
+// One persistent kernel, D[M, N] = A . B with fp32 accumulation in TMEM:
+//   bf16  tcgen05.mma kind::f16, one product per 16 k;
+//   tf32  kind::tf32, lo.hi + hi.lo + hi.hi per 8 k (3xTF32).
+// Either operand may lie in either major order (k contiguous, or the M / N
+// index), so ds and W serve their products in place and nothing is transposed.
+//   warp 0      TMA producer: boxes of 128-byte rows, 192 KB ring;
+//   warp 1      allocates the 512 TMEM columns (two accumulators of 256) and
+//               issues the MMAs from one thread;
+//   warps 2-9   epilogue, two per TMEM lane quarter, 128 columns each.
+// A tile is 256 x 256 on a CTA pair (cta_group::2: each CTA loads its 128 rows
+// of A and 128 columns of B), or 128 x bn on one CTA for the scores of at most
+// 128 rows, where reading W is all and bn spreads it evenly over the SMs.
+//
+// What bounds it: the tensor pipe and, over many milliseconds, the card's
+// power.  The one thread that issues the MMAs was the limit at first: with a
+// commit per CTA of the pair, descriptors built per MMA and a stage of 64 k,
+// the scores of 8192 x 131072 x 2048 took 3.73 ms (1181 TFLOP/s); one multicast
+// commit for both CTAs 3.53; descriptors advanced by an add and the wait's
+// first poll inline 3.31; stages of 128 k 3.13 (1405; torch.matmul's library
+// product alone 3.35 at the same shape and load).  4 to 7 stages of 64 k gave the
+// same times, and prefetching operands to the L2 made them worse.
+//
+// Sums: the tensor core truncates as it accumulates, so sums that need more
+// than its 2^-22 per step are cut into chunks (128 k of tf32, 1024 k of the bf16
+// scores that become lse); the epilogue adds each chunk in fp32 registers, to
+// nearest, while the next one runs.  What is rounded to bf16 next takes one chunk.
+//
+// Every wait is bounded; on expiry the kernel records a code, unwinds, frees
+// its TMEM and exits.  No load is multicast.
+#pragma once
+
+#include <cuda.h>
+
+#include "elem.cuh"
+#include "loss_epilogue.cuh"
+#include "tc_common.cuh"
+
+namespace silcu {
+namespace lossmm {
+using namespace tc;
+
+constexpr int BM = 128, BN = 256;
+
+enum Epilogue { kStats = 0, kScoreGrad = 1, kOut = 2 };
+enum OutMode { kDirect = 0, kPlane = 1, kPlaneAdd = 2 };
+
+struct Bf16 {
+  using T = __nv_bfloat16;
+  static constexpr int PARTS = 1, KROW = 64, KMMA = 16;  // k in a 128-byte row, and of one MMA
+  static constexpr uint32_t FORMAT = (1u << 7) | (1u << 10);
+};
+struct Tf32 {
+  using T = float;
+  static constexpr int PARTS = 2, KROW = 32, KMMA = 8;
+  static constexpr uint32_t FORMAT = (2u << 7) | (2u << 10);
+};
+
+template <typename Ty, int EPI, bool PAIR>
+struct Cfg {
+  static constexpr int TM = PAIR ? 2 * BM : BM;
+  static constexpr int ROWS_B = PAIR ? BN / 2 : BN;  // B columns held per CTA
+  static constexpr int SUBS = PAIR && Ty::PARTS == 1 ? 2 : 1;  // 128-byte-row tiles of each operand per stage
+  static constexpr int BK = SUBS * Ty::KROW;
+  static constexpr int TILE_A = BM * 128, TILE_B = ROWS_B * 128;
+  static constexpr int STAGE_BYTES = SUBS * Ty::PARTS * (TILE_A + TILE_B);
+  static constexpr int STAGES = 192 * 1024 / STAGE_BYTES;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int SMEM_BYTES = RING_BYTES + EPI_WARPS * 4096 + 1024 + 512;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int NBUF = 2;
+  // stages per accumulation chunk; MULTI: a tile may take several, which meet in registers
+  static constexpr bool MULTI = Ty::PARTS == 2 || EPI == kStats;
+  // The sum goes back to TMEM for an epilogue that has no registers beside it
+  // (with the 128 sums in registers the tf32 score gradients spill 2.8 KB a thread).
+  static constexpr bool BACK = MULTI && EPI == kScoreGrad;
+  static constexpr int CHUNK = !MULTI ? 1 << 30 : (Ty::PARTS == 2 ? 128 : 1024) / BK;
+  static constexpr int GROUP_M = EPI == kOut ? 8 : 16;
+  static constexpr uint32_t MN_BOX = Ty::KROW * 128;       // KROW elements of M / N x KROW k
+  static constexpr uint32_t MN_STEP = Ty::KMMA * 128;      // one MMA's k inside it
+  static constexpr int MN_BOXES_A = BM / Ty::KROW, MN_BOXES_B = ROWS_B / Ty::KROW;
+  static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+};
+
+struct Problem {
+  CUtensorMap a[2], b[2];  // [part]: hi, lo (tf32)
+  int M, N, K, tiles_m, tiles_n;
+  int ksplit;              // each tile's K range in this many parts (kOut; part i -> plane i)
+  int amn;                 // kOut: A is stored with the M index contiguous
+  int mode, vec;           // vec: kDirect rows are 16-byte aligned
+  void *out;
+  int64_t ldo, plane;      // row stride; elements from one plane to the next
+  const float *alpha;      // kDirect: factor of the result, or null
+};
+
+struct __align__(64) Params {
+  Problem p[2];  // kOut: up to two products in one launch
+  CUtensorMap c[2];  // score gradients' stores [part]
+  int bn;            // tile columns
+  // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
+  int units, n0, n1, tail, extra;
+  LossArgs loss;
+  int part0;  // index of this launch's first part
+  int *err;
+};
+
+struct Work {
+  int prob, item;
+};
+
+// The k-th item of unit u.  The first product's items go round the units; if
+// the last round leaves units tail.. without one, those start with `extra` rounds of
+// the second product's (about one item of the first in cost), and the rest goes
+// round all units.
+__device__ __forceinline__ bool work_at(const Params &p, int u, int k, Work &w) {
+  const int q0 = u < p.n0 ? (p.n0 - u + p.units - 1) / p.units : 0;
+  if (k < q0) {
+    w = Work{0, u + k * p.units};
+    return true;
+  }
+  k -= q0;
+  const int low = p.units - p.tail;  // units short of one item
+  int j;
+  if (p.tail && u >= p.tail) j = k < p.extra ? k * low + u - p.tail : p.extra * low + (k - p.extra) * p.units + u;
+  else j = p.extra * low + k * p.units + u;
+  w = Work{1, j};
+  return j < p.n1;
+}
+
+struct Tile {
+  int m0, n0, kb0, kb1, part;
+};
+
+template <typename C>
+__device__ __forceinline__ Tile tile_of(const Problem &q, int bn, int item) {
+  const int t = item / q.ksplit, part = item - t * q.ksplit;
+  const int group = t / (C::GROUP_M * q.tiles_n);
+  const int first = group * C::GROUP_M;
+  const int gm = q.tiles_m - first < C::GROUP_M ? q.tiles_m - first : C::GROUP_M;
+  const int r = t - group * C::GROUP_M * q.tiles_n;
+  const int nk = (q.K + C::BK - 1) / C::BK;
+  return Tile{(first + r % gm) * C::TM, (r / gm) * bn, int(int64_t(part) * nk / q.ksplit),
+              int(int64_t(part + 1) * nk / q.ksplit), part};
+}
+
+template <typename Ty, typename C>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
+  if (!mn) return make_desc(addr);
+  return Ty::PARTS == 1 ? make_desc_mn16(addr, C::MN_BOX) : make_desc_mn32(addr, C::MN_BOX);
+}
+
+// BMN: B is stored with the N index contiguous (kOut; A's order is Problem::amn).
+template <typename Ty, int EPI, bool PAIR>
+__global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __grid_constant__ Params p) {
+  using C = Cfg<Ty, EPI, PAIR>;
+  using T = typename Ty::T;
+  constexpr bool BMN = EPI == kOut;
+  constexpr int STAGES = C::STAGES, NBUF = C::NBUF, PARTS = Ty::PARTS, SUBS = C::SUBS;
+  constexpr int TILE_A = C::TILE_A, TILE_B = C::TILE_B, SUB_BYTES = PARTS * (TILE_A + TILE_B);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING_BYTES + C::EPI_WARPS * 4096);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2 * NBUF);
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+  const uint32_t tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + NBUF);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const int unit = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
+  const int bn = PAIR ? BN : p.bn;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int j = 0; j < NBUF; j++) {
+      mbar_init(tfull0 + 8 * j, 1);
+      mbar_init(tempty0 + 8 * j, C::EPI_WARPS * (PAIR ? 2 : 1));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Work w;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t kbg = 0;
+      bool ok = true;
+      const uint32_t bytes = SUBS * PARTS * (TILE_A + (PAIR ? TILE_B : bn * 128)) * (PAIR ? 2 : 1);
+      for (int k = 0; ok && work_at(p, unit, k, w); k++) {
+        const Problem &q = p.p[w.prob];
+        const Tile tl = tile_of<C>(q, bn, w.item);
+        const int am = tl.m0 + BM * int(rank), nb = tl.n0 + C::ROWS_B * int(rank);
+        const bool amn = EPI == kOut && q.amn;
+        for (int kb = tl.kb0; kb < tl.kb1; kb++, kbg++) {
+          const uint32_t s = kbg % STAGES, ph = (kbg / STAGES) & 1;
+          if (kbg >= uint32_t(STAGES) && !mbar_try_wait(empty0 + 8 * s, ph ^ 1) &&
+              !mbar_wait(empty0 + 8 * s, ph ^ 1, p.err, 21)) {
+            ok = false;
+            break;
+          }
+          // a pair's bytes all complete on the even CTA's barrier
+          const uint32_t bar = PAIR ? mapa_shared(full0 + 8 * s, 0) : full0 + 8 * s;
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, bytes);
+          auto load = [&](uint32_t dst, const CUtensorMap *map, int c0, int c1) {
+            if (PAIR) tma_load_2d_pair(dst, map, bar, c0, c1);
+            else tma_load_2d(dst, map, bar, c0, c1);
+          };
+#pragma unroll
+          for (int u = 0; u < SUBS; u++) {
+            const int kc = kb * C::BK + u * Ty::KROW;
+            uint32_t dst = smem_u32(smem + s * C::STAGE_BYTES + u * SUB_BYTES);
+#pragma unroll
+            for (int h = 0; h < PARTS; h++, dst += TILE_A) {
+              if (amn) {
+#pragma unroll
+                for (int i = 0; i < C::MN_BOXES_A; i++) load(dst + i * C::MN_BOX, &q.a[h], am + Ty::KROW * i, kc);
+              } else {
+                load(dst, &q.a[h], kc, am);
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < PARTS; h++, dst += TILE_B) {
+              if (BMN) {
+#pragma unroll
+                for (int i = 0; i < C::MN_BOXES_B; i++) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
+              } else {
+                load(dst, &q.b[h], kc, nb);
+              }
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {  // the pair's MMAs are issued by the even CTA
+      uint32_t kbg = 0, cg = 0;
+      bool ok = true;
+      const uint32_t base = smem_u32(smem);
+      for (int k = 0; ok && work_at(p, unit, k, w); k++) {
+        const Problem &q = p.p[w.prob];
+        const Tile tl = tile_of<C>(q, bn, w.item);
+        const bool amn = EPI == kOut && q.amn;
+        const uint64_t adesc = operand_desc<Ty, C>(base, amn), bdesc = operand_desc<Ty, C>(base + PARTS * TILE_A, BMN);
+        const uint32_t astep = (amn ? C::MN_STEP : 32u) >> 4, bstep = (BMN ? C::MN_STEP : 32u) >> 4;
+        const uint32_t idesc = (1u << 4) | Ty::FORMAT | (uint32_t(amn) << 15) | (uint32_t(BMN) << 16) |
+                               (uint32_t(bn >> 3) << 17) | (uint32_t(C::TM >> 4) << 24);
+        for (int c0 = tl.kb0; c0 < tl.kb1 && ok; c0 += C::CHUNK, cg++) {
+          const int c1 = tl.kb1 - c0 < C::CHUNK ? tl.kb1 : c0 + C::CHUNK;
+          const uint32_t j = cg % NBUF, use = cg / NBUF;
+          if (cg >= uint32_t(NBUF) && !mbar_wait(tempty0 + 8 * j, (use & 1) ^ 1, p.err, 24)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t acc = tmem + j * BN;
+          for (int kb = c0; kb < c1; kb++, kbg++) {
+            const uint32_t s = kbg % STAGES, ph = (kbg / STAGES) & 1;
+            if (!mbar_try_wait(full0 + 8 * s, ph) && !mbar_wait(full0 + 8 * s, ph, p.err, 22)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int u = 0; u < SUBS; u++) {
+              const uint32_t off = (s * C::STAGE_BYTES + u * SUB_BYTES) >> 4;
+#pragma unroll
+              for (int kk = 0; kk < Ty::KROW / Ty::KMMA; kk++) {
+                const uint64_t a = adesc + uint64_t(off + kk * astep), b = bdesc + uint64_t(off + kk * bstep);
+                const uint32_t first = (kb == c0 && u == 0 && kk == 0) ? 0u : 1u;
+                if constexpr (PARTS == 1) {
+                  if (PAIR) mma_f16_pair(acc, a, b, idesc, first);
+                  else mma_f16(acc, a, b, idesc, first);
+                } else {  // small terms first
+                  const uint64_t al = a + uint64_t(TILE_A >> 4), bl = b + uint64_t(TILE_B >> 4);
+                  if (PAIR) {
+                    mma_tf32_pair(acc, al, b, idesc, first);
+                    mma_tf32_pair(acc, a, bl, idesc, 1u);
+                    mma_tf32_pair(acc, a, b, idesc, 1u);
+                  } else {
+                    mma_tf32(acc, al, b, idesc, first);
+                    mma_tf32(acc, a, bl, idesc, 1u);
+                    mma_tf32(acc, a, b, idesc, 1u);
+                  }
+                }
+              }
+            }
+            if (PAIR) mma_commit_both(empty0 + 8 * s);  // the stage is free in both CTAs
+            else mma_commit(empty0 + 8 * s);
+          }
+          if (PAIR) mma_commit_both(tfull0 + 8 * j);
+          else mma_commit(tfull0 + 8 * j);
+        }
+      }
+    }
+  } else {
+    const int qr = warp & 3, h = (warp - 2) >> 2;
+    float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
+    uint32_t cg = 0;
+    bool ok = true;
+    for (int k = 0; ok && work_at(p, unit, k, w); k++) {
+      const Problem &q = p.p[w.prob];
+      const Tile tl = tile_of<C>(q, bn, w.item);
+      const int r0 = tl.m0 + BM * int(rank) + 32 * qr, c0 = tl.n0 + 128 * h;
+      const int row = r0 + lane;
+      const int cols = min(q.N, tl.n0 + bn) - c0;  // this warp's columns of the tile, up to 128 (may be <= 0)
+      // what the epilogue needs of the row arrives while the MMAs run
+      int y = -1;
+      float lse = 0.f, g = 0.f;
+      if (EPI != kOut && row < q.M) {
+        y = p.loss.targets[row];
+        if (EPI == kScoreGrad) {
+          lse = p.loss.lse[row] * kLog2e;
+          g = p.loss.scale ? p.loss.scale[row] : 1.0f;
+        }
+      }
+      auto finished = [&](uint32_t t) {  // the accumulator of chunk t is complete
+        const uint32_t j = t % NBUF, use = t / NBUF;
+        const bool got = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * j, use & 1, p.err, 23));
+        tc_fence_after();
+        return got;
+      };
+      auto release = [&](uint32_t t) {  // the MMAs may write it again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t bar = tempty0 + 8 * (t % NBUF);
+          if (PAIR) mbar_arrive_cluster(mapa_shared(bar, 0));
+          else mbar_arrive(bar);
+        }
+      };
+      const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + 128 * h;
+      float acc[C::MULTI ? 128 : 1];
+      if constexpr (C::MULTI) {
+        for (int kc = tl.kb0; kc < tl.kb1; kc += C::CHUNK, cg++) {
+          if (!finished(cg)) {
+            ok = false;
+            break;
+          }
+          if (cols > 0) {
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++) {
+              uint32_t r[32];
+              tmem_ld32_nowait(src0 + (cg % NBUF) * BN + 32 * cb, r);
+              tmem_ld_wait();
+              if (kc == tl.kb0) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) acc[32 * cb + i] = __uint_as_float(r[i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i++) acc[32 * cb + i] = __fadd_rn(acc[32 * cb + i], __uint_as_float(r[i]));
+              }
+            }
+          }
+          if (!C::BACK || kc + C::CHUNK < tl.kb1) release(cg);
+        }
+        if constexpr (C::BACK) {
+          if (ok && cols > 0) {
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++) {
+              uint32_t r[32];
+#pragma unroll
+              for (int i = 0; i < 32; i++) r[i] = __float_as_uint(acc[32 * cb + i]);
+              tmem_st32_cols(src0 + ((cg - 1) % NBUF) * BN + 32 * cb, r);
+            }
+            tmem_st_wait();
+          }
+        }
+      } else {
+        ok = finished(cg++);
+      }
+      if (!__all_sync(0xffffffffu, ok && *reinterpret_cast<volatile int *>(p.err) == 0)) break;
+      constexpr bool IN_REGS = C::MULTI && !C::BACK;
+      // Columns 32 cb .. 32 cb + 31 of this thread's row.
+      auto block = [&](int cb, float (&v)[32]) {
+        if constexpr (IN_REGS) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) v[i] = acc[32 * cb + i];
+        } else {
+          uint32_t r[32];
+          tmem_ld32_nowait(src0 + ((cg - 1) % NBUF) * BN + 32 * cb, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+        }
+      };
+      constexpr int UNROLL = IN_REGS ? 4 : 1;
+
+      if constexpr (EPI == kStats) {
+        if (r0 < q.M) {
+          float m = -INFINITY, l = 0.f;
+          const int at = y - p.loss.v0 - c0;  // the target among this thread's columns
+          const bool mine = y >= 0 && y < p.loss.V && at >= 0 && at < cols;
+#pragma unroll
+          for (int cb = 0; cb < 4; cb++) {
+            const int valid = cols - 32 * cb;
+            if (valid > 0) {
+              float v[32];
+              block(cb, v);
+              if (valid >= 32) softmax_fold(v, 32, m, l);
+              else softmax_fold(v, valid, m, l);
+              if (mine && (at >> 5) == cb) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                  if (i == (at & 31)) p.loss.target_score[row] = v[i];
+              }
+            }
+          }
+          if (row < q.M) p.loss.part[int64_t(p.part0 + 2 * (tl.n0 / bn) + h) * q.M + row] = make_float2(m, l);
+        }
+      } else if constexpr (EPI == kScoreGrad) {
+        if (r0 < q.M) {
+          const bool counts = y >= 0 && y < p.loss.V;
+          const int at = y - p.loss.v0 - c0;
+          auto stage_ready = [&] {  // the staging block's last store has read it
+            if (lane == 0) bulk_wait_read0();
+            __syncwarp();
+          };
+          auto send = [&](const CUtensorMap *map, int col) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(map, smem_u32(st), col, r0);
+              bulk_commit();
+            }
+          };
+          auto put = [&](int i, uint4 v) {  // 16-byte chunk i of this lane's 128-byte row
+            *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(st) + lane * 128 + 16 * (i ^ (lane & 7))) = v;
+          };
+#pragma unroll UNROLL
+          for (int cb = 0; cb < 4; cb++) {
+            if (32 * cb < cols) {
+              float v[32];
+              block(cb, v);
+              score_gradient(v, lse, g, at - 32 * cb, counts);
+              if constexpr (PARTS == 1) {  // 64 bf16 columns per 128-byte row: two blocks a store
+                if ((cb & 1) == 0) stage_ready();
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                  put(4 * (cb & 1) + i, make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                                                   pack_bf16(v[8 * i + 4], v[8 * i + 5]),
+                                                   pack_bf16(v[8 * i + 6], v[8 * i + 7])));
+                if ((cb & 1) || 32 * (cb + 1) >= cols) send(&p.c[0], c0 + 32 * (cb & ~1));
+              } else {  // the exact tf32 pair, 32 columns per row each
+#pragma unroll
+                for (int part = 0; part < 2; part++) {
+                  stage_ready();
+#pragma unroll
+                  for (int i = 0; i < 8; i++) {
+                    uint32_t e[4];
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                      const float x = v[4 * i + t], hi = tf32_rna(x);
+                      e[t] = __float_as_uint(part ? __fsub_rn(x, hi) : hi);
+                    }
+                    put(i, make_uint4(e[0], e[1], e[2], e[3]));
+                  }
+                  send(&p.c[part], c0 + 32 * cb);
+                }
+              }
+            }
+          }
+        }
+      } else if (r0 < q.M) {
+        const float alpha = q.mode == kDirect && q.alpha ? *q.alpha : 1.0f;
+#pragma unroll UNROLL
+        for (int cb = 0; cb < 4; cb++) {
+          if (32 * cb < cols) {
+            float v[32];
+            block(cb, v);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              *reinterpret_cast<float4 *>(st + lane * 32 + 4 * (i ^ (lane & 7))) =
+                  make_float4(alpha * v[4 * i], alpha * v[4 * i + 1], alpha * v[4 * i + 2], alpha * v[4 * i + 3]);
+            __syncwarp();
+            const int col0 = c0 + 32 * cb;
+            if (q.mode != kDirect || PARTS == 2) {  // fp32: 8 lanes per row, 16 bytes each
+              float *out = static_cast<float *>(q.out) + tl.part * q.plane;
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const int rr = 4 * i + (lane >> 3), ch = lane & 7, col = col0 + 4 * ch;
+                float4 x = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * (ch ^ (rr & 7)));
+                if (r0 + rr < q.M && col < q.N) {
+                  float *dst = out + int64_t(r0 + rr) * q.ldo + col;
+                  if (q.mode == kPlaneAdd) {
+                    const float4 o = *reinterpret_cast<const float4 *>(dst);
+                    x.x += o.x, x.y += o.y, x.z += o.z, x.w += o.w;
+                  }
+                  if (q.mode != kDirect || (q.vec && col + 4 <= q.N)) {  // a plane's rows hold whole vectors
+                    *reinterpret_cast<float4 *>(dst) = x;
+                  } else {
+                    const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                      if (col + t < q.N) dst[t] = e[t];
+                  }
+                }
+              }
+            } else {  // bf16: 4 lanes per row, 8 columns each
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int rr = 8 * i + (lane >> 2), ch = 2 * (lane & 3), col = col0 + 4 * ch;
+                const float4 x = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * (ch ^ (rr & 7)));
+                const float4 u = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * ((ch + 1) ^ (rr & 7)));
+                if (r0 + rr < q.M && col < q.N) {
+                  __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(q.out) + int64_t(r0 + rr) * q.ldo + col;
+                  if (q.vec && col + 8 <= q.N) {
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w),
+                                                                 pack_bf16(u.x, u.y), pack_bf16(u.z, u.w));
+                  } else {
+                    const float e[8] = {x.x, x.y, x.z, x.w, u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int t = 0; t < 8; t++)
+                      if (col + t < q.N) dst[t] = __float2bfloat16_rn(e[t]);
+                  }
+                }
+              }
+            }
+          }
+        }
+      }
+      if constexpr (!IN_REGS) release(cg - 1);
+    }
+    if (EPI == kScoreGrad) {
+      if (lane == 0) bulk_wait_all0();  // every store has completed before exit
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // no CTA frees TMEM or leaves while its peer may still use the pair
+  if (warp == 1) {
+    tc_fence_after();
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---------------------------------------------------------------- host side
+// An operand in memory: [MN, k] rows, or with `mn` [k, MN] rows; the row
+// stride in elements.  Pointers and row strides are multiples of 16 bytes.
+struct Operand {
+  const void *p, *lo;  // lo: tf32 only
+  int64_t ld;
+  bool mn;
+};
+
+template <typename Ty>
+bool operand_map(CUtensorMap (&m)[2], const Operand &o, int64_t extent, int64_t K, int rows) {
+  for (int h = 0; h < Ty::PARTS; h++) {
+    const void *p = h ? o.lo : o.p;
+    const bool ok = o.mn ? make_map2<typename Ty::T>(&m[h], p, extent, K, o.ld, Ty::KROW, Ty::KROW, Ty::PARTS == 2)
+                         : make_map2<typename Ty::T>(&m[h], p, K, extent, o.ld, Ty::KROW, rows, false);
+    if (!ok) return false;
+  }
+  return true;
+}
+
+template <typename Ty>
+bool set_problem(Problem &q, bool pair, int bn, int64_t M, int64_t N, int64_t K, const Operand &a, const Operand &b) {
+  q.M = int(M);
+  q.N = int(N);
+  q.K = int(K);
+  const int TM = pair ? 2 * BM : BM;
+  q.tiles_m = int((M + TM - 1) / TM);
+  q.tiles_n = int((N + bn - 1) / bn);
+  q.ksplit = 1;
+  q.amn = a.mn;
+  return operand_map<Ty>(q.a, a, M, K, BM) && operand_map<Ty>(q.b, b, N, K, pair ? BN / 2 : bn);
+}
+
+inline int64_t items_of(const Problem &q) { return int64_t(q.tiles_m) * q.tiles_n * q.ksplit; }
+
+template <typename Ty, int EPI, bool PAIR>
+silcu_status launch(Params &p, int problems, cudaStream_t s) {
+  using C = Cfg<Ty, EPI, PAIR>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(gemm<Ty, EPI, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               C::SMEM_BYTES);
+    if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "cross_entropy: smem attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int64_t n0 = items_of(p.p[0]), n1 = problems > 1 ? items_of(p.p[1]) : 0;
+  if (n0 + n1 > 0x3FFFFFFF) return fail(SILCU_UNSUPPORTED, "cross_entropy: too many tiles");
+  const int64_t most = PAIR ? sm_count() / 2 : sm_count();
+  p.n0 = int(n0);
+  p.n1 = int(n1);
+  p.units = int(n0 + n1 < most ? n0 + n1 : most);
+  p.tail = int(n0 % p.units);
+  p.extra = 0;
+  if (n1 && p.tail) {  // an item of the first product in items of the second, by their k
+    const double c0 = double(p.p[0].K) / p.p[0].ksplit, c1 = double(p.p[1].K) / p.p[1].ksplit;
+    p.extra = int(c0 / c1 + 0.5);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(uint32_t(p.units * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = PAIR ? 2 : 1;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm<Ty, EPI, PAIR>, p);
+  if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "cross_entropy: launch: %s", cudaGetErrorString(e));
+  return check_launch("cross_entropy");
+}
+
+}  // namespace lossmm
+}  // namespace silcu

@@ -244,6 +244,19 @@ __device__ __forceinline__ uint64_t make_desc_mn16(uint32_t addr, uint32_t mn_by
   return d;
 }
 
+// MN-major 32-bit operand, 128-byte swizzle with 32-byte atoms: rows of 32 MN
+// elements, groups of 4 k 512 B apart (SBO), the next 32 elements `mn_bytes`
+// away (LBO); written by boxes with SWIZZLE_128B_ATOM_32B.
+__device__ __forceinline__ uint64_t make_desc_mn32(uint32_t addr, uint32_t mn_bytes) {
+  uint64_t d = 0;
+  d |= uint64_t((addr & 0x3FFFFu) >> 4);
+  d |= uint64_t(mn_bytes >> 4) << 16;
+  d |= uint64_t(512 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(1) << 61;
+  return d;
+}
+
 // bf16 (or f16) operands, fp32 accumulation, K = 16 per instruction.
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accum) {
@@ -290,6 +303,14 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t cluster_bar) {
                : "memory");
 }
 
+// The same arriving on the barrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void mma_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(uint16_t(3))
+      : "memory");
+}
+
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                : "memory");
@@ -309,6 +330,20 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[3
 }
 
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this lane's TMEM row, and the wait for such stores.
+__device__ __forceinline__ void tmem_st32_cols(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -353,19 +388,22 @@ inline bool make_map4(CUtensorMap *m, const float *base, int64_t inner, int64_t 
   return r == CUDA_SUCCESS;
 }
 
-// A 2-D bf16 view {inner, rows} with row stride ld, boxes {box0, box1},
-// 128-byte swizzle (box0 = 64).
-inline bool make_map2_bf16(CUtensorMap *m, const void *base, int64_t inner, int64_t rows, int64_t ld, int box0,
-                           int box1) {
+// A 2-D view {inner, rows} of fp32 or 16-bit (bf16) elements with row stride
+// ld, boxes {box0, box1} of 128-byte rows, 128-byte swizzle (atom32: with
+// 32-byte atoms, for MN-major 32-bit operands).
+template <typename T>
+bool make_map2(CUtensorMap *m, const void *base, int64_t inner, int64_t rows, int64_t ld, int box0, int box1,
+               bool atom32) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(rows)};
-  cuuint64_t strides[1] = {cuuint64_t(ld) * 2};
+  cuuint64_t strides[1] = {cuuint64_t(ld) * sizeof(T)};
   cuuint32_t box[2] = {cuuint32_t(box0), cuuint32_t(box1)};
   cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(m, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+            const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 typedef CUresult (*EncodeIm2colFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,

@@ -30,8 +30,6 @@
 #include <stdlib.h>
 #include <string.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "gemm_internal.cuh"
 #include "tc_common.cuh"
@@ -109,7 +107,6 @@ struct __align__(64) TcParams {
   // each K block (16 channels of one filter tap) loads as one im2col box.
   int conv, cv_H, cv_W, cv_C, cv_K, cv_pad;
   TcEpi epi;
-  LossArgs loss;  // LOSS != kLossNone
   int *err;
 };
 
@@ -179,9 +176,7 @@ __device__ __forceinline__ void stage_row_swz(float *st, int lane, const float (
 // SPLIT: the launch has split-K tiles (full_items < all tiles).  Launches
 // without them use the SPLIT = false instance, which has none of the part
 // logic and so the register allocation of the plain epilogue.
-// LOSS: the scores of a cross entropy (loss_epilogue.cuh) instead of the plain
-// epilogue, or before its store.
-template <int BN_, bool PAIR, bool SPLIT, int LOSS>
+template <int BN_, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(Cfg<BN_>::NUM_THREADS, 1) tc_gemm_kernel(const __grid_constant__ TcParams p) {
   using C = Cfg<BN_, PAIR>;
   constexpr int BN = C::BN, STAGES = C::STAGES, NBUF = C::NBUF, RING_BYTES = C::RING_BYTES;
@@ -419,35 +414,6 @@ __global__ void __launch_bounds__(Cfg<BN_>::NUM_THREADS, 1) tc_gemm_kernel(const
       }
       const bool good = __all_sync(0xffffffffu, ok && *reinterpret_cast<volatile int *>(p.err) == 0);
       if (!good) break;
-      if constexpr (LOSS == kLossStats) {
-        const int row = m0 + 32 * q + lane, c0 = tl.n0 + h * EC;
-        if (row < p.M && c0 < p.N) {
-          const int y = p.loss.targets[row] - p.loss.v0 - c0;
-          float m = -INFINITY, l = 0.f;
-#pragma unroll
-          for (int cb = 0; cb < EC / 32; cb++) {
-            const int valid = p.N - c0 - 32 * cb;
-            if (valid <= 0) break;
-            softmax_fold(acc, 32 * cb, valid < 32 ? valid : 32, m, l);
-          }
-          p.loss.part[int64_t((p.loss.v0 + c0) / 128) * p.M + row] = make_float2(m, l);
-          if (y >= 0 && y < EC && y < p.N - c0) {
-#pragma unroll
-            for (int i = 0; i < EC; i++)
-              if (i == y) p.loss.target_score[row] = acc[i];
-          }
-        }
-        continue;
-      }
-      if constexpr (LOSS == kLossGrad) {
-        const int row = m0 + 32 * q + lane, c0 = tl.n0 + h * EC;
-        const bool in = row < p.M;
-        const int t = in ? p.loss.targets[row] : -1;
-        const float lse = in ? p.loss.lse[row] * kLog2e : 0.f, g = in ? p.loss.scale[row] : 0.f;
-#pragma unroll
-        for (int cb = 0; cb < EC / 32; cb++)
-          score_gradient(acc, 32 * cb, lse, g, t - p.loss.v0 - c0 - 32 * cb, t >= 0 && t < p.loss.V);
-      }
       const int part = item_part(tile);
       if (SPLIT && part >= 0) {
         // A K part of a split tile: its plain partial, no epilogue.
@@ -735,14 +701,14 @@ __global__ void __launch_bounds__(256) split_contig(const float *__restrict__ sr
 // ---------------------------------------------------------------- host side
 int64_t padded_k(int64_t K) { return ((K + KPAD - 1) / KPAD) * KPAD; }
 
-template <int BN, bool PAIR, bool SPLIT, int LOSS = kLossNone>
+template <int BN, bool PAIR, bool SPLIT>
 silcu_status launch_tc(const TcParams &p, uint32_t grid, cudaStream_t s) {
   using C = Cfg<BN, PAIR>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(tc_gemm_kernel<BN, PAIR, SPLIT, LOSS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(tc_gemm_kernel<BN, PAIR, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::SMEM_BYTES);
     if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "sgemm(tc): smem attribute: %s", cudaGetErrorString(e));
     configured[dev] = true;
@@ -759,7 +725,7 @@ silcu_status launch_tc(const TcParams &p, uint32_t grid, cudaStream_t s) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tc_gemm_kernel<BN, PAIR, SPLIT, LOSS>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tc_gemm_kernel<BN, PAIR, SPLIT>, p);
   if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "sgemm(tc): launch: %s", cudaGetErrorString(e));
   return check_launch("sgemm(tc)");
 }
@@ -827,7 +793,7 @@ struct TcPlan {
 // 3 parts and N = 3072 runs 74 whole pair tiles plus 22 in 3 parts.  Every
 // part keeps at least two accumulation chunks (256 k).  SILCU_TC_KSPLIT = 1
 // disables splitting, 2..8 splits every tile in that many parts (tuning).
-TcPlan tc_plan(const silcu_gemm_args &a, bool whole_tiles = false) {
+TcPlan tc_plan(const silcu_gemm_args &a) {
   TcPlan pl;
   const int64_t Kp = padded_k(a.K > 0 ? a.K : 1);
   const int64_t nb = total_batch(a);
@@ -845,7 +811,7 @@ TcPlan tc_plan(const silcu_gemm_args &a, bool whole_tiles = false) {
   const int64_t T = pl.tiles_m * pl.tiles_n * nb;
   pl.full_items = T;
   const int64_t nkb = (Kp + BK - 1) / BK;
-  if (nb != 1 || whole_tiles || forced == 1 || T > 65535) return pl;  // the finishing pass's grid.y counts split tiles
+  if (nb != 1 || forced == 1 || T > 65535) return pl;  // the finishing pass's grid.y counts split tiles
   if (forced >= 2 && forced <= 8) {
     pl.ksplit = int(forced < nkb ? forced : nkb);
     pl.full_items = 0;
@@ -968,34 +934,12 @@ void tc_describe(const silcu_gemm_args &a, silcu_gemm_plan *out) {
   out->whole_tiles = pl.full_items;
 }
 
-namespace {
-size_t workspace_bytes(const silcu_gemm_args &a, bool whole_tiles) {
+size_t tc_workspace_bytes(const silcu_gemm_args &a) {
   const int64_t Kp = padded_k(a.K > 0 ? a.K : 1);
   size_t bytes = 256;
   if (!a_given_split(a)) bytes += size_t(2) * Kp * size_t(total_batch(a)) * size_t(a.M) * sizeof(float);
   if (!b_given_split_kmajor(a)) bytes += size_t(2) * Kp * size_t(total_batch(a)) * size_t(a.N) * sizeof(float);
-  return bytes + partial_bytes(a, tc_plan(a, whole_tiles));
-}
-silcu_status run(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs *loss, void *ws, size_t wsb,
-                 cudaStream_t s, const TcConv *conv);
-}  // namespace
-
-size_t tc_workspace_bytes(const silcu_gemm_args &a) { return workspace_bytes(a, false); }
-size_t tc_loss_workspace_bytes(const silcu_gemm_args &a) { return workspace_bytes(a, true); }
-silcu_status tc_run(const silcu_gemm_args &a, void *ws, size_t wsb, cudaStream_t s, const TcConv *conv) {
-  return run(a, kLossNone, nullptr, ws, wsb, s, conv);
-}
-silcu_status tc_run_loss(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs &loss, void *ws, size_t wsb,
-                         cudaStream_t s) {
-  return run(a, kind, &loss, ws, wsb, s, nullptr);
-}
-
-silcu_status split_rows(const float *src, int64_t rs, int64_t ks, int64_t rows, int64_t K, int64_t Kp, float *hi,
-                        float *lo, cudaStream_t s) {
-  if ((rows + 31) / 32 > 65535) return fail(SILCU_UNSUPPORTED, "split: extent too large");
-  const dim3 g(uint32_t((Kp + 31) / 32), uint32_t((rows + 31) / 32), 1);
-  pack_split<<<g, 256, 0, s>>>(src, nullptr, rs, ks, 0, 1, 0, rows, K, Kp, hi, lo);
-  return check_launch("split");
+  return bytes + partial_bytes(a, tc_plan(a));
 }
 
 silcu_status split_contiguous(const float *src, uint64_t n, float *hi, float *lo, cudaStream_t s) {
@@ -1006,17 +950,15 @@ silcu_status split_contiguous(const float *src, uint64_t n, float *hi, float *lo
   return check_launch("split");
 }
 
-namespace {
-silcu_status run(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs *loss, void *ws, size_t wsb,
-                 cudaStream_t s, const TcConv *conv) {
+silcu_status tc_run(const silcu_gemm_args &a, void *ws, size_t wsb, cudaStream_t s, const TcConv *conv) {
   const int64_t Kp = padded_k(a.K > 0 ? a.K : 1);
-  const size_t need = workspace_bytes(a, kind != kLossNone);
+  const size_t need = tc_workspace_bytes(a);
   if (need > 256 && (!ws || wsb < need))
     return fail(SILCU_WORKSPACE_TOO_SMALL, "sgemm(tc): workspace %zu < %zu", wsb, need);
   if (a.M > (1 << 30) || a.N > (1 << 30) || Kp > (1 << 30))
     return fail(SILCU_UNSUPPORTED, "sgemm(tc): extent >= 2^30");
   const int64_t nb = total_batch(a), bin = a.batch_inner > 1 ? a.batch_inner : 1, bout = a.batch;
-  const TcPlan plan = tc_plan(a, kind != kLossNone);
+  const TcPlan plan = tc_plan(a);
   const bool pair = plan.pair;
   const int BN = plan.BN;
   const int64_t tiles_n = plan.tiles_n, tiles_m = plan.tiles_m;
@@ -1036,7 +978,7 @@ silcu_status run(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs *lo
   if (split_out && !(aligned_view(a.C_hi, a.ldc, a.stride_c_inner, a.stride_c) &&
                      aligned_view(a.C_lo, a.ldc, a.stride_c_inner, a.stride_c)))
     return fail(SILCU_INVALID_ARGUMENT, "sgemm(tc): split output needs 16-byte aligned rows and batch strides");
-  if (!a.C && !split_out && kind != kLossStats) return fail(SILCU_INVALID_ARGUMENT, "sgemm(tc): no output");
+  if (!a.C && !split_out) return fail(SILCU_INVALID_ARGUMENT, "sgemm(tc): no output");
 
   float *cur = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
   TcParams p;
@@ -1157,22 +1099,6 @@ silcu_status run(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs *lo
   const int64_t total = plan.full_items + split_tiles * plan.ksplit;
   silcu_status st;
   const bool split = plan.ksplit > 1;
-  if (kind != kLossNone) {
-    p.loss = *loss;
-    const int64_t units = pair ? sm_count() / 2 : sm_count();
-    const uint32_t grid = uint32_t((total < units ? total : units) * (pair ? 2 : 1));
-    auto go = [&](auto bn) {
-      constexpr int W = decltype(bn)::value;
-      if (kind == kLossStats)
-        return pair ? launch_tc<W, true, false, kLossStats>(p, grid, s)
-                    : launch_tc<W, false, false, kLossStats>(p, grid, s);
-      return pair ? launch_tc<W, true, false, kLossGrad>(p, grid, s)
-                  : launch_tc<W, false, false, kLossGrad>(p, grid, s);
-    };
-    if (BN == 256) return go(std::integral_constant<int, 256>{});
-    if (BN == 128) return go(std::integral_constant<int, 128>{});
-    return go(std::integral_constant<int, 64>{});
-  }
   if (pair) {
     const int64_t pairs = sm_count() / 2;
     const uint32_t grid = uint32_t(2 * (total < pairs ? total : pairs));
@@ -1203,7 +1129,6 @@ silcu_status run(const silcu_gemm_args &a, LossEpilogue kind, const LossArgs *lo
                                    a.C, a.ldc, c_hi, c_lo, vec);
   return check_launch("sgemm(tc) split-K finish");
 }
-}  // namespace
 
 }  // namespace silcu
 
