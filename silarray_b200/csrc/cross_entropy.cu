@@ -214,7 +214,10 @@ using lossmm::Operand;
 using lossmm::Tf32;
 
 // Of a piece's ds (and of its copied weights).
-constexpr int64_t kPieceBytes[2] = {int64_t(512) << 20, int64_t(256) << 20};  // by silcu_dtype
+// Larger pieces add to dH's planes less often, smaller ones stay nearer to the
+// L2's size: 8192 rows of bf16 (131072 columns, D 2048) 13.4 ms at 256 MB, 13.0 at
+// 128, 13.7 at 64; 16384 fp32 rows (32768 columns, D 768) 15.6 ms at 512 MB, 16.4 at 256.
+constexpr int64_t kPieceBytes[2] = {int64_t(512) << 20, int64_t(128) << 20};  // by silcu_dtype
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -235,11 +238,11 @@ int64_t piece_of(int64_t V, int64_t bytes, int dtype) {
 // Tile columns of the scores.  More than 128 rows: CTA pairs, 256.  Else one
 // CTA per tile, as wide as spreads n columns evenly over rounds of all SMs
 // (32768 columns: 147 tiles of 224 on 148 SMs instead of 128 of 256), in steps
-// of an MMA's 16 columns, or of the 64 that a store of score gradients writes.
-int score_columns(int64_t rows, int64_t n, int step) {
+// of an MMA's 16 columns.
+int score_columns(int64_t rows, int64_t n) {
   if (rows > lossmm::BM) return lossmm::BN;
   const int64_t sms = sm_count(), rounds = ceil_div(n, sms * lossmm::BN);
-  return int(up(ceil_div(n, sms * rounds), step));
+  return int(up(ceil_div(n, sms * rounds), 16));
 }
 
 bool rows16(const void *p, int64_t ld, int dtype) {
@@ -293,7 +296,7 @@ struct Forward {
     copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
     copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
     piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype) : a.V;
-    bn = score_columns(a.rows, piece, 16);
+    bn = score_columns(a.rows, piece);
     nparts = 0;
     for (int64_t v0 = 0; v0 < a.V; v0 += piece) nparts += parts(a, v0);
     part = sp.take<float2>(int64_t(nparts) * a.rows);
@@ -332,7 +335,7 @@ struct Backward {
     copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
     const int64_t of_ds = e * a.rows, of_w = copy_w ? e * up(a.D, 8) : 0;
     piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype);
-    bn = score_columns(a.rows, piece, 64);
+    bn = score_columns(a.rows, piece);
     scale = sp.take<float>(a.rows);
     h.take(sp, a.rows, a.D);
     if (copy_w) w.take(sp, piece, a.D);
@@ -461,11 +464,11 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     memset(&p, 0, sizeof(p));
     p.err = device_error_ptr();
     p.bn = b.bn;
-    bool ok = lossmm::set_problem<Ty>(p.p[0], a.rows > lossmm::BM, b.bn, a.rows, n, a.D, b.h.operand(false), w);
-    for (int h = 0; h < Ty::PARTS; h++)
-      ok = ok && tc::make_map2<T>(&p.c[h], h ? static_cast<const void *>(b.ds.lo) : b.ds.p, n, a.rows, b.lds, Ty::KROW,
-                                  32, false);
-    if (!ok) return map_error();
+    if (!lossmm::set_problem<Ty>(p.p[0], a.rows > lossmm::BM, b.bn, a.rows, n, a.D, b.h.operand(false), w))
+      return map_error();
+    p.ds[0] = b.ds.p;
+    p.ds[1] = b.ds.lo;
+    p.lds = b.lds;
     p.loss.targets = a.targets;
     p.loss.V = int32_t(a.V);
     p.loss.v0 = int32_t(v0);

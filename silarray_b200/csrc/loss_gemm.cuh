@@ -47,6 +47,30 @@ constexpr int BM = 128, BN = 256;
 enum Epilogue { kStats = 0, kScoreGrad = 1, kOut = 2 };
 enum OutMode { kDirect = 0, kPlane = 1, kPlaneAdd = 2 };
 
+// mbar_wait without its call: around a call the 128 sums of an epilogue thread
+// would have to be saved.
+__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, int *err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer();
+#pragma unroll 1
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); i++) {
+    if ((i & 63u) == 0) {
+      if (*reinterpret_cast<volatile int *>(err) != 0) return false;
+      if (globaltimer() - t0 > WAIT_NS) {
+        atomicCAS(err, 0, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
+// x rounded to tf32 as cvt.rna.tf32 does (halves away from zero), on the
+// integer pipe: the conversion took 70 of 660 us of the score gradients.
+__device__ __forceinline__ float tf32_rna_bits(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+}
+
 struct Bf16 {
   using T = __nv_bfloat16;
   static constexpr int PARTS = 1, KROW = 64, KMMA = 16;  // k in a 128-byte row, and of one MMA
@@ -98,7 +122,8 @@ struct Problem {
 
 struct __align__(64) Params {
   Problem p[2];  // kOut: up to two products in one launch
-  CUtensorMap c[2];  // score gradients' stores [part]
+  void *ds[2];       // score gradients [part]: [M, lds], lds a multiple of 64
+  int64_t lds;
   int bn;            // tile columns
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, tail, extra;
@@ -321,19 +346,9 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
       const int r0 = tl.m0 + BM * int(rank) + 32 * qr, c0 = tl.n0 + 128 * h;
       const int row = r0 + lane;
       const int cols = min(q.N, tl.n0 + bn) - c0;  // this warp's columns of the tile, up to 128 (may be <= 0)
-      // what the epilogue needs of the row arrives while the MMAs run
-      int y = -1;
-      float lse = 0.f, g = 0.f;
-      if (EPI != kOut && row < q.M) {
-        y = p.loss.targets[row];
-        if (EPI == kScoreGrad) {
-          lse = p.loss.lse[row] * kLog2e;
-          g = p.loss.scale ? p.loss.scale[row] : 1.0f;
-        }
-      }
       auto finished = [&](uint32_t t) {  // the accumulator of chunk t is complete
         const uint32_t j = t % NBUF, use = t / NBUF;
-        const bool got = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * j, use & 1, p.err, 23));
+        const bool got = __all_sync(0xffffffffu, wait_inline(tfull0 + 8 * j, use & 1, p.err, 23));
         tc_fence_after();
         return got;
       };
@@ -349,24 +364,22 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
       const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + 128 * h;
       float acc[C::MULTI ? 128 : 1];
       if constexpr (C::MULTI) {
+#pragma unroll
+        for (int i = 0; i < 128; i++) acc[i] = 0.f;
         for (int kc = tl.kb0; kc < tl.kb1; kc += C::CHUNK, cg++) {
           if (!finished(cg)) {
             ok = false;
             break;
           }
           if (cols > 0) {
+// 16 columns at a time: with 32 the sums spill, and every chunk pays for it
 #pragma unroll
-            for (int cb = 0; cb < 4; cb++) {
-              uint32_t r[32];
-              tmem_ld32_nowait(src0 + (cg % NBUF) * BN + 32 * cb, r);
+            for (int cb = 0; cb < 8; cb++) {
+              uint32_t r[16];
+              tmem_ld16_nowait(src0 + (cg % NBUF) * BN + 16 * cb, r);
               tmem_ld_wait();
-              if (kc == tl.kb0) {
 #pragma unroll
-                for (int i = 0; i < 32; i++) acc[32 * cb + i] = __uint_as_float(r[i]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; i++) acc[32 * cb + i] = __fadd_rn(acc[32 * cb + i], __uint_as_float(r[i]));
-              }
+              for (int i = 0; i < 16; i++) acc[16 * cb + i] = __fadd_rn(acc[16 * cb + i], __uint_as_float(r[i]));
             }
           }
           if (!C::BACK || kc + C::CHUNK < tl.kb1) release(cg);
@@ -387,6 +400,15 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
         ok = finished(cg++);
       }
       if (!__all_sync(0xffffffffu, ok && *reinterpret_cast<volatile int *>(p.err) == 0)) break;
+      int y = -1;
+      float lse = 0.f, g = 0.f;
+      if (EPI != kOut && row < q.M) {
+        y = p.loss.targets[row];
+        if (EPI == kScoreGrad) {
+          lse = p.loss.lse[row] * kLog2e;
+          g = p.loss.scale ? p.loss.scale[row] : 1.0f;
+        }
+      }
       constexpr bool IN_REGS = C::MULTI && !C::BACK;
       // Columns 32 cb .. 32 cb + 31 of this thread's row.
       auto block = [&](int cb, float (&v)[32]) {
@@ -429,20 +451,22 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
         if (r0 < q.M) {
           const bool counts = y >= 0 && y < p.loss.V;
           const int at = y - p.loss.v0 - c0;
-          auto stage_ready = [&] {  // the staging block's last store has read it
-            if (lane == 0) bulk_wait_read0();
-            __syncwarp();
-          };
-          auto send = [&](const CUtensorMap *map, int col) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(map, smem_u32(st), col, r0);
-              bulk_commit();
-            }
-          };
           auto put = [&](int i, uint4 v) {  // 16-byte chunk i of this lane's 128-byte row
             *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(st) + lane * 128 + 16 * (i ^ (lane & 7))) = v;
+          };
+          // The staged rows, 8 lanes each; plain stores need no wait before the next block.
+          auto send = [&](int part, int col0) {
+            constexpr int W = 16 / int(sizeof(T));
+            T *out = static_cast<T *>(p.ds[part]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const int rr = 4 * i + (lane >> 3), ch = lane & 7, col = col0 + W * ch;
+              const uint4 x =
+                  *reinterpret_cast<const uint4 *>(reinterpret_cast<char *>(st) + rr * 128 + 16 * (ch ^ (rr & 7)));
+              if (r0 + rr < q.M && col < c0 + cols) *reinterpret_cast<uint4 *>(out + int64_t(r0 + rr) * p.lds + col) = x;
+            }
+            __syncwarp();
           };
 #pragma unroll UNROLL
           for (int cb = 0; cb < 4; cb++) {
@@ -451,28 +475,26 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
               block(cb, v);
               score_gradient(v, lse, g, at - 32 * cb, counts);
               if constexpr (PARTS == 1) {  // 64 bf16 columns per 128-byte row: two blocks a store
-                if ((cb & 1) == 0) stage_ready();
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                   put(4 * (cb & 1) + i, make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
                                                    pack_bf16(v[8 * i + 4], v[8 * i + 5]),
                                                    pack_bf16(v[8 * i + 6], v[8 * i + 7])));
-                if ((cb & 1) || 32 * (cb + 1) >= cols) send(&p.c[0], c0 + 32 * (cb & ~1));
+                if ((cb & 1) || 32 * (cb + 1) >= cols) send(0, c0 + 32 * (cb & ~1));
               } else {  // the exact tf32 pair, 32 columns per row each
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
-                  stage_ready();
 #pragma unroll
                   for (int i = 0; i < 8; i++) {
                     uint32_t e[4];
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
-                      const float x = v[4 * i + t], hi = tf32_rna(x);
+                      const float x = v[4 * i + t], hi = tf32_rna_bits(x);
                       e[t] = __float_as_uint(part ? __fsub_rn(x, hi) : hi);
                     }
                     put(i, make_uint4(e[0], e[1], e[2], e[3]));
                   }
-                  send(&p.c[part], c0 + 32 * cb);
+                  send(part, c0 + 32 * cb);
                 }
               }
             }
@@ -538,10 +560,6 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
         }
       }
       if constexpr (!IN_REGS) release(cg - 1);
-    }
-    if (EPI == kScoreGrad) {
-      if (lane == 0) bulk_wait_all0();  // every store has completed before exit
-      __syncwarp();
     }
   }
   tc_fence_before();
