@@ -235,14 +235,26 @@ int64_t piece_of(int64_t V, int64_t bytes, int dtype) {
   return up(ceil_div(V, ceil_div(V, p)), 256);
 }
 
-// Tile columns of the scores.  More than 128 rows: CTA pairs, 256.  Else one
-// CTA per tile, as wide as spreads n columns evenly over rounds of all SMs
-// (32768 columns: 147 tiles of 224 on 148 SMs instead of 128 of 256), in steps
-// of an MMA's 16 columns.
-int score_columns(int64_t rows, int64_t n) {
-  if (rows > lossmm::BM) return lossmm::BN;
-  const int64_t sms = sm_count(), rounds = ceil_div(n, sms * lossmm::BN);
-  return int(up(ceil_div(n, sms * rounds), 16));
+// Tiles of the scores: 256 x 256 on CTA pairs, or 128 x bn on single CTAs.
+// Whichever takes the shortest rounds of all SMs, counting a tile by its columns
+// (below 128 an MMA costs more than its share) and single CTAs, which read B
+// once per 128 rows, at 1.1: 32768 columns of 8 rows run as 147 tiles of 224
+// instead of 128 of 256; 333 x 10007 as one round of 147 tiles of 128 x 208
+// instead of two of pairs.
+struct ScoreTiles {
+  bool pair;
+  int bn;
+};
+ScoreTiles score_tiles(int64_t rows, int64_t n) {
+  const int64_t sms = sm_count();
+  ScoreTiles best{true, lossmm::BN};
+  double cost = double(ceil_div(ceil_div(rows, 2 * lossmm::BM) * ceil_div(n, lossmm::BN), sms / 2)) * lossmm::BN;
+  for (int bn = lossmm::BN; bn >= 16; bn -= 16) {
+    const int64_t rounds = ceil_div(ceil_div(rows, lossmm::BM) * ceil_div(n, bn), sms);
+    const double c = 1.1 * double(rounds) * (bn >= 128 ? bn : 0.5 * (bn + 128));
+    if (c < cost) cost = c, best = ScoreTiles{false, bn};
+  }
+  return best;
 }
 
 bool rows16(const void *p, int64_t ld, int dtype) {
@@ -286,7 +298,8 @@ struct Copy {
 template <typename Ty>
 struct Forward {
   int64_t piece;
-  int bn, nparts;
+  ScoreTiles tiles;
+  int nparts;
   bool copy_h, copy_w;  // operands that are not read in place
   Copy<Ty> h, w;
   float2 *part;
@@ -296,7 +309,7 @@ struct Forward {
     copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
     copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
     piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype) : a.V;
-    bn = score_columns(a.rows, piece);
+    tiles = score_tiles(a.rows, piece);
     nparts = 0;
     for (int64_t v0 = 0; v0 < a.V; v0 += piece) nparts += parts(a, v0);
     part = sp.take<float2>(int64_t(nparts) * a.rows);
@@ -306,7 +319,7 @@ struct Forward {
     if (copy_w) w.take(sp, piece, a.D);
   }
   int64_t columns(const Args &a, int64_t v0) const { return a.V - v0 < piece ? a.V - v0 : piece; }
-  int parts(const Args &a, int64_t v0) const { return 2 * int(ceil_div(columns(a, v0), bn)); }
+  int parts(const Args &a, int64_t v0) const { return 2 * int(ceil_div(columns(a, v0), tiles.bn)); }
 };
 
 // One of the two products of ds, with M x N results from sums of K: its K is
@@ -320,10 +333,60 @@ struct Gradient {
   int64_t tiles() const { return ceil_div(M, 2 * lossmm::BM) * ceil_div(N, lossmm::BN); }
 };
 
+// Time of both products in one launch, in k of one tile: the slowest SM pair's
+// items (work_at; `first` has the longer ones), each with its epilogue, and
+// the planes' traffic.  One k of a tile takes 131072 flops of a pair's share of
+// the measured 1.4 PFLOP/s (7 ns; six times that in 3xTF32).
+double out_time(const Gradient &first, const Gradient &second, bool tf32) {
+  const int64_t units = sm_count() / 2;
+  const int64_t n0 = first.wanted ? first.tiles() * first.split : 0;
+  const int64_t n1 = second.wanted ? second.tiles() * second.split : 0;
+  if (n0 + n1 == 0) return 0.0;
+  const int64_t u = n0 + n1 < units ? n0 + n1 : units, tail = n0 % u, low = u - tail;
+  const double epilogue = tf32 ? 128.0 : 512.0, ns = tf32 ? 42.0 : 7.0;
+  const double c0 = double(first.K) / first.split, c1 = double(second.K) / second.split;
+  const int64_t extra = n1 && tail ? int64_t(c0 / c1 + 0.5) : 0;
+  auto rounds = [&](int64_t begin, int64_t step) { return begin < n1 ? ceil_div(n1 - begin, step) : 0; };
+  const int64_t after = tail ? extra * low : 0;
+  const int64_t high = rounds(after, u);  // unit 0: after the short units' extra rounds
+  double time = double(ceil_div(n0, u)) * (c0 + epilogue) + double(high) * (c1 + epilogue);
+  if (tail) {
+    const int64_t own = rounds(0, low) < extra ? rounds(0, low) : extra;
+    const double t = double(n0 / u) * (c0 + epilogue) + double(own + rounds(after + tail, u)) * (c1 + epilogue);
+    if (t > time) time = t;
+  }
+  double bytes = 0.0;
+  for (const Gradient *g : {&first, &second})
+    if (g->wanted) bytes += 8.0 * (g->split - 1) * double(g->M) * double(g->N);
+  return time * ns + bytes / 6500.0;
+}
+
+// Cuts the products' K so that the launch ends evenly: long sums of few tiles
+// (few rows, or a short vocabulary) and the last round of many.  At least 512 k
+// a part.
+void choose_splits(Gradient &dh, Gradient &dw, bool tf32) {
+  static const int counts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
+  double best = -1.0;
+  int bh = 1, bw = 1;
+  for (const int h : counts) {
+    if (h > 1 && (!dh.wanted || dh.K < 512 * int64_t(h))) break;
+    for (const int w : counts) {
+      if (w > 1 && (!dw.wanted || dw.K < 512 * int64_t(w))) break;
+      dh.split = h;
+      dw.split = w;
+      const bool dw_first = dw.K / w > dh.K / h;
+      const double t = out_time(dw_first ? dw : dh, dw_first ? dh : dw, tf32);
+      if (best < 0.0 || t < best) best = t, bh = h, bw = w;
+    }
+  }
+  dh.split = bh;
+  dw.split = bw;
+}
+
 template <typename Ty>
 struct Backward {
   int64_t piece, lds;  // lds: row stride of ds
-  int bn;
+  ScoreTiles score;
   bool copy_w;
   float *scale;
   Copy<Ty> h, w;       // H with left-out rows zero; a piece of W
@@ -335,7 +398,7 @@ struct Backward {
     copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
     const int64_t of_ds = e * a.rows, of_w = copy_w ? e * up(a.D, 8) : 0;
     piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype);
-    bn = score_columns(a.rows, piece);
+    score = score_tiles(a.rows, piece);
     scale = sp.take<float>(a.rows);
     h.take(sp, a.rows, a.D);
     if (copy_w) w.take(sp, piece, a.D);
@@ -343,15 +406,7 @@ struct Backward {
     lds = ds.dp;
     dh.M = a.rows, dh.N = a.D, dh.K = piece, dh.wanted = a.dH;
     dw.M = piece, dw.N = a.D, dw.K = a.rows, dw.wanted = a.dW;
-    // Parts of K where a single item would be more than half of what each SM
-    // pair has to do altogether; at least 512 k in each.
-    const double units = sm_count() / 2;
-    const double load = ((dh.wanted ? double(dh.tiles()) * dh.K : 0.0) + (dw.wanted ? double(dw.tiles()) * dw.K : 0.0)) / units;
-    for (Gradient *g : {&dh, &dw}) {
-      const double item = load / 2 > 512.0 ? load / 2 : 512.0;
-      const int64_t want = int64_t(double(g->K) / item) + (double(g->K) > item * double(int64_t(double(g->K) / item)));
-      g->split = int(want < 1 ? 1 : want > 32 ? 32 : want);
-    }
+    choose_splits(dh, dw, Ty::PARTS == 2);
     dh.direct = dh.split == 1 && piece == a.V;  // else pieces add up in the planes
     dw.direct = dw.split == 1;
     for (Gradient *g : {&dh, &dw})
@@ -362,9 +417,19 @@ struct Backward {
 // ---------------------------------------------------------------------- run
 silcu_status map_error() { return fail(SILCU_CUDA_ERROR, "cross_entropy: cuTensorMapEncodeTiled failed"); }
 
+// Few rows need no whole tile of A: 8 rows of 32768 x 4096 bf16 take 51 us with
+// boxes of 8 rows, 60 with boxes of 128 that are zeros for the most part.
+template <typename Ty>
+bool set_scores(lossmm::Params &p, const ScoreTiles &t, int64_t rows, int64_t n, int64_t D, const Operand &h,
+                const Operand &w) {
+  p.bn = t.bn;
+  p.rows_a = !t.pair && rows < lossmm::BM ? int(up(rows, 8)) : lossmm::BM;
+  return lossmm::set_problem<Ty>(p.p[0], t.pair, t.bn, p.rows_a, rows, n, D, h, w);
+}
+
 template <typename Ty, int EPI>
-silcu_status scores(lossmm::Params &p, int64_t rows, cudaStream_t s) {
-  return rows > lossmm::BM ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
+silcu_status scores(lossmm::Params &p, bool pair, cudaStream_t s) {
+  return pair ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
 }
 
 template <typename T>
@@ -392,8 +457,7 @@ silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
     }
     lossmm::Params p;
     memset(&p, 0, sizeof(p));
-    if (!lossmm::set_problem<Ty>(p.p[0], a.rows > lossmm::BM, f.bn, a.rows, n, a.D, h, w)) return map_error();
-    p.bn = f.bn;
+    if (!set_scores<Ty>(p, f.tiles, a.rows, n, a.D, h, w)) return map_error();
     p.part0 = part0;
     p.err = device_error_ptr();
     p.loss.targets = a.targets;
@@ -401,7 +465,7 @@ silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
     p.loss.v0 = int32_t(v0);
     p.loss.part = f.part;
     p.loss.target_score = f.target_score;
-    if ((st = scores<Ty, lossmm::kStats>(p, a.rows, s)) != SILCU_OK) return st;
+    if ((st = scores<Ty, lossmm::kStats>(p, f.tiles.pair, s)) != SILCU_OK) return st;
     part0 += f.parts(a, v0);
   }
   loss_finish<<<uint32_t((a.rows + 31) / 32), 1024, 0, s>>>(f.part, f.nparts, a.rows, a.targets, int(a.V),
@@ -463,9 +527,7 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     lossmm::Params p;
     memset(&p, 0, sizeof(p));
     p.err = device_error_ptr();
-    p.bn = b.bn;
-    if (!lossmm::set_problem<Ty>(p.p[0], a.rows > lossmm::BM, b.bn, a.rows, n, a.D, b.h.operand(false), w))
-      return map_error();
+    if (!set_scores<Ty>(p, b.score, a.rows, n, a.D, b.h.operand(false), w)) return map_error();
     p.ds[0] = b.ds.p;
     p.ds[1] = b.ds.lo;
     p.lds = b.lds;
@@ -474,7 +536,7 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     p.loss.v0 = int32_t(v0);
     p.loss.lse = a.lse;
     p.loss.scale = shared ? nullptr : b.scale;
-    if ((st = scores<Ty, lossmm::kScoreGrad>(p, a.rows, s)) != SILCU_OK) return st;
+    if ((st = scores<Ty, lossmm::kScoreGrad>(p, b.score.pair, s)) != SILCU_OK) return st;
 
     // Both products of ds in one launch, the one with the longer items first.
     memset(&p, 0, sizeof(p));
@@ -487,12 +549,12 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
       if (!(is_dw ? b.dw : b.dh).wanted) continue;
       lossmm::Problem &q = p.p[count++];
       if (is_dw) {
-        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
+        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
           return map_error();
         set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, alpha, a.D,
                    ceil_div(a.rows, BK));
       } else {
-        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
+        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
         set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, alpha, a.D, ceil_div(n, BK));
       }
     }

@@ -65,6 +65,15 @@ __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, int *
   return true;
 }
 
+// Adds to an earlier launch's sum.  Nothing else adds to this element in this
+// launch, so the order is fixed; done in the L2, no thread waits for the old sum
+// (as loads and stores, which may alias, 32 in a row cost a tile 15 us and more).
+__device__ __forceinline__ void red_add4(float *p, const float4 &v) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z),
+               "f"(v.w)
+               : "memory");
+}
+
 // x rounded to tf32 as cvt.rna.tf32 does (halves away from zero), on the
 // integer pipe: the conversion took 70 of 660 us of the score gradients.
 __device__ __forceinline__ float tf32_rna_bits(float x) {
@@ -98,6 +107,9 @@ struct Cfg {
   static constexpr int NBUF = 2;
   // stages per accumulation chunk; MULTI: a tile may take several, which meet in registers
   static constexpr bool MULTI = Ty::PARTS == 2 || EPI == kStats;
+  // Columns that join the sums at a time: 32 leave the tf32 sums no registers, and
+  // what spills there every chunk pays for (score gradients 660 -> 477 us with 16).
+  static constexpr int LD = Ty::PARTS == 2 ? 16 : 32;
   // The sum goes back to TMEM for an epilogue that has no registers beside it
   // (with the 128 sums in registers the tf32 score gradients spill 2.8 KB a thread).
   static constexpr bool BACK = MULTI && EPI == kScoreGrad;
@@ -125,6 +137,7 @@ struct __align__(64) Params {
   void *ds[2];       // score gradients [part]: [M, lds], lds a multiple of 64
   int64_t lds;
   int bn;            // tile columns
+  int rows_a;        // rows of A's boxes (single CTAs; the rest of a tile is never stored)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, tail, extra;
   LossArgs loss;
@@ -228,7 +241,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
     if (lane == 0) {
       uint32_t kbg = 0;
       bool ok = true;
-      const uint32_t bytes = SUBS * PARTS * (TILE_A + (PAIR ? TILE_B : bn * 128)) * (PAIR ? 2 : 1);
+      const uint32_t bytes = SUBS * PARTS * ((PAIR ? TILE_A : p.rows_a * 128) + (PAIR ? TILE_B : bn * 128)) * (PAIR ? 2 : 1);
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
         const Problem &q = p.p[w.prob];
         const Tile tl = tile_of<C>(q, bn, w.item);
@@ -372,14 +385,14 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
             break;
           }
           if (cols > 0) {
-// 16 columns at a time: with 32 the sums spill, and every chunk pays for it
 #pragma unroll
-            for (int cb = 0; cb < 8; cb++) {
-              uint32_t r[16];
-              tmem_ld16_nowait(src0 + (cg % NBUF) * BN + 16 * cb, r);
+            for (int cb = 0; cb < 128 / C::LD; cb++) {
+              uint32_t r[C::LD];
+              tmem_ld_nowait(src0 + (cg % NBUF) * BN + C::LD * cb, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; i++) acc[16 * cb + i] = __fadd_rn(acc[16 * cb + i], __uint_as_float(r[i]));
+              for (int i = 0; i < C::LD; i++)
+                acc[C::LD * cb + i] = __fadd_rn(acc[C::LD * cb + i], __uint_as_float(r[i]));
             }
           }
           if (!C::BACK || kc + C::CHUNK < tl.kb1) release(cg);
@@ -519,14 +532,12 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
 #pragma unroll
               for (int i = 0; i < 8; i++) {
                 const int rr = 4 * i + (lane >> 3), ch = lane & 7, col = col0 + 4 * ch;
-                float4 x = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * (ch ^ (rr & 7)));
+                const float4 x = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * (ch ^ (rr & 7)));
                 if (r0 + rr < q.M && col < q.N) {
                   float *dst = out + int64_t(r0 + rr) * q.ldo + col;
                   if (q.mode == kPlaneAdd) {
-                    const float4 o = *reinterpret_cast<const float4 *>(dst);
-                    x.x += o.x, x.y += o.y, x.z += o.z, x.w += o.w;
-                  }
-                  if (q.mode != kDirect || (q.vec && col + 4 <= q.N)) {  // a plane's rows hold whole vectors
+                    red_add4(dst, x);
+                  } else if (q.mode != kDirect || (q.vec && col + 4 <= q.N)) {  // a plane's rows hold whole vectors
                     *reinterpret_cast<float4 *>(dst) = x;
                   } else {
                     const float e[4] = {x.x, x.y, x.z, x.w};
@@ -593,7 +604,8 @@ bool operand_map(CUtensorMap (&m)[2], const Operand &o, int64_t extent, int64_t 
 }
 
 template <typename Ty>
-bool set_problem(Problem &q, bool pair, int bn, int64_t M, int64_t N, int64_t K, const Operand &a, const Operand &b) {
+bool set_problem(Problem &q, bool pair, int bn, int rows_a, int64_t M, int64_t N, int64_t K, const Operand &a,
+                 const Operand &b) {
   q.M = int(M);
   q.N = int(N);
   q.K = int(K);
@@ -602,7 +614,7 @@ bool set_problem(Problem &q, bool pair, int bn, int64_t M, int64_t N, int64_t K,
   q.tiles_n = int((N + bn - 1) / bn);
   q.ksplit = 1;
   q.amn = a.mn;
-  return operand_map<Ty>(q.a, a, M, K, BM) && operand_map<Ty>(q.b, b, N, K, pair ? BN / 2 : bn);
+  return operand_map<Ty>(q.a, a, M, K, rows_a) && operand_map<Ty>(q.b, b, N, K, pair ? BN / 2 : bn);
 }
 
 inline int64_t items_of(const Problem &q) { return int64_t(q.tiles_m) * q.tiles_n * q.ksplit; }
