@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCtasPerSm = 6;
+constexpr int kCtasPerSm = 5;  // what the registers hold; a sixth would run as a tail (700 MB: 120 us, 105 with 5)
 constexpr uint64_t kMinSpan = 256;  // elements; a launch of few elements uses few warps
 
 template <int CAP>

@@ -27,22 +27,23 @@ struct LossArgs {
   const float *scale;      // backward: [rows] gradient of each row's loss, or null = 1
 };
 
-// Folds 32 scores, of which the first `valid` exist, into (m, l).  The terms
-// are 2^(s log2 e - m log2 e): one multiply-add and one ex2 each.  A row of
-// -inf alone keeps l = 0; NaN and +inf make l NaN.
-__device__ __forceinline__ void softmax_fold(const float (&v)[32], int valid, float &m, float &l) {
-  float mx = m;
+// (m, l) of 128 scores, of which the first `valid` exist.  The terms are
+// 2^(s log2 e - m log2 e): one multiply-add and one ex2 each, in chains short
+// enough that two warps per scheduler keep up.  A row of -inf alone has l = 0;
+// NaN and +inf make l NaN.
+__device__ __forceinline__ void softmax_part(const float (&v)[128], int valid, float &m, float &l) {
+  float mx[8], a[8];
 #pragma unroll
-  for (int i = 0; i < 32; i++)
-    if (i < valid) mx = fmaxf(mx, v[i]);
-  const float neg = mx == -INFINITY ? 0.f : -mx * kLog2e;
-  l *= ex2(fmaf(m, kLog2e, neg));  // m = -inf: 0
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < 8; i++) mx[i] = -INFINITY, a[i] = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; i++)
-    if (i < valid) a[i & 3] += ex2(fmaf(v[i], kLog2e, neg));
-  l += (a[0] + a[1]) + (a[2] + a[3]);
-  m = mx;
+  for (int i = 0; i < 128; i++)
+    if (i < valid) mx[i & 7] = fmaxf(mx[i & 7], v[i]);
+  m = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+  const float neg = m == -INFINITY ? 0.f : -m * kLog2e;
+#pragma unroll
+  for (int i = 0; i < 128; i++)
+    if (i < valid) a[i & 7] += ex2(fmaf(v[i], kLog2e, neg));
+  l = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
 }
 
 // The scores' gradients in place of the scores.  `at` = the target's column

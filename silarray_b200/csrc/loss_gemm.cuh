@@ -377,25 +377,32 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
       const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + 128 * h;
       float acc[C::MULTI ? 128 : 1];
       if constexpr (C::MULTI) {
+        int kc = tl.kb0;
+        if constexpr (PARTS == 1) {  // the first chunk lands in the sums' registers
+          ok = finished(cg);
+          if (ok && cols > 0) {
 #pragma unroll
-        for (int i = 0; i < 128; i++) acc[i] = 0.f;
-        for (int kc = tl.kb0; kc < tl.kb1; kc += C::CHUNK, cg++) {
-          if (!finished(cg)) {
-            ok = false;
-            break;
+            for (int cb = 0; cb < 128; cb += 32) tmem_ld_cols<32>(src0 + (cg % NBUF) * BN + cb, acc, cb);
+            tmem_ld_done(acc);
           }
-          if (cols > 0) {
+          if ((kc += C::CHUNK) < tl.kb1) release(cg++);
+        } else {
 #pragma unroll
-            for (int cb = 0; cb < 128 / C::LD; cb++) {
-              uint32_t r[C::LD];
-              tmem_ld_nowait(src0 + (cg % NBUF) * BN + C::LD * cb, r);
-              tmem_ld_wait();
+          for (int i = 0; i < 128; i++) acc[i] = 0.f;
+        }
+        while (ok && kc < tl.kb1) {
+          ok = finished(cg);
+          if (ok && cols > 0) {
 #pragma unroll
-              for (int i = 0; i < C::LD; i++)
-                acc[C::LD * cb + i] = __fadd_rn(acc[C::LD * cb + i], __uint_as_float(r[i]));
+            for (int cb = 0; cb < 128; cb += C::LD) {
+              float r[C::LD];
+              tmem_ld_cols<C::LD>(src0 + (cg % NBUF) * BN + cb, r);
+              tmem_ld_done(r);
+#pragma unroll
+              for (int i = 0; i < C::LD; i++) acc[cb + i] = __fadd_rn(acc[cb + i], r[i]);
             }
           }
-          if (!C::BACK || kc + C::CHUNK < tl.kb1) release(cg);
+          if ((kc += C::CHUNK) < tl.kb1) release(cg++);
         }
         if constexpr (C::BACK) {
           if (ok && cols > 0) {
@@ -404,14 +411,17 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
               uint32_t r[32];
 #pragma unroll
               for (int i = 0; i < 32; i++) r[i] = __float_as_uint(acc[32 * cb + i]);
-              tmem_st32_cols(src0 + ((cg - 1) % NBUF) * BN + 32 * cb, r);
+              tmem_st32_cols(src0 + (cg % NBUF) * BN + 32 * cb, r);
             }
             tmem_st_wait();
           }
+        } else {
+          release(cg);
         }
       } else {
-        ok = finished(cg++);
+        ok = finished(cg);
       }
+      cg++;
       if (!__all_sync(0xffffffffu, ok && *reinterpret_cast<volatile int *>(p.err) == 0)) break;
       int y = -1;
       float lse = 0.f, g = 0.f;
@@ -423,40 +433,33 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
         }
       }
       constexpr bool IN_REGS = C::MULTI && !C::BACK;
-      // Columns 32 cb .. 32 cb + 31 of this thread's row.
+      // Columns 32 cb .. 32 cb + 31 of this thread's row, for cb = 0, 1, 2, 3 in
+      // turn; from TMEM the next ones are on their way while these are used.
+      float ahead[IN_REGS ? 1 : 32];
+      if constexpr (!IN_REGS) tmem_ld_cols<32>(src0 + ((cg - 1) % NBUF) * BN, ahead);
       auto block = [&](int cb, float (&v)[32]) {
         if constexpr (IN_REGS) {
 #pragma unroll
           for (int i = 0; i < 32; i++) v[i] = acc[32 * cb + i];
         } else {
-          uint32_t r[32];
-          tmem_ld32_nowait(src0 + ((cg - 1) % NBUF) * BN + 32 * cb, r);
-          tmem_ld_wait();
+          tmem_ld_done(ahead);
 #pragma unroll
-          for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+          for (int i = 0; i < 32; i++) v[i] = ahead[i];
+          if (cb < 3) tmem_ld_cols<32>(src0 + ((cg - 1) % NBUF) * BN + 32 * (cb + 1), ahead);
         }
       };
       constexpr int UNROLL = IN_REGS ? 4 : 1;
 
       if constexpr (EPI == kStats) {
         if (r0 < q.M) {
-          float m = -INFINITY, l = 0.f;
+          float m, l;
+          if (cols >= 128) softmax_part(acc, 128, m, l);
+          else softmax_part(acc, cols, m, l);
           const int at = y - p.loss.v0 - c0;  // the target among this thread's columns
-          const bool mine = y >= 0 && y < p.loss.V && at >= 0 && at < cols;
+          if (y >= 0 && y < p.loss.V && at >= 0 && at < min(cols, 128)) {
 #pragma unroll
-          for (int cb = 0; cb < 4; cb++) {
-            const int valid = cols - 32 * cb;
-            if (valid > 0) {
-              float v[32];
-              block(cb, v);
-              if (valid >= 32) softmax_fold(v, 32, m, l);
-              else softmax_fold(v, valid, m, l);
-              if (mine && (at >> 5) == cb) {
-#pragma unroll
-                for (int i = 0; i < 32; i++)
-                  if (i == (at & 31)) p.loss.target_score[row] = v[i];
-              }
-            }
+            for (int i = 0; i < 128; i++)
+              if (i == at) p.loss.target_score[row] = acc[i];
           }
           if (row < q.M) p.loss.part[int64_t(p.part0 + 2 * (tl.n0 / bn) + h) * q.M + row] = make_float2(m, l);
         }
@@ -570,7 +573,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
           }
         }
       }
-      if constexpr (!IN_REGS) release(cg - 1);
+      if constexpr (!IN_REGS) {
+        tmem_ld_wait();  // a load that no block took
+        release(cg - 1);
+      }
     }
   }
   tc_fence_before();

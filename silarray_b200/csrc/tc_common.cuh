@@ -323,17 +323,42 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[3
       : "r"(taddr));
 }
 
-__device__ __forceinline__ void tmem_ld_nowait(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32_nowait(taddr, r); }
-__device__ __forceinline__ void tmem_ld_nowait(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
+// N = 16 or 32 columns of this lane's TMEM row as floats, from r[at] on; not
+// to be read before tmem_ld_done.
+template <int N, int SIZE>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&r)[SIZE], int at = 0) {
+  static_assert(N == 16 || N == 32, "columns");
+  if constexpr (N == 16)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(r[at + 0]), "=f"(r[at + 1]), "=f"(r[at + 2]), "=f"(r[at + 3]), "=f"(r[at + 4]), "=f"(r[at + 5]),
+          "=f"(r[at + 6]), "=f"(r[at + 7]), "=f"(r[at + 8]), "=f"(r[at + 9]), "=f"(r[at + 10]), "=f"(r[at + 11]),
+          "=f"(r[at + 12]), "=f"(r[at + 13]), "=f"(r[at + 14]), "=f"(r[at + 15])
+        : "r"(taddr));
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[at + 0]), "=f"(r[at + 1]), "=f"(r[at + 2]), "=f"(r[at + 3]), "=f"(r[at + 4]), "=f"(r[at + 5]),
+          "=f"(r[at + 6]), "=f"(r[at + 7]), "=f"(r[at + 8]), "=f"(r[at + 9]), "=f"(r[at + 10]), "=f"(r[at + 11]),
+          "=f"(r[at + 12]), "=f"(r[at + 13]), "=f"(r[at + 14]), "=f"(r[at + 15]), "=f"(r[at + 16]), "=f"(r[at + 17]),
+          "=f"(r[at + 18]), "=f"(r[at + 19]), "=f"(r[at + 20]), "=f"(r[at + 21]), "=f"(r[at + 22]), "=f"(r[at + 23]),
+          "=f"(r[at + 24]), "=f"(r[at + 25]), "=f"(r[at + 26]), "=f"(r[at + 27]), "=f"(r[at + 28]), "=f"(r[at + 29]),
+          "=f"(r[at + 30]), "=f"(r[at + 31])
+        : "r"(taddr));
 }
 
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// The loads so far are complete, and r is read only after this.
+template <int SIZE>
+__device__ __forceinline__ void tmem_ld_done(float (&r)[SIZE]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < SIZE; i++) asm volatile("" : "+f"(r[i]));
+}
 
 // 32 columns of this lane's TMEM row, and the wait for such stores.
 __device__ __forceinline__ void tmem_st32_cols(uint32_t taddr, const uint32_t (&r)[32]) {
