@@ -324,3 +324,56 @@ class Block:
         gpu.gemm(h, self.w1_t, M=T, N=f, K=d, trans_b=True, bias=self.b1, act="relu", no_c=True, C_split=ff,
                  acc_chunk_k=ck)
         gpu.gemm(ff, self.w2_t, outs, M=T, N=d, K=f, trans_b=True, bias=self.b2, residual=r1, acc_chunk_k=ck)
+
+
+def init_head(vocab, d_model, seed=0):
+    """A loss head's parameters: gamma 1, beta 0, W [vocab, d_model] ~ N(0, 0.02^2)."""
+    rng = np.random.default_rng(seed)
+    return {"g": np.ones(d_model, np.float32), "be": np.zeros(d_model, np.float32),
+            "w": _normal(rng, (vocab, d_model), 0.02)}
+
+
+class LossHead:
+    """What follows the last block in training: the final layer_norm, the
+    vocabulary projection with its mean cross entropy, their gradients, and
+    the clipping of the parameters' gradients.
+
+        loss = head.forward(block.forward(x), targets)   # 0-d device tensor
+        dx = head.backward()                              # gradient of the block's output
+        norm = head.clip(1.0)                             # head.grads, in place
+
+    Activations and W are fp32, or bf16 with dtype=torch.bfloat16 (gamma, beta
+    and their gradients stay fp32).  Targets are int32; one outside
+    [0, vocab) leaves its row out.  A whole step can be captured in a CUDA graph."""
+
+    def __init__(self, params, device="cuda", dtype=torch.float32, eps=1e-5):
+        t = lambda a, dt: torch.from_numpy(np.ascontiguousarray(a)).to(device, dt)  # noqa: E731
+        self.gamma, self.beta = t(params["g"], torch.float32), t(params["be"], torch.float32)
+        self.w = t(params["w"], dtype)
+        self.eps = eps
+        self.grads = {"g": torch.empty_like(self.gamma), "be": torch.empty_like(self.beta),
+                      "w": torch.empty_like(self.w)}
+        self._grad_list = gpu.TensorList(self.grads.values())
+        self._saved = None
+
+    def forward(self, x, targets):
+        """Mean loss of x [rows, d_model] against targets [rows]."""
+        h, mean, rstd = gpu.layer_norm_forward(x, gamma=self.gamma, beta=self.beta, eps=self.eps)
+        loss, lse = gpu.linear_cross_entropy(h, self.w, targets)
+        self._saved = (x, targets, h, mean, rstd, lse)
+        return loss
+
+    def backward(self, dloss=None, dresidual=None):
+        """Gradient of the last forward's x (dresidual is added to it); the
+        parameters' gradients are written to self.grads.  dloss: 0-d, None = 1."""
+        if self._saved is None:
+            raise RuntimeError("LossHead: backward without a forward")
+        x, targets, h, mean, rstd, lse = self._saved
+        dh, _ = gpu.linear_cross_entropy_backward(h, self.w, targets, lse, dloss=dloss, dW=self.grads["w"])
+        dx, _, _ = gpu.layer_norm_backward(dh, x, mean, rstd, self.gamma, dresidual=dresidual, din=dh,
+                                           dgamma=self.grads["g"], dbeta=self.grads["be"])
+        return dx
+
+    def clip(self, max_norm):
+        """Clips self.grads by their common norm; returns it (0-d)."""
+        return gpu.clip_grad_norm(self._grad_list, max_norm)
