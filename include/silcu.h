@@ -398,7 +398,7 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
  * dloss, or dloss / count); NULL = 1.  dH / dW may be NULL when not wanted;
  * they are written, not added to.  f32 products are 3xTF32; with bf16, ds is
  * rounded to bf16 once (the products' operand type) and sums are fp32.
- * dH may not overlap H, nor dW W. */
+ * The gradients may not overlap the operands. */
 typedef enum silcu_reduction { SILCU_REDUCE_MEAN = 0, SILCU_REDUCE_SUM = 1, SILCU_REDUCE_NONE = 2 } silcu_reduction;
 typedef struct silcu_cross_entropy_args {
   const void *H, *W;
@@ -425,7 +425,8 @@ silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args 
  * host at call time.  clip multiplies every element by
  * min(1, max_norm / (norm + eps)), a factor rounded to fp32: in place when outputs_host is
  * NULL, else into outputs_host[i], a tensor of the same size and dtype that
- * either is tensors[i] or overlaps none of the list.  A norm that is NaN makes
+ * either is tensors[i] or overlaps none of the list.  Clipped tensors do not
+ * overlap one another (for the norm alone they may: each counts).  A norm that is NaN makes
  * every element NaN; an infinite one makes finite elements 0. */
 typedef struct silcu_tensor {
   void *data;

@@ -597,6 +597,9 @@ silcu_status check_pointers(const char *what, const Args &a) {
   if (!a.H || !a.W || !a.targets || !a.lse) return fail(SILCU_INVALID_ARGUMENT, "%s: null pointer", what);
   for (const void *p : {a.H, a.W, static_cast<const void *>(a.dH), static_cast<const void *>(a.dW)})
     if (reinterpret_cast<uintptr_t>(p) & mask) return fail(SILCU_INVALID_ARGUMENT, "%s: misaligned pointer", what);
+  for (const void *p : {static_cast<const void *>(a.targets), static_cast<const void *>(a.lse),
+                        static_cast<const void *>(a.loss), static_cast<const void *>(a.dloss)})
+    if (reinterpret_cast<uintptr_t>(p) & 3) return fail(SILCU_INVALID_ARGUMENT, "%s: misaligned pointer", what);
   return SILCU_OK;
 }
 
@@ -667,6 +670,8 @@ silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args 
     return SILCU_OK;
   }
   if ((st = check_pointers(what, a)) != SILCU_OK) return st;
+  if (a.dH == a.H || a.dW == a.W || a.dH == a.W || a.dW == a.H)
+    return fail(SILCU_INVALID_ARGUMENT, "%s: a gradient overlaps an operand", what);
   if ((st = check_space(what, a, 1, workspace, workspace_bytes)) != SILCU_OK) return st;
   Space sp{align256(workspace)};
   return a.dtype == SILCU_BF16 ? backward(a, Backward<Bf16>(a, sp), s) : backward(a, Backward<Tf32>(a, sp), s);

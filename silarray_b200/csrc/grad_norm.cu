@@ -230,7 +230,8 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) clip_scale(const __grid_constant__ ListArgs<CAP> a) {
   const double norm = total_norm(a.all, a.nparts);
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm) *a.norm = float(norm);
-  double c = double(a.max_norm) / (norm + double(a.eps));
+  const double below = norm + double(a.eps);
+  double c = below > 0.0 || !(below == below) ? double(a.max_norm) / below : 1.0;  // all zeros stay zeros
   if (c > 1.0) c = 1.0;  // a NaN stays one
   const uint64_t worker = uint64_t(gridDim.x - 1 - blockIdx.x) * kWarps + (threadIdx.x >> 5);
   for_span(a, worker, [&](int t, uint64_t first, uint64_t n) {
@@ -364,7 +365,8 @@ silcu_status silcu_grad_norm(const silcu_tensor *tensors, size_t count, float *n
   using namespace silcu;
   silcu_status st = check_list("grad_norm", tensors, nullptr, count);
   if (st != SILCU_OK) return st;
-  if (!norm) return fail(SILCU_INVALID_ARGUMENT, "grad_norm: null pointer");
+  if (!norm || (reinterpret_cast<uintptr_t>(norm) & 3))
+    return fail(SILCU_INVALID_ARGUMENT, "grad_norm: null or misaligned pointer");
   st = check_workspace("grad_norm", tensors, count, workspace, workspace_bytes);
   if (st != SILCU_OK) return st;
   cudaStream_t s = as_stream(stream);
@@ -380,7 +382,8 @@ silcu_status silcu_clip_grad_norm(const silcu_tensor *tensors, void *const *outp
   using namespace silcu;
   silcu_status st = check_list("clip_grad_norm", tensors, outputs, count);
   if (st != SILCU_OK) return st;
-  if (!norm) return fail(SILCU_INVALID_ARGUMENT, "clip_grad_norm: null pointer");
+  if (!norm || (reinterpret_cast<uintptr_t>(norm) & 3))
+    return fail(SILCU_INVALID_ARGUMENT, "clip_grad_norm: null or misaligned pointer");
   if (!(max_norm >= 0.f) || !(eps >= 0.f))
     return fail(SILCU_INVALID_ARGUMENT, "clip_grad_norm: max_norm and eps must not be negative");
   st = check_workspace("clip_grad_norm", tensors, count, workspace, workspace_bytes);

@@ -29,6 +29,8 @@
 //                      warp per row (151 registers, one CTA per SM); 8190 x 4096
 //                      bf16: 72 us with the sums in shared memory instead.
 // All sums are fp32 in an order fixed by the shape and the SM count.
+#include <initializer_list>
+
 #include "elem.cuh"
 
 namespace silcu {
@@ -671,6 +673,17 @@ silcu_status check_extent(const char *what, size_t rows, size_t cols, int dtype)
   return SILCU_OK;
 }
 
+// Row pointers and float pointers lie on their elements' boundaries (null ones pass).
+silcu_status check_aligned(const char *what, int dtype, std::initializer_list<const void *> rows,
+                           std::initializer_list<const void *> floats) {
+  const uintptr_t mask = dtype_bytes(dtype) - 1;
+  for (const void *p : rows)
+    if (reinterpret_cast<uintptr_t>(p) & mask) return fail(SILCU_INVALID_ARGUMENT, "%s: misaligned pointer", what);
+  for (const void *p : floats)
+    if (reinterpret_cast<uintptr_t>(p) & 3) return fail(SILCU_INVALID_ARGUMENT, "%s: misaligned pointer", what);
+  return SILCU_OK;
+}
+
 }  // namespace
 }  // namespace silcu
 
@@ -684,6 +697,8 @@ silcu_status silcu_layer_norm_forward(const void *in, void *out, float *mean, fl
   silcu_status st = check_extent("layer_norm_forward", rows, cols, dtype);
   if (st != SILCU_OK) return st;
   if (!in || !out || !gamma || !beta) return fail(SILCU_INVALID_ARGUMENT, "layer_norm_forward: null pointer");
+  st = check_aligned("layer_norm_forward", dtype, {in, out}, {mean, rstd, gamma, beta});
+  if (st != SILCU_OK) return st;
   LnArgs a = {};
   a.in = in;
   a.out = out;
@@ -721,6 +736,8 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
   silcu_status st = check_extent("layer_norm_backward", rows, cols, dtype);
   if (st != SILCU_OK) return st;
   if (!dgamma || !dbeta) return fail(SILCU_INVALID_ARGUMENT, "layer_norm_backward: null pointer");
+  st = check_aligned("layer_norm_backward", dtype, {dout, in, dresidual, din}, {mean, rstd, gamma, dgamma, dbeta, workspace});
+  if (st != SILCU_OK) return st;
   cudaStream_t s = as_stream(stream);
   uint32_t grid = 0;
   if (rows) {
@@ -729,8 +746,6 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
     const size_t need = silcu_layer_norm_backward_workspace_bytes(rows, cols, dtype);
     if (!workspace || workspace_bytes < need)
       return fail(SILCU_WORKSPACE_TOO_SMALL, "layer_norm_backward: workspace %zu < %zu", workspace_bytes, need);
-    if (reinterpret_cast<uintptr_t>(workspace) & 3)
-      return fail(SILCU_INVALID_ARGUMENT, "layer_norm_backward: misaligned workspace");
     LnArgs a = {};
     a.in = in;
     a.dout = dout;

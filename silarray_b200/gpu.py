@@ -627,19 +627,20 @@ def linear_cross_entropy_backward(H, W, targets, lse, dloss=None, reduction="mea
 class TensorList:
     """The gradients of a model as grad_norm and clip_grad_norm take them: a
     list of fp32 / bf16 CUDA tensors, laid out once for the C call (and again
-    when a tensor's storage has moved)."""
+    when a tensor has another storage or size)."""
 
     def __init__(self, tensors):
         self.tensors = list(tensors)
         if not self.tensors:
             raise ValueError("TensorList: no tensors")
-        self._addresses = None
+        self._addresses = self._counts = None
         self._layout()
 
     def _layout(self):
-        """Checks the tensors and fills the C arrays, unless no address changed."""
+        """Checks the tensors and fills the C arrays, unless nothing moved."""
         addresses = [t.data_ptr() for t in self.tensors]
-        if addresses == self._addresses:
+        counts = [t.numel() for t in self.tensors]
+        if addresses == self._addresses and counts == self._counts:
             return self
         n = len(self.tensors)
         self.array = (_lib.Tensor * n)()
@@ -648,15 +649,34 @@ class TensorList:
             k = _kind(t)
             if i == 0:
                 self.device, self.index = t.device, t.get_device()
-            _at(f"TensorList tensor {i}", t, t.dtype, t.numel(), self.index)
-            self.array[i] = _lib.Tensor(addresses[i], t.numel(), k)
-        self.shapes = [(t.dtype, t.numel()) for t in self.tensors]
+            _at(f"TensorList tensor {i}", t, t.dtype, counts[i], self.index)
+            self.array[i] = _lib.Tensor(addresses[i], counts[i], k)
+        self.shapes = [(t.dtype, c) for t, c in zip(self.tensors, counts)]
+        self.spans = sorted((a, a + c * t.element_size())
+                            for a, c, t in zip(addresses, counts, self.tensors) if c)
         self.nbytes = lib().silcu_grad_norm_workspace_bytes(self.array, n)
-        self._addresses = addresses
+        self._addresses, self._counts = addresses, counts
+        self._clips_into = None
         return self
 
     def __len__(self):
         return len(self.tensors)
+
+    def _check_clip(self, out):
+        """Refuses to clip into `out` (a TensorList, maybe this one) where tensors overlap."""
+        if self._clips_into is out.spans:
+            return  # these two have been checked
+        if out is not self and (self.shapes != out.shapes or self.index != out.index):
+            raise ValueError("clip_grad_norm: OUT must match the tensors in number, size, dtype and device")
+        # an output may be its own input; apart from that all spans are disjoint
+        mine, theirs = set(self.spans), set(out.spans)
+        spans = sorted(mine | theirs)
+        starts = {a for a, _ in theirs}
+        if len(mine) < len(self.spans) or len(theirs) < len(out.spans) \
+                or any(a[1] > b[0] for a, b in zip(spans, spans[1:])) \
+                or any(c and p != q and p in starts for p, q, c in zip(self._addresses, out._addresses, self._counts)):
+            raise ValueError("clip_grad_norm: tensors overlap")
+        self._clips_into = out.spans
 
 
 def _list(tensors):
@@ -677,12 +697,9 @@ def clip_grad_norm(tensors, max_norm, OUT=None, eps=1e-6):
     into OUT (a list or TensorList of the same shapes); returns the norm before
     clipping as a 0-d device tensor."""
     tl = _list(tensors)
-    pointers = None
-    if OUT is not None:
-        out = _list(OUT)
-        if tl.shapes != out.shapes or tl.index != out.index:
-            raise ValueError("clip_grad_norm: OUT must match the tensors in number, size, dtype and device")
-        pointers = out.pointers
+    out = tl if OUT is None else _list(OUT)
+    tl._check_clip(out)
+    pointers = None if OUT is None else out.pointers
     norm = torch.empty((), dtype=_F32, device=tl.device)
     buf, ws = _scratch(tl.nbytes, tl.device)
     _launch(lib().silcu_clip_grad_norm, tl.index, tl.array, pointers, len(tl), max_norm, eps, norm.data_ptr(), ws,

@@ -259,6 +259,24 @@ def test_norm_of_bad_values(cuda):
     zero = [torch.zeros(100, device="cuda")]
     assert float(gpu.clip_grad_norm(zero, 1.0)) == 0 and bool((zero[0] == 0).all())
     assert float(gpu.clip_grad_norm([torch.ones(4, device="cuda")], 0.0)) == 2.0
+    gpu.clip_grad_norm(zero, 0.0, eps=0.0)
+    assert bool((zero[0] == 0).all())
+
+
+def test_overlapping_lists(cuda):
+    """The norm counts a tensor as often as it is listed; clipping refuses
+    tensors, or outputs, that overlap."""
+    buf = torch.ones(1000, device="cuda")
+    a, b = buf[:600], buf[500:]
+    assert abs(float(gpu.grad_norm([a, a])) - 1200 ** 0.5) <= 6 * U * 1200 ** 0.5
+    c, d = torch.ones(600, device="cuda"), torch.ones(500, device="cuda")
+    for tensors, out in (([a, b], None), ([a, a], None), ([a, d], [b[:0].new_empty(600), a[:500]]), ([c, d], [a, b]),
+                         ([c, c.clone()], [c.clone(), c])):
+        with pytest.raises(ValueError):
+            gpu.clip_grad_norm(tensors, 1.0, OUT=out)
+    tl = gpu.TensorList([c, d])
+    gpu.clip_grad_norm(tl, 1.0, OUT=[c, torch.empty_like(d)])  # an output that is its own input is fine
+    assert bool((buf == 1).all()) and bool((d == 1).all()) and bool((c < 1).all())
 
 
 def test_tensor_list_follows_its_tensors(cuda):

@@ -94,6 +94,11 @@ def test_layer_norm_refusals(lib):
     assert b(*args, C.c_void_p((1 << 20) + 2), need, None) == 1
     assert b(P, P, None, P, P, None, P, P, P, 100, 768, 0, P, need, None) == 1
     assert b(P, P, P, P, P, None, P, None, P, 100, 768, 0, P, need, None) == 1
+    odd, half = C.c_void_p((1 << 20) + 1), C.c_void_p((1 << 20) + 2)
+    assert f(half, P, None, None, P, P, 4, 8, 1e-5, 0, None) == 1 and f(P, odd, None, None, P, P, 4, 8, 1e-5, 1, None) == 1
+    assert f(P, P, half, None, P, P, 4, 8, 1e-5, 1, None) == 1
+    assert b(P, P, P, P, P, half, P, P, P, 100, 768, 0, P, need, None) == 1
+    assert b(P, P, P, P, P, None, P, half, P, 100, 768, 1, P, need, None) == 1
     assert lib.silcu_layer_norm_backward_workspace_bytes(0, 768, 0) == 0
 
 
@@ -120,8 +125,8 @@ def test_gradient_list_refusals(lib):
 
 def _loss_args(**kw):
     a = _lib.CrossEntropyArgs()
-    for k in ("H", "W", "targets", "loss", "lse", "dH", "dW"):
-        setattr(a, k, 1 << 20)
+    for i, k in enumerate(("dH", "W", "targets", "loss", "lse", "H", "dW")):
+        setattr(a, k, (1 << 20) + (i << 16))
     a.rows, a.V, a.D, a.ldh, a.ldw, a.lddh, a.lddw = 10, 100, 64, 64, 64, 64, 64
     for k, v in kw.items():
         setattr(a, k, v)
@@ -142,7 +147,8 @@ def test_cross_entropy_refusals(lib):
     assert fwd(None, P, big, None) == 1 and bwd(None, P, big, None) == 1
     a = _loss_args(loss=0)
     assert fwd(C.byref(a), P, big, None) == 1
-    for kw in (dict(lddh=63), dict(lddw=1), dict(dH=(1 << 20) + 1)):
+    for kw in (dict(lddh=63), dict(lddw=1), dict(dH=(1 << 20) + 1), dict(dloss=(1 << 20) + 2), dict(targets=(1 << 20) + 2),
+               dict(dW=(1 << 20) + (1 << 16)), dict(dH=(1 << 20) + (5 << 16))):
         a = _loss_args(**kw)
         assert bwd(C.byref(a), P, big, None) == 1, kw
     for dtype in (0, 1):
