@@ -242,23 +242,40 @@ int64_t piece_of(int64_t V, int64_t bytes, int dtype) {
 // instead of 128 of 256; 333 x 10007 as one round of 147 tiles of 128 x 208
 // instead of two of pairs.
 struct ScoreTiles {
-  bool pair;
+  bool pair, raw;
   int bn;
 };
-ScoreTiles score_tiles(int64_t rows, int64_t n) {
+ScoreTiles score_tiles(int64_t rows, int64_t n, bool raw) {
   const int64_t sms = sm_count();
-  ScoreTiles best{true, lossmm::BN};
+  if (raw) {  // each tile reads its A from shared memory again: wide ones, and 16 columns' time for starting
+    ScoreTiles best{false, true, 32};
+    double cost = 0.0;
+    for (int bn = 32; bn <= lossmm::BN; bn += 16) {
+      const double c = double(ceil_div(ceil_div(rows, lossmm::BM) * ceil_div(n, bn), sms)) * (bn + 16);
+      if (bn == 32 || c < cost) cost = c, best.bn = bn;
+    }
+    return best;
+  }
+  ScoreTiles best{true, false, lossmm::BN};
   double cost = double(ceil_div(ceil_div(rows, 2 * lossmm::BM) * ceil_div(n, lossmm::BN), sms / 2)) * lossmm::BN;
   for (int bn = lossmm::BN; bn >= 16; bn -= 16) {
     const int64_t rounds = ceil_div(ceil_div(rows, lossmm::BM) * ceil_div(n, bn), sms);
     const double c = 1.1 * double(rounds) * (bn >= 128 ? bn : 0.5 * (bn + 128));
-    if (c < cost) cost = c, best = ScoreTiles{false, bn};
+    if (c < cost) cost = c, best = ScoreTiles{false, false, bn};
   }
   return best;
 }
 
 bool rows16(const void *p, int64_t ld, int dtype) {
   return aligned16(p) && (ld * int64_t(dtype_bytes(dtype))) % 16 == 0;
+}
+
+// fp32 W is read as it is, and split inside the products, where few rows make
+// reading it the larger part of the work.
+constexpr int64_t kRawRows = 128;
+template <typename Ty>
+bool raw_w(const Args &a) {
+  return Ty::PARTS == 2 && a.rows <= kRawRows && rows16(a.W, a.ldw, a.dtype);
 }
 
 // A bump allocator over the workspace (or, with none, its size).
@@ -307,9 +324,9 @@ struct Forward {
 
   Forward(const Args &a, Space &sp) {
     copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
-    copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
+    copy_w = Ty::PARTS == 2 ? !raw_w<Ty>(a) : !rows16(a.W, a.ldw, a.dtype);
     piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype) : a.V;
-    tiles = score_tiles(a.rows, piece);
+    tiles = score_tiles(a.rows, piece, raw_w<Ty>(a));
     nparts = 0;
     for (int64_t v0 = 0; v0 < a.V; v0 += piece) nparts += parts(a, v0);
     part = sp.take<float2>(int64_t(nparts) * a.rows);
@@ -330,20 +347,24 @@ struct Gradient {
   int split = 1;
   bool wanted, direct;
   float *planes = nullptr;
-  int64_t tiles() const { return ceil_div(M, 2 * lossmm::BM) * ceil_div(N, lossmm::BN); }
+  int tile = 2 * lossmm::BM;  // rows and columns of a tile (CTA pairs: 256; single CTAs: 128)
+  int64_t tiles() const { return ceil_div(M, tile) * ceil_div(N, tile); }
+  int64_t units() const { return tile == lossmm::BM ? sm_count() : sm_count() / 2; }
 };
 
 // Time of both products in one launch, in k of one tile: the slowest SM pair's
 // items (work_at; `first` has the longer ones), each with its epilogue, and
 // the planes' traffic.  One k of a tile takes 131072 flops of a pair's share of
-// the measured 1.4 PFLOP/s (7 ns; six times that in 3xTF32).
+// the measured 1.4 PFLOP/s (7 ns; half that for a tile of 128 on one SM; six
+// times that in 3xTF32).
 double out_time(const Gradient &first, const Gradient &second, bool tf32) {
-  const int64_t units = sm_count() / 2;
+  const int64_t units = first.units();
   const int64_t n0 = first.wanted ? first.tiles() * first.split : 0;
   const int64_t n1 = second.wanted ? second.tiles() * second.split : 0;
   if (n0 + n1 == 0) return 0.0;
   const int64_t u = n0 + n1 < units ? n0 + n1 : units, tail = n0 % u, low = u - tail;
-  const double epilogue = tf32 ? 128.0 : 512.0, ns = tf32 ? 42.0 : 7.0;
+  const double epilogue = tf32 ? 128.0 : 512.0;
+  const double ns = (tf32 ? 42.0 : 7.0) * (first.tile == lossmm::BM ? 0.5 : 1.0);
   const double c0 = double(first.K) / first.split, c1 = double(second.K) / second.split;
   const int64_t extra = n1 && tail ? int64_t(c0 / c1 + 0.5) : 0;
   auto rounds = [&](int64_t begin, int64_t step) { return begin < n1 ? ceil_div(n1 - begin, step) : 0; };
@@ -395,10 +416,10 @@ struct Backward {
 
   Backward(const Args &a, Space &sp) {
     const int64_t e = int64_t(Ty::PARTS) * sizeof(typename Ty::T);
-    copy_w = Ty::PARTS == 2 || !rows16(a.W, a.ldw, a.dtype);
+    copy_w = Ty::PARTS == 2 ? !raw_w<Ty>(a) : !rows16(a.W, a.ldw, a.dtype);
     const int64_t of_ds = e * a.rows, of_w = copy_w ? e * up(a.D, 8) : 0;
     piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype);
-    score = score_tiles(a.rows, piece);
+    score = score_tiles(a.rows, piece, raw_w<Ty>(a));
     scale = sp.take<float>(a.rows);
     h.take(sp, a.rows, a.D);
     if (copy_w) w.take(sp, piece, a.D);
@@ -406,6 +427,7 @@ struct Backward {
     lds = ds.dp;
     dh.M = a.rows, dh.N = a.D, dh.K = piece, dh.wanted = a.dH;
     dw.M = piece, dw.N = a.D, dw.K = a.rows, dw.wanted = a.dW;
+    if (score.raw) dh.tile = dw.tile = lossmm::BM;
     choose_splits(dh, dw, Ty::PARTS == 2);
     dh.direct = dh.split == 1 && piece == a.V;  // else pieces add up in the planes
     dw.direct = dw.split == 1;
@@ -417,6 +439,13 @@ struct Backward {
 // ---------------------------------------------------------------------- run
 silcu_status map_error() { return fail(SILCU_CUDA_ERROR, "cross_entropy: cuTensorMapEncodeTiled failed"); }
 
+// The ring and the epilogue warps' columns of a RAW launch with p.bn and p.rows_a.
+void set_raw(lossmm::Params &p) {
+  const int stages = 192 * 1024 / (2 * 128 * (p.rows_a + p.bn));
+  p.stages = stages < 8 ? stages : 8;
+  p.half = int(up((p.bn + 1) / 2, 32));
+}
+
 // Few rows need no whole tile of A: 8 rows of 32768 x 4096 bf16 take 51 us with
 // boxes of 8 rows, 60 with boxes of 128 that are zeros for the most part.
 template <typename Ty>
@@ -424,12 +453,22 @@ bool set_scores(lossmm::Params &p, const ScoreTiles &t, int64_t rows, int64_t n,
                 const Operand &w) {
   p.bn = t.bn;
   p.rows_a = !t.pair && rows < lossmm::BM ? int(up(rows, 8)) : lossmm::BM;
+  if (t.raw) set_raw(p);
   return lossmm::set_problem<Ty>(p.p[0], t.pair, t.bn, p.rows_a, rows, n, D, h, w);
 }
 
 template <typename Ty, int EPI>
-silcu_status scores(lossmm::Params &p, bool pair, cudaStream_t s) {
-  return pair ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
+silcu_status scores(lossmm::Params &p, const ScoreTiles &t, cudaStream_t s) {
+  if constexpr (Ty::PARTS == 2)
+    if (t.raw) return lossmm::launch<Ty, EPI, false, true>(p, 1, s);
+  return t.pair ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
+}
+
+template <typename Ty>
+silcu_status products(lossmm::Params &p, bool pairs, int count, cudaStream_t s) {
+  if constexpr (Ty::PARTS == 2)
+    if (!pairs) return lossmm::launch<Ty, lossmm::kOut, false, true>(p, count, s);
+  return lossmm::launch<Ty, lossmm::kOut, true>(p, count, s);
 }
 
 template <typename T>
@@ -465,7 +504,7 @@ silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
     p.loss.v0 = int32_t(v0);
     p.loss.part = f.part;
     p.loss.target_score = f.target_score;
-    if ((st = scores<Ty, lossmm::kStats>(p, f.tiles.pair, s)) != SILCU_OK) return st;
+    if ((st = scores<Ty, lossmm::kStats>(p, f.tiles, s)) != SILCU_OK) return st;
     part0 += f.parts(a, v0);
   }
   loss_finish<<<uint32_t((a.rows + 31) / 32), 1024, 0, s>>>(f.part, f.nparts, a.rows, a.targets, int(a.V),
@@ -536,12 +575,15 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     p.loss.v0 = int32_t(v0);
     p.loss.lse = a.lse;
     p.loss.scale = shared ? nullptr : b.scale;
-    if ((st = scores<Ty, lossmm::kScoreGrad>(p, b.score.pair, s)) != SILCU_OK) return st;
+    if ((st = scores<Ty, lossmm::kScoreGrad>(p, b.score, s)) != SILCU_OK) return st;
 
     // Both products of ds in one launch, the one with the longer items first.
     memset(&p, 0, sizeof(p));
     p.err = device_error_ptr();
-    p.bn = lossmm::BN;
+    const bool pairs = !b.score.raw;
+    p.bn = pairs ? lossmm::BN : lossmm::BM;
+    p.rows_a = lossmm::BM;
+    if (!pairs) set_raw(p);
     int count = 0;
     w.mn = true;
     const bool dw_first = b.dw.K / b.dw.split > b.dh.K / b.dh.split;
@@ -549,16 +591,16 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
       if (!(is_dw ? b.dw : b.dh).wanted) continue;
       lossmm::Problem &q = p.p[count++];
       if (is_dw) {
-        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
+        if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
           return map_error();
         set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, alpha, a.D,
                    ceil_div(a.rows, BK));
       } else {
-        if (!lossmm::set_problem<Ty>(q, true, lossmm::BN, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
+        if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
         set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, alpha, a.D, ceil_div(n, BK));
       }
     }
-    if ((st = lossmm::launch<Ty, lossmm::kOut, true>(p, count, s)) != SILCU_OK) return st;
+    if ((st = products<Ty>(p, pairs, count, s)) != SILCU_OK) return st;
     if (b.dw.wanted && !b.dw.direct) {
       st = finish_planes<Ty>(b.dw, n, a.D, alpha, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, s);
       if (st != SILCU_OK) return st;

@@ -33,6 +33,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <limits.h>
 
 #include "elem.cuh"
 #include "loss_epilogue.cuh"
@@ -80,6 +81,11 @@ __device__ __forceinline__ float tf32_rna_bits(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
 }
 
+// What the tensor core reads of x as a tf32 operand.
+__device__ __forceinline__ float tf32_trunc(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+}
+
 struct Bf16 {
   using T = __nv_bfloat16;
   static constexpr int PARTS = 1, KROW = 64, KMMA = 16;  // k in a 128-byte row, and of one MMA
@@ -91,16 +97,17 @@ struct Tf32 {
   static constexpr uint32_t FORMAT = (2u << 7) | (2u << 10);
 };
 
-template <typename Ty, int EPI, bool PAIR>
+template <typename Ty, int EPI, bool PAIR, bool RAW = false>
 struct Cfg {
+  static_assert(!RAW || (Ty::PARTS == 2 && !PAIR), "raw operands: tf32 on single CTAs");
   static constexpr int TM = PAIR ? 2 * BM : BM;
   static constexpr int ROWS_B = PAIR ? BN / 2 : BN;  // B columns held per CTA
   static constexpr int SUBS = PAIR && Ty::PARTS == 1 ? 2 : 1;  // 128-byte-row tiles of each operand per stage
   static constexpr int BK = SUBS * Ty::KROW;
   static constexpr int TILE_A = BM * 128, TILE_B = ROWS_B * 128;
   static constexpr int STAGE_BYTES = SUBS * Ty::PARTS * (TILE_A + TILE_B);
-  static constexpr int STAGES = 192 * 1024 / STAGE_BYTES;
-  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int RING_BYTES = 192 * 1024;
+  static constexpr int STAGES = RAW ? 8 : RING_BYTES / STAGE_BYTES;  // RAW: at most, see Params::stages
   static constexpr int EPI_WARPS = 8;
   static constexpr int SMEM_BYTES = RING_BYTES + EPI_WARPS * 4096 + 1024 + 512;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
@@ -126,6 +133,7 @@ struct Problem {
   int M, N, K, tiles_m, tiles_n;
   int ksplit;              // each tile's K range in this many parts (kOut; part i -> plane i)
   int amn;                 // kOut: A is stored with the M index contiguous
+  int raw;                 // RAW kernels: B is plain fp32 (b[0]), split in shared memory
   int mode, vec;           // vec: kDirect rows are 16-byte aligned
   void *out;
   int64_t ldo, plane;      // row stride; elements from one plane to the next
@@ -138,6 +146,8 @@ struct __align__(64) Params {
   int64_t lds;
   int bn;            // tile columns
   int rows_a;        // rows of A's boxes (single CTAs; the rest of a tile is never stored)
+  int half;          // columns of an epilogue warp (RAW; else 128)
+  int stages;        // ring stages (RAW)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, tail, extra;
   LossArgs loss;
@@ -191,19 +201,28 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
 }
 
 // BMN: B is stored with the N index contiguous (kOut; A's order is Problem::amn).
-template <typename Ty, int EPI, bool PAIR>
-__global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __grid_constant__ Params p) {
-  using C = Cfg<Ty, EPI, PAIR>;
+//
+// RAW: B may be plain fp32.  Its tile is the hi operand as it stands (the
+// tensor core reads the upper 19 bits of a value), and the epilogue warps, idle
+// while the MMAs run, write the remainders beside it.  For few rows, where the
+// time is that of reading W, this spares writing and reading a split copy.
+// Stages are as large as the tile needs.
+template <typename Ty, int EPI, bool PAIR, bool RAW>
+__global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(const __grid_constant__ Params p) {
+  using C = Cfg<Ty, EPI, PAIR, RAW>;
   using T = typename Ty::T;
   constexpr bool BMN = EPI == kOut;
-  constexpr int STAGES = C::STAGES, NBUF = C::NBUF, PARTS = Ty::PARTS, SUBS = C::SUBS;
-  constexpr int TILE_A = C::TILE_A, TILE_B = C::TILE_B, SUB_BYTES = PARTS * (TILE_A + TILE_B);
+  constexpr int NBUF = C::NBUF, PARTS = Ty::PARTS, SUBS = C::SUBS;
+  const int TILE_A = RAW ? p.rows_a * 128 : C::TILE_A, TILE_B = RAW ? p.bn * 128 : C::TILE_B;
+  const int SUB_BYTES = PARTS * (TILE_A + TILE_B), STAGE_BYTES = SUBS * SUB_BYTES;
+  const uint32_t STAGES = RAW ? uint32_t(p.stages) : uint32_t(C::STAGES);
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::RING_BYTES + C::EPI_WARPS * 4096);
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2 * NBUF);
-  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
-  const uint32_t tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + NBUF);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * C::STAGES + 2 * NBUF);
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + C::STAGES);
+  const uint32_t tfull0 = smem_u32(bars + 2 * C::STAGES), tempty0 = smem_u32(bars + 2 * C::STAGES + NBUF);
+  const uint32_t ready0 = smem_u32(bars + 2 * C::STAGES + 2 * NBUF);  // RAW: the stage's remainders are written
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -211,9 +230,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
   const int bn = PAIR ? BN : p.bn;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; s++) {
+    for (int s = 0; s < C::STAGES; s++) {
       mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 1);
+      if (RAW) mbar_init(ready0 + 8 * s, C::EPI_WARPS);
     }
     for (int j = 0; j < NBUF; j++) {
       mbar_init(tfull0 + 8 * j, 1);
@@ -242,6 +262,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
       uint32_t kbg = 0;
       bool ok = true;
       const uint32_t bytes = SUBS * PARTS * ((PAIR ? TILE_A : p.rows_a * 128) + (PAIR ? TILE_B : bn * 128)) * (PAIR ? 2 : 1);
+      const int boxes_b = RAW ? bn / Ty::KROW : C::MN_BOXES_B;
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
         const Problem &q = p.p[w.prob];
         const Tile tl = tile_of<C>(q, bn, w.item);
@@ -249,14 +270,14 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
         const bool amn = EPI == kOut && q.amn;
         for (int kb = tl.kb0; kb < tl.kb1; kb++, kbg++) {
           const uint32_t s = kbg % STAGES, ph = (kbg / STAGES) & 1;
-          if (kbg >= uint32_t(STAGES) && !mbar_try_wait(empty0 + 8 * s, ph ^ 1) &&
+          if (kbg >= STAGES && !mbar_try_wait(empty0 + 8 * s, ph ^ 1) &&
               !mbar_wait(empty0 + 8 * s, ph ^ 1, p.err, 21)) {
             ok = false;
             break;
           }
           // a pair's bytes all complete on the even CTA's barrier
           const uint32_t bar = PAIR ? mapa_shared(full0 + 8 * s, 0) : full0 + 8 * s;
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, bytes);
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, RAW && q.raw ? bytes - TILE_B : bytes);
           auto load = [&](uint32_t dst, const CUtensorMap *map, int c0, int c1) {
             if (PAIR) tma_load_2d_pair(dst, map, bar, c0, c1);
             else tma_load_2d(dst, map, bar, c0, c1);
@@ -264,7 +285,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
 #pragma unroll
           for (int u = 0; u < SUBS; u++) {
             const int kc = kb * C::BK + u * Ty::KROW;
-            uint32_t dst = smem_u32(smem + s * C::STAGE_BYTES + u * SUB_BYTES);
+            uint32_t dst = smem_u32(smem + s * STAGE_BYTES + u * SUB_BYTES);
 #pragma unroll
             for (int h = 0; h < PARTS; h++, dst += TILE_A) {
               if (amn) {
@@ -276,9 +297,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
             }
 #pragma unroll
             for (int h = 0; h < PARTS; h++, dst += TILE_B) {
+              if (RAW && q.raw && h == 1) break;
               if (BMN) {
 #pragma unroll
-                for (int i = 0; i < C::MN_BOXES_B; i++) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
+                for (int i = 0; i < boxes_b; i++) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
               } else {
                 load(dst, &q.b[h], kc, nb);
               }
@@ -289,7 +311,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {  // the pair's MMAs are issued by the even CTA
-      uint32_t kbg = 0, cg = 0;
+      uint32_t kbg = 0, cg = 0, raw_uses = 0;  // raw_uses: parity of each slot's raw uses so far
       bool ok = true;
       const uint32_t base = smem_u32(smem);
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
@@ -311,14 +333,17 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
           const uint32_t acc = tmem + j * BN;
           for (int kb = c0; kb < c1; kb++, kbg++) {
             const uint32_t s = kbg % STAGES, ph = (kbg / STAGES) & 1;
-            if (!mbar_try_wait(full0 + 8 * s, ph) && !mbar_wait(full0 + 8 * s, ph, p.err, 22)) {
+            if ((!mbar_try_wait(full0 + 8 * s, ph) && !mbar_wait(full0 + 8 * s, ph, p.err, 22)) ||
+                (RAW && q.raw && !mbar_try_wait(ready0 + 8 * s, (raw_uses >> s) & 1) &&
+                 !mbar_wait(ready0 + 8 * s, (raw_uses >> s) & 1, p.err, 26))) {
               ok = false;
               break;
             }
+            if (RAW && q.raw) raw_uses ^= 1u << s;
             tc_fence_after();
 #pragma unroll
             for (int u = 0; u < SUBS; u++) {
-              const uint32_t off = (s * C::STAGE_BYTES + u * SUB_BYTES) >> 4;
+              const uint32_t off = (s * STAGE_BYTES + u * SUB_BYTES) >> 4;
 #pragma unroll
               for (int kk = 0; kk < Ty::KROW / Ty::KMMA; kk++) {
                 const uint64_t a = adesc + uint64_t(off + kk * astep), b = bdesc + uint64_t(off + kk * bstep);
@@ -351,14 +376,42 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
   } else {
     const int qr = warp & 3, h = (warp - 2) >> 2;
     float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
-    uint32_t cg = 0;
+    const int half = RAW ? p.half : 128;
+    uint32_t cg = 0, kbe = 0;
     bool ok = true;
     for (int k = 0; ok && work_at(p, unit, k, w); k++) {
       const Problem &q = p.p[w.prob];
       const Tile tl = tile_of<C>(q, bn, w.item);
-      const int r0 = tl.m0 + BM * int(rank) + 32 * qr, c0 = tl.n0 + 128 * h;
+      const int r0 = tl.m0 + BM * int(rank) + 32 * qr, c0 = tl.n0 + half * h;
       const int row = r0 + lane;
-      const int cols = min(q.N, tl.n0 + bn) - c0;  // this warp's columns of the tile, up to 128 (may be <= 0)
+      // this warp's columns of the tile, 128 at most in use (may be <= 0)
+      const int cols = min(min(q.N, tl.n0 + bn), RAW ? c0 + half : INT_MAX) - c0;
+      // RAW: the next `n` stages' remainders x - tf32(x) of a raw B, for the MMAs.
+      // Every warp sees every raw use of a slot, so no barrier is ever more than
+      // one phase ahead of it.
+      auto remainders = [&](int n) {
+        if (!q.raw) {
+          kbe += n;
+          return true;
+        }
+        for (int i = 0; i < n; i++, kbe++) {
+          const uint32_t s = kbe % STAGES;
+          if (!__all_sync(0xffffffffu, wait_inline(full0 + 8 * s, (kbe / STAGES) & 1, p.err, 25))) return false;
+          float4 *hi = reinterpret_cast<float4 *>(smem + s * STAGE_BYTES + 2 * TILE_A), *lo = hi + TILE_B / 16;
+          for (int e = int(threadIdx.x) - 64; e < TILE_B / 16; e += 32 * C::EPI_WARPS) {
+            float4 x = hi[e];
+            x.x = __fsub_rn(x.x, tf32_trunc(x.x));
+            x.y = __fsub_rn(x.y, tf32_trunc(x.y));
+            x.z = __fsub_rn(x.z, tf32_trunc(x.z));
+            x.w = __fsub_rn(x.w, tf32_trunc(x.w));
+            lo[e] = x;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ready0 + 8 * s);
+        }
+        return true;
+      };
       auto finished = [&](uint32_t t) {  // the accumulator of chunk t is complete
         const uint32_t j = t % NBUF, use = t / NBUF;
         const bool got = __all_sync(0xffffffffu, wait_inline(tfull0 + 8 * j, use & 1, p.err, 23));
@@ -374,7 +427,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
           else mbar_arrive(bar);
         }
       };
-      const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + 128 * h;
+      const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + half * h;
       float acc[C::MULTI ? 128 : 1];
       if constexpr (C::MULTI) {
         int kc = tl.kb0;
@@ -390,8 +443,11 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
 #pragma unroll
           for (int i = 0; i < 128; i++) acc[i] = 0.f;
         }
+        if (RAW) ok = remainders(min(C::CHUNK, tl.kb1 - kc));
         while (ok && kc < tl.kb1) {
-          ok = finished(cg);
+          // the next chunk's remainders before this chunk's sums: its MMAs can start
+          if (RAW && kc + C::CHUNK < tl.kb1) ok = remainders(min(C::CHUNK, tl.kb1 - kc - C::CHUNK));
+          ok = ok && finished(cg);
           if (ok && cols > 0) {
 #pragma unroll
             for (int cb = 0; cb < 128; cb += C::LD) {
@@ -593,14 +649,14 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR>::THREADS, 1) gemm(const __g
 // An operand in memory: [MN, k] rows, or with `mn` [k, MN] rows; the row
 // stride in elements.  Pointers and row strides are multiples of 16 bytes.
 struct Operand {
-  const void *p, *lo;  // lo: tf32 only
+  const void *p, *lo;  // lo: the tf32 pair's (null for bf16 and raw fp32)
   int64_t ld;
   bool mn;
 };
 
 template <typename Ty>
 bool operand_map(CUtensorMap (&m)[2], const Operand &o, int64_t extent, int64_t K, int rows) {
-  for (int h = 0; h < Ty::PARTS; h++) {
+  for (int h = 0; h < (o.lo ? 2 : 1); h++) {
     const void *p = h ? o.lo : o.p;
     const bool ok = o.mn ? make_map2<typename Ty::T>(&m[h], p, extent, K, o.ld, Ty::KROW, Ty::KROW, Ty::PARTS == 2)
                          : make_map2<typename Ty::T>(&m[h], p, K, extent, o.ld, Ty::KROW, rows, false);
@@ -620,19 +676,20 @@ bool set_problem(Problem &q, bool pair, int bn, int rows_a, int64_t M, int64_t N
   q.tiles_n = int((N + bn - 1) / bn);
   q.ksplit = 1;
   q.amn = a.mn;
+  q.raw = Ty::PARTS == 2 && !b.lo;
   return operand_map<Ty>(q.a, a, M, K, rows_a) && operand_map<Ty>(q.b, b, N, K, pair ? BN / 2 : bn);
 }
 
 inline int64_t items_of(const Problem &q) { return int64_t(q.tiles_m) * q.tiles_n * q.ksplit; }
 
-template <typename Ty, int EPI, bool PAIR>
+template <typename Ty, int EPI, bool PAIR, bool RAW = false>
 silcu_status launch(Params &p, int problems, cudaStream_t s) {
-  using C = Cfg<Ty, EPI, PAIR>;
+  using C = Cfg<Ty, EPI, PAIR, RAW>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm<Ty, EPI, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(gemm<Ty, EPI, PAIR, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                C::SMEM_BYTES);
     if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "cross_entropy: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) configured[dev] = true;
@@ -661,7 +718,7 @@ silcu_status launch(Params &p, int problems, cudaStream_t s) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm<Ty, EPI, PAIR>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm<Ty, EPI, PAIR, RAW>, p);
   if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "cross_entropy: launch: %s", cudaGetErrorString(e));
   return check_launch("cross_entropy");
 }
