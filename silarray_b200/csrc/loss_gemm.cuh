@@ -33,7 +33,6 @@
 #pragma once
 
 #include <cuda.h>
-#include <limits.h>
 
 #include "elem.cuh"
 #include "loss_epilogue.cuh"
@@ -69,9 +68,9 @@ __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, int *
 // Adds to an earlier launch's sum.  Nothing else adds to this element in this
 // launch, so the order is fixed; done in the L2, no thread waits for the old sum
 // (as loads and stores, which may alias, 32 in a row cost a tile 15 us and more).
-__device__ __forceinline__ void red_add4(float *p, const float4 &v) {
-  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z),
-               "f"(v.w)
+__device__ __forceinline__ void red_add4(float *p, const uint4 &v) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(__uint_as_float(v.x)),
+               "f"(__uint_as_float(v.y)), "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w))
                : "memory");
 }
 
@@ -119,7 +118,7 @@ struct Cfg {
   static constexpr int LD = Ty::PARTS == 2 ? 16 : 32;
   // The sum goes back to TMEM for an epilogue that has no registers beside it
   // (with the 128 sums in registers the tf32 score gradients spill 2.8 KB a thread).
-  static constexpr bool BACK = MULTI && EPI == kScoreGrad;
+  static constexpr bool BACK = MULTI && EPI != kStats;
   static constexpr int CHUNK = !MULTI ? 1 << 30 : (Ty::PARTS == 2 ? 128 : 1024) / BK;
   static constexpr int GROUP_M = EPI == kOut ? 8 : 16;
   static constexpr uint32_t MN_BOX = Ty::KROW * 128;       // KROW elements of M / N x KROW k
@@ -384,8 +383,8 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       const Tile tl = tile_of<C>(q, bn, w.item);
       const int r0 = tl.m0 + BM * int(rank) + 32 * qr, c0 = tl.n0 + half * h;
       const int row = r0 + lane;
-      // this warp's columns of the tile, 128 at most in use (may be <= 0)
-      const int cols = min(min(q.N, tl.n0 + bn), RAW ? c0 + half : INT_MAX) - c0;
+      // this warp's columns of the tile (may be <= 0)
+      const int cols = min(min(q.N, tl.n0 + bn), c0 + half) - c0;
       // RAW: the next `n` stages' remainders x - tf32(x) of a raw B, for the MMAs.
       // Every warp sees every raw use of a slot, so no barrier is ever more than
       // one phase ahead of it.
@@ -504,6 +503,28 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           if (cb < 3) tmem_ld_cols<32>(src0 + ((cg - 1) % NBUF) * BN + 32 * (cb + 1), ahead);
         }
       };
+      // 16-byte chunk i of this lane's row in the staging block: 32 rows of 128
+      // bytes, chunks swizzled by the row.
+      auto put = [&](int i, uint4 v) {
+        *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(st) + lane * 128 + 16 * (i ^ (lane & 7))) = v;
+      };
+      // The staged block to rows r0.. of `out` from column col0 on, 8 lanes a row:
+      // write(address, 16 bytes, columns that exist from there on), where any do.
+      const int rows_left = q.M - r0 - (lane >> 3);
+      auto send = [&](auto *out, int64_t ld, int col0, auto &&write) {
+        constexpr int W = 16 / int(sizeof(*out));
+        const int ch = lane & 7, left = c0 + cols - col0 - W * ch;
+        auto *dst = out + int64_t(r0 + (lane >> 3)) * ld + col0 + W * ch;
+        const char *src = reinterpret_cast<const char *>(st) + (lane >> 3) * 128;
+        const int even = 16 * (ch ^ (lane >> 3)), odd = 16 * (ch ^ ((lane >> 3) + 4));
+        __syncwarp();
+        if (left > 0) {
+#pragma unroll
+          for (int i = 0; i < 8; i++, dst += 4 * ld)
+            if (4 * i < rows_left) write(dst, *reinterpret_cast<const uint4 *>(src + 512 * i + (i & 1 ? odd : even)), left);
+        }
+        __syncwarp();
+      };
       constexpr int UNROLL = IN_REGS ? 4 : 1;
 
       if constexpr (EPI == kStats) {
@@ -523,23 +544,8 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         if (r0 < q.M) {
           const bool counts = y >= 0 && y < p.loss.V;
           const int at = y - p.loss.v0 - c0;
-          auto put = [&](int i, uint4 v) {  // 16-byte chunk i of this lane's 128-byte row
-            *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(st) + lane * 128 + 16 * (i ^ (lane & 7))) = v;
-          };
-          // The staged rows, 8 lanes each; plain stores need no wait before the next block.
-          auto send = [&](int part, int col0) {
-            constexpr int W = 16 / int(sizeof(T));
-            T *out = static_cast<T *>(p.ds[part]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const int rr = 4 * i + (lane >> 3), ch = lane & 7, col = col0 + W * ch;
-              const uint4 x =
-                  *reinterpret_cast<const uint4 *>(reinterpret_cast<char *>(st) + rr * 128 + 16 * (ch ^ (rr & 7)));
-              if (r0 + rr < q.M && col < c0 + cols) *reinterpret_cast<uint4 *>(out + int64_t(r0 + rr) * p.lds + col) = x;
-            }
-            __syncwarp();
-          };
+          // plain stores need no wait before the next block; rows of ds end on whole vectors
+          auto whole = [](T *dst, const uint4 &x, int) { *reinterpret_cast<uint4 *>(dst) = x; };
 #pragma unroll UNROLL
           for (int cb = 0; cb < 4; cb++) {
             if (32 * cb < cols) {
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
                   put(4 * (cb & 1) + i, make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
                                                    pack_bf16(v[8 * i + 4], v[8 * i + 5]),
                                                    pack_bf16(v[8 * i + 6], v[8 * i + 7])));
-                if ((cb & 1) || 32 * (cb + 1) >= cols) send(0, c0 + 32 * (cb & ~1));
+                if ((cb & 1) || 32 * (cb + 1) >= cols) send(static_cast<T *>(p.ds[0]), p.lds, c0 + 32 * (cb & ~1), whole);
               } else {  // the exact tf32 pair, 32 columns per row each
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
@@ -566,65 +572,58 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
                     }
                     put(i, make_uint4(e[0], e[1], e[2], e[3]));
                   }
-                  send(part, c0 + 32 * cb);
+                  send(static_cast<T *>(p.ds[part]), p.lds, c0 + 32 * cb, whole);
                 }
               }
             }
           }
         }
       } else if (r0 < q.M) {
-        const float alpha = q.mode == kDirect && q.alpha ? *q.alpha : 1.0f;
+        const bool direct16 = q.mode == kDirect && PARTS == 1;
+        const float alpha = direct16 && q.alpha ? *q.alpha : 1.0f;
+        float *out = static_cast<float *>(q.out) + tl.part * q.plane;
 #pragma unroll UNROLL
         for (int cb = 0; cb < 4; cb++) {
           if (32 * cb < cols) {
             float v[32];
             block(cb, v);
-            __syncwarp();
+            if (direct16) {  // 64 bf16 columns per staged row: two blocks a store
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-              *reinterpret_cast<float4 *>(st + lane * 32 + 4 * (i ^ (lane & 7))) =
-                  make_float4(alpha * v[4 * i], alpha * v[4 * i + 1], alpha * v[4 * i + 2], alpha * v[4 * i + 3]);
-            __syncwarp();
-            const int col0 = c0 + 32 * cb;
-            if (q.mode != kDirect || PARTS == 2) {  // fp32: 8 lanes per row, 16 bytes each
-              float *out = static_cast<float *>(q.out) + tl.part * q.plane;
+              for (int i = 0; i < 4; i++)
+                put(4 * (cb & 1) + i,
+                    make_uint4(pack_bf16(alpha * v[8 * i], alpha * v[8 * i + 1]),
+                               pack_bf16(alpha * v[8 * i + 2], alpha * v[8 * i + 3]),
+                               pack_bf16(alpha * v[8 * i + 4], alpha * v[8 * i + 5]),
+                               pack_bf16(alpha * v[8 * i + 6], alpha * v[8 * i + 7])));
+              if ((cb & 1) || 32 * (cb + 1) >= cols)
+                send(static_cast<unsigned short *>(q.out), q.ldo, c0 + 32 * (cb & ~1),
+                     [&](unsigned short *dst, const uint4 &x, int left) {
+                       if (q.vec && left >= 8) {
+                         *reinterpret_cast<uint4 *>(dst) = x;
+                       } else {
+                         const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
-                const int rr = 4 * i + (lane >> 3), ch = lane & 7, col = col0 + 4 * ch;
-                const float4 x = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * (ch ^ (rr & 7)));
-                if (r0 + rr < q.M && col < q.N) {
-                  float *dst = out + int64_t(r0 + rr) * q.ldo + col;
-                  if (q.mode == kPlaneAdd) {
-                    red_add4(dst, x);
-                  } else if (q.mode != kDirect || (q.vec && col + 4 <= q.N)) {  // a plane's rows hold whole vectors
-                    *reinterpret_cast<float4 *>(dst) = x;
-                  } else {
-                    const float e[4] = {x.x, x.y, x.z, x.w};
+                         for (int t = 0; t < 8; t++)
+                           if (t < left) dst[t] = static_cast<unsigned short>(e[t >> 1] >> (16 * (t & 1)));
+                       }
+                     });
+            } else {  // 32 fp32 columns
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
-                      if (col + t < q.N) dst[t] = e[t];
-                  }
+              for (int i = 0; i < 8; i++)
+                put(i, make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                  __float_as_uint(v[4 * i + 3])));
+              send(out, q.ldo, c0 + 32 * cb, [&](float *dst, const uint4 &x, int left) {
+                if (q.mode == kPlaneAdd) {
+                  red_add4(dst, x);
+                } else if (q.mode == kPlane || (q.vec && left >= 4)) {  // a plane's rows hold whole vectors
+                  *reinterpret_cast<uint4 *>(dst) = x;
+                } else {
+                  const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                  for (int t = 0; t < 4; t++)
+                    if (t < left) dst[t] = __uint_as_float(e[t]);
                 }
-              }
-            } else {  // bf16: 4 lanes per row, 8 columns each
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const int rr = 8 * i + (lane >> 2), ch = 2 * (lane & 3), col = col0 + 4 * ch;
-                const float4 x = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * (ch ^ (rr & 7)));
-                const float4 u = *reinterpret_cast<const float4 *>(st + rr * 32 + 4 * ((ch + 1) ^ (rr & 7)));
-                if (r0 + rr < q.M && col < q.N) {
-                  __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(q.out) + int64_t(r0 + rr) * q.ldo + col;
-                  if (q.vec && col + 8 <= q.N) {
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w),
-                                                                 pack_bf16(u.x, u.y), pack_bf16(u.z, u.w));
-                  } else {
-                    const float e[8] = {x.x, x.y, x.z, x.w, u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int t = 0; t < 8; t++)
-                      if (col + t < q.N) dst[t] = __float2bfloat16_rn(e[t]);
-                  }
-                }
-              }
+              });
             }
           }
         }
