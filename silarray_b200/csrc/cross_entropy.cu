@@ -516,10 +516,9 @@ silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
 
 // Where a product of ds goes: the result itself, or planes that earlier
 // pieces may have begun.
-void set_output(lossmm::Problem &q, const Gradient &g, bool add, void *out, int64_t ldo, int vec, const float *alpha,
-                int64_t D, int64_t nk) {
+void set_output(lossmm::Problem &q, const Gradient &g, bool add, void *out, int64_t ldo, int vec, int64_t D,
+                int64_t nk) {
   q.ksplit = int(g.split < nk ? g.split : nk);  // a short last piece adds to the first planes only
-  q.alpha = alpha;
   if (g.direct) {
     q.mode = lossmm::kDirect;
     q.out = out;
@@ -583,6 +582,7 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     const bool pairs = !b.score.raw;
     p.bn = pairs ? lossmm::BN : lossmm::BM;
     p.rows_a = lossmm::BM;
+    p.alpha = alpha;
     if (!pairs) set_raw(p);
     int count = 0;
     w.mn = true;
@@ -593,11 +593,11 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
       if (is_dw) {
         if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
           return map_error();
-        set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, alpha, a.D,
+        set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, a.D,
                    ceil_div(a.rows, BK));
       } else {
         if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
-        set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, alpha, a.D, ceil_div(n, BK));
+        set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
       }
     }
     if ((st = products<Ty>(p, pairs, count, s)) != SILCU_OK) return st;

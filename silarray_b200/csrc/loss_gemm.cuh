@@ -136,7 +136,6 @@ struct Problem {
   int mode, vec;           // vec: kDirect rows are 16-byte aligned
   void *out;
   int64_t ldo, plane;      // row stride; elements from one plane to the next
-  const float *alpha;      // kDirect: factor of the result, or null
 };
 
 struct __align__(64) Params {
@@ -149,6 +148,7 @@ struct __align__(64) Params {
   int stages;        // ring stages (RAW)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, tail, extra;
+  const float *alpha;  // kOut: factor of kDirect results in bf16, or null
   LossArgs loss;
   int part0;  // index of this launch's first part
   int *err;
@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
     const int qr = warp & 3, h = (warp - 2) >> 2;
     float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
     const int half = RAW ? p.half : 128;
+    const float alpha = EPI == kOut && p.alpha ? *p.alpha : 1.0f;
     uint32_t cg = 0, kbe = 0;
     bool ok = true;
     for (int k = 0; ok && work_at(p, unit, k, w); k++) {
@@ -426,6 +427,21 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           else mbar_arrive(bar);
         }
       };
+      // What the epilogue needs of the row: asked for while the MMAs run, where
+      // three registers are left beside the sums.
+      constexpr bool EARLY = !C::BACK;
+      int y = -1;
+      float lse = 0.f, g = 0.f;
+      auto row_data = [&] {
+        if (EPI != kOut && row < q.M) {
+          y = p.loss.targets[row];
+          if (EPI == kScoreGrad) {
+            lse = p.loss.lse[row] * kLog2e;
+            g = p.loss.scale ? p.loss.scale[row] : 1.0f;
+          }
+        }
+      };
+      if (EARLY) row_data();
       const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + half * h;
       float acc[C::MULTI ? 128 : 1];
       if constexpr (C::MULTI) {
@@ -477,16 +493,8 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         ok = finished(cg);
       }
       cg++;
-      if (!__all_sync(0xffffffffu, ok && *reinterpret_cast<volatile int *>(p.err) == 0)) break;
-      int y = -1;
-      float lse = 0.f, g = 0.f;
-      if (EPI != kOut && row < q.M) {
-        y = p.loss.targets[row];
-        if (EPI == kScoreGrad) {
-          lse = p.loss.lse[row] * kLog2e;
-          g = p.loss.scale ? p.loss.scale[row] : 1.0f;
-        }
-      }
+      if (!ok) break;  // a wait gave up; ok is the same in all lanes
+      if (!EARLY) row_data();
       constexpr bool IN_REGS = C::MULTI && !C::BACK;
       // Columns 32 cb .. 32 cb + 31 of this thread's row, for cb = 0, 1, 2, 3 in
       // turn; from TMEM the next ones are on their way while these are used.
@@ -580,7 +588,6 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         }
       } else if (r0 < q.M) {
         const bool direct16 = q.mode == kDirect && PARTS == 1;
-        const float alpha = direct16 && q.alpha ? *q.alpha : 1.0f;
         float *out = static_cast<float *>(q.out) + tl.part * q.plane;
 #pragma unroll UNROLL
         for (int cb = 0; cb < 4; cb++) {
