@@ -29,7 +29,29 @@ inline bool aligned16(const void *p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
 
+// Launches a kernel that may start before the one ahead of it in the stream
+// has ended (programmatic dependent launch): its start-up overlaps the other's
+// tail.  It calls wait_for_previous() before it reads or writes anything that
+// others touch; the one ahead calls let_next_start() early on.
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 // ---------------------------------------------------------------- device side
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // IEEE round-to-nearest arithmetic without contraction: the reference CPU
 // path rounds after every operation, so fused kernels use these to keep the
 // same rounding sequence (nvcc would otherwise fuse a*b+c into one FMA).

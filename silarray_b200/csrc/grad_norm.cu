@@ -185,6 +185,7 @@ __device__ __forceinline__ void for_span(const ListArgs<CAP> &a, uint64_t worker
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) sum_squares(const __grid_constant__ ListArgs<CAP> a) {
   __shared__ double sm[kWarps];
+  let_next_start();
   double acc = 0.0;
   for_span(a, uint64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5), [&](int t, uint64_t first, uint64_t n) {
     if (a.dtype[t] == SILCU_BF16) {
@@ -222,6 +223,7 @@ __device__ __forceinline__ double total_norm(const double *part, int nparts) {
 }
 
 __global__ void __launch_bounds__(kThreads) norm_finish(const double *part, int nparts, float *norm) {
+  wait_for_previous();
   const double n = total_norm(part, nparts);
   if (threadIdx.x == 0) *norm = float(n);
 }
@@ -372,7 +374,7 @@ silcu_status silcu_grad_norm(const silcu_tensor *tensors, size_t count, float *n
   cudaStream_t s = as_stream(stream);
   double *part = static_cast<double *>(workspace);
   const uint32_t parts = sum_list(tensors, count, part, s);
-  norm_finish<<<1, kThreads, 0, s>>>(part, int(parts), norm);
+  launch_after(norm_finish, 1, kThreads, 0, s, part, int(parts), norm);
   return check_launch("grad_norm", pieces(tensors, count) + 1);
 }
 

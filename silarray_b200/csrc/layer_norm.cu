@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
     for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NT * GROUPS) acc_s[c] = 0.f;
     __syncthreads();
   }
+  let_next_start();
   const float inv_n = 1.0f / float(a.cols);
   const uint64_t step = uint64_t(gridDim.x) * GROUPS;
   int buf = 0;
@@ -501,6 +502,7 @@ __global__ void __launch_bounds__(1024) ln_finish(const float *__restrict__ part
   const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const uint32_t c = blockIdx.x * 32 + lane;
   float s = 0.f;
+  wait_for_previous();
   if (c < 2 * cols) {
 #pragma unroll 8
     for (uint32_t i = slice; i < nparts; i += 32) s += __ldcs(part + uint64_t(i) * 2 * cols + c);
@@ -763,8 +765,8 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
       st = dresidual ? backward<float, true>(a, s, &grid) : backward<float, false>(a, s, &grid);
     if (st != SILCU_OK) return st;
   }
-  ln_finish<<<uint32_t((2 * cols + 31) / 32), 1024, 0, s>>>(static_cast<const float *>(workspace), grid,
-                                                           uint32_t(cols), dgamma, dbeta);
+  launch_after(ln_finish, uint32_t((2 * cols + 31) / 32), 1024, 0, s, static_cast<const float *>(workspace), grid,
+               uint32_t(cols), dgamma, dbeta);
   return check_launch("layer_norm_backward finish");
 }
 
