@@ -45,6 +45,8 @@ __global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ p
   __shared__ float2 sm[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int64_t row = int64_t(blockIdx.x) * 32 + lane;
+  let_next_start();
+  wait_for_previous();
   float m = -INFINITY, l = 0.f;
   auto join = [&](float2 x) {
     const float mx = fmaxf(m, x.x);
@@ -94,6 +96,8 @@ __global__ void __launch_bounds__(1024) loss_reduce(const float *__restrict__ ro
                                                     const int32_t *__restrict__ targets, int64_t rows, int V, int mean,
                                                     float *__restrict__ loss) {
   __shared__ double sm[32];
+  let_next_start();
+  wait_for_previous();
   double s = 0.0;
   for (int64_t i = threadIdx.x; i < rows; i += 1024) s += double(row_loss[i]);
   s = cta_sum(s, sm);
@@ -109,6 +113,8 @@ __global__ void __launch_bounds__(1024) row_scales(const float *__restrict__ dlo
                                                    const int32_t *__restrict__ targets, int64_t rows, int V,
                                                    int reduction, float *__restrict__ scale) {
   __shared__ double sm[32];
+  let_next_start();
+  wait_for_previous();
   float g = 1.0f;
   if (reduction == SILCU_REDUCE_MEAN) {
     const double n = count_rows(targets, rows, V, sm);
@@ -131,6 +137,8 @@ __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int6
   const int per_row = dp / W;
   const bool vec = ld % W == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   const int64_t n = rows * per_row;
+  let_next_start();
+  wait_for_previous();
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
     const int64_t r = i / per_row;
     const int c = int(i - r * per_row) * W;
@@ -175,6 +183,8 @@ __global__ void __launch_bounds__(256) planes_finish(const float *__restrict__ p
   constexpr int W = 16 / sizeof(T);
   const int per_row = (D + W - 1) / W;
   const int64_t n = rows * per_row;
+  let_next_start();
+  wait_for_previous();
   const float k0 = alpha ? *alpha : 1.0f;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
     const int64_t r = i / per_row;
@@ -305,8 +315,8 @@ struct Copy {
   silcu_status fill(const void *src, int64_t ld, int64_t rows, int64_t D, const int32_t *targets, int64_t V,
                     cudaStream_t s) const {
     using T = typename Ty::T;
-    copy_rows<T><<<stream_grid(rows * dp * int64_t(sizeof(T)) / 16), 256, 0, s>>>(
-        static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo);
+    launch_after(copy_rows<T>, stream_grid(rows * dp * int64_t(sizeof(T)) / 16), 256, 0, s,
+                 static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo);
     return check_launch("cross_entropy copy");
   }
   Operand operand(bool mn) const { return Operand{p, lo, dp, mn}; }
@@ -507,10 +517,11 @@ silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
     if ((st = scores<Ty, lossmm::kStats>(p, f.tiles, s)) != SILCU_OK) return st;
     part0 += f.parts(a, v0);
   }
-  loss_finish<<<uint32_t((a.rows + 31) / 32), 1024, 0, s>>>(f.part, f.nparts, a.rows, a.targets, int(a.V),
-                                                            f.target_score, a.lse, f.row_loss);
+  launch_after(loss_finish, uint32_t((a.rows + 31) / 32), 1024, 0, s, f.part, f.nparts, a.rows, a.targets, int(a.V),
+               f.target_score, a.lse, f.row_loss);
   if ((st = check_launch("cross_entropy finish")) != SILCU_OK || a.reduction == SILCU_REDUCE_NONE) return st;
-  loss_reduce<<<1, 1024, 0, s>>>(f.row_loss, a.targets, a.rows, int(a.V), a.reduction == SILCU_REDUCE_MEAN, a.loss);
+  launch_after(loss_reduce, 1, 1024, 0, s, f.row_loss, a.targets, a.rows, int(a.V),
+               int(a.reduction == SILCU_REDUCE_MEAN), a.loss);
   return check_launch("cross_entropy reduce");
 }
 
@@ -537,8 +548,8 @@ silcu_status finish_planes(const Gradient &g, int64_t rows, int64_t D, const flo
                            int vec, cudaStream_t s) {
   using T = typename Ty::T;
   const int64_t ldp = up(D, 8);
-  planes_finish<T><<<stream_grid(rows * ceil_div(D * int64_t(sizeof(T)), 16)), 256, 0, s>>>(
-      g.planes, g.split, g.M * ldp, rows, int(D), int(ldp), alpha, static_cast<T *>(out), ldo, vec);
+  launch_after(planes_finish<T>, stream_grid(rows * ceil_div(D * int64_t(sizeof(T)), 16)), 256, 0, s, g.planes, g.split,
+               g.M * ldp, rows, int(D), int(ldp), alpha, static_cast<T *>(out), ldo, vec);
   return check_launch("cross_entropy planes");
 }
 
@@ -547,7 +558,7 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
   using T = typename Ty::T;
   constexpr int BK = lossmm::Cfg<Ty, lossmm::kOut, true>::BK;
   silcu_status st;
-  row_scales<<<1, 1024, 0, s>>>(a.dloss, a.targets, a.rows, int(a.V), a.reduction, b.scale);
+  launch_after(row_scales, 1, 1024, 0, s, a.dloss, a.targets, a.rows, int(a.V), a.reduction, b.scale);
   if ((st = check_launch("cross_entropy scales")) != SILCU_OK) return st;
   if ((st = b.h.fill(a.H, a.ldh, a.rows, a.D, a.targets, a.V, s)) != SILCU_OK) return st;
   // A factor that all rows share leaves ds alone where ds is rounded.

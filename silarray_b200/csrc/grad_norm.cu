@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(kThreads) norm_finish(const double *part, int 
 
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) clip_scale(const __grid_constant__ ListArgs<CAP> a) {
+  wait_for_previous();
   const double norm = total_norm(a.all, a.nparts);
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm) *a.norm = float(norm);
   const double below = norm + double(a.eps);
@@ -334,7 +335,7 @@ void launch_sum(const silcu_tensor *t, const Piece &p, double *part, cudaStream_
 template <int CAP>
 void launch_scale(const silcu_tensor *t, void *const *outs, const Piece &p, ListArgs<CAP> a, cudaStream_t s) {
   fill(a, t, outs, p);
-  clip_scale<CAP><<<p.grid, kThreads, 0, s>>>(a);
+  launch_after(clip_scale<CAP>, p.grid, kThreads, 0, s, a);
 }
 
 // The partials of the whole list; their number.

@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
   const int unit = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
   const int bn = PAIR ? BN : p.bn;
 
+  let_next_start();
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; s++) {
       mbar_init(full0 + 8 * s, 1);
@@ -254,6 +255,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
   if (PAIR) cluster_sync_all();  // the peer's barriers are initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_previous();
   Work w;
 
   if (warp == 0) {
@@ -717,13 +719,15 @@ silcu_status launch(Params &p, int problems, cudaStream_t s) {
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = PAIR ? 2 : 1;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_after
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm<Ty, EPI, PAIR, RAW>, p);
   if (e != cudaSuccess) return fail(SILCU_CUDA_ERROR, "cross_entropy: launch: %s", cudaGetErrorString(e));
   return check_launch("cross_entropy");
