@@ -640,17 +640,18 @@ class TensorList:
         """Checks the tensors and fills the C arrays, unless nothing moved."""
         addresses = [t.data_ptr() for t in self.tensors]
         counts = [t.numel() for t in self.tensors]
-        if addresses == self._addresses and counts == self._counts:
+        if addresses == self._addresses and counts == self._counts \
+                and all(t.dtype is d and t.is_contiguous() for t, (d, _) in zip(self.tensors, self.shapes)):
             return self
         n = len(self.tensors)
-        self.array = (_lib.Tensor * n)()
-        self.pointers = (ct.c_void_p * n)(*addresses)
-        for i, t in enumerate(self.tensors):
+        array = (_lib.Tensor * n)()
+        index = self.tensors[0].get_device()
+        for i, t in enumerate(self.tensors):  # nothing changes if one is refused
             k = _kind(t)
-            if i == 0:
-                self.device, self.index = t.device, t.get_device()
-            _at(f"TensorList tensor {i}", t, t.dtype, counts[i], self.index)
-            self.array[i] = _lib.Tensor(addresses[i], counts[i], k)
+            _at(f"TensorList tensor {i}", t, t.dtype, counts[i], index)
+            array[i] = _lib.Tensor(addresses[i], counts[i], k)
+        self.array, self.pointers = array, (ct.c_void_p * n)(*addresses)
+        self.device, self.index = self.tensors[0].device, index
         self.shapes = [(t.dtype, c) for t, c in zip(self.tensors, counts)]
         self.spans = sorted((a, a + c * t.element_size())
                             for a, c, t in zip(addresses, counts, self.tensors) if c)

@@ -288,6 +288,22 @@ def test_tensor_list_follows_its_tensors(cuda):
     assert abs(float(gpu.grad_norm(tl)) - (100 + 2700) ** 0.5) < 1e-4
 
 
+def test_tensor_list_sees_other_views(cuda):
+    """The same storage read as another type, or with gaps, is checked again."""
+    a = torch.full((100,), 2.0, device="cuda")
+    tl = gpu.TensorList([a])
+    assert float(gpu.grad_norm(tl)) == 20.0
+    whole = a.data
+    a.data = whole.view(torch.int32)
+    with pytest.raises(TypeError):
+        gpu.grad_norm(tl)
+    a.data = torch.empty_strided((100,), (2,), device="cuda")
+    with pytest.raises((TypeError, ValueError)):
+        gpu.grad_norm(tl)
+    a.data = whole
+    assert float(gpu.grad_norm(tl)) == 20.0
+
+
 def test_streams_and_graphs(cuda):
     """Calls on a side stream, and two captured graphs replayed at the same
     time on two streams, give what eager calls give."""
