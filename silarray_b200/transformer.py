@@ -376,4 +376,5 @@ class LossHead:
 
     def clip(self, max_norm):
         """Clips self.grads by their common norm; returns it (0-d)."""
+        self._grad_list.tensors = list(self.grads.values())  # whatever tensors are there now
         return gpu.clip_grad_norm(self._grad_list, max_norm)

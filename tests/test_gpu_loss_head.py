@@ -112,3 +112,18 @@ def test_three_steps_move_the_weights_like_autograd(cuda):
     # three gradients of 1e-5 and three roundings of W
     assert float((head.w.double() - w64).norm()) <= 1e-5 * 3 * moved + 3 * 2.0 ** -24 * float(w64.norm())
     assert np.isfinite(moved) and moved > 0
+
+
+def test_clip_takes_the_gradients_that_are_there(cuda):
+    """A gradient replaced by another tensor is the one that is written and clipped."""
+    head = transformer.LossHead(transformer.init_head(VOCAB, CFG.d_model, seed=4))
+    x, y = block_output(2), make_targets(3)
+    head.forward(x, y)
+    head.backward()
+    norm = head.clip(1e9)
+    first, head.grads["w"] = head.grads["w"], torch.empty_like(head.w)
+    head.backward()
+    kept = first.clone()
+    assert torch.equal(head.grads["w"], first)
+    assert torch.equal(head.clip(1e-3), norm)
+    assert torch.equal(first, kept) and float(head.grads["w"].norm()) <= 1e-3
