@@ -366,7 +366,7 @@ typedef enum silcu_dtype { SILCU_F32 = 0, SILCU_BF16 = 1 } silcu_dtype;
  * each row's statistics for the backward pass (fp32, NULL = not wanted):
  * mean, and rstd = 1 / sqrt(var + eps).  gamma and beta are fp32 for either
  * dtype; all arithmetic is fp32, and the output is rounded once.  out may be
- * `in` itself. */
+ * `in` itself; apart from that no output overlaps an operand. */
 silcu_status silcu_layer_norm_forward(const void *in, void *out, float *mean, float *rstd, const float *gamma,
                                       const float *beta, size_t rows, size_t cols, float eps, int dtype,
                                       silcu_stream stream);
@@ -374,7 +374,8 @@ silcu_status silcu_layer_norm_forward(const void *in, void *out, float *mean, fl
  *   din = rstd * (a - avg(a) - xh * avg(a * xh)) (+ dresidual),
  * and over all rows dgamma = sum(dout * xh), dbeta = sum(dout) (fp32).
  * dresidual (NULL = none) is the gradient that reaches `in` past the norm, as in
- * a pre-norm block.  din may be dout, in or dresidual itself.  dgamma and dbeta
+ * a pre-norm block.  din may be dout, in or dresidual itself; apart from that no
+ * output overlaps an operand.  dgamma and dbeta
  * are written, not added to; rows = 0 writes zeros.  The sums' order depends on
  * the shape and the GPU only, so results repeat bit for bit.  The workspace
  * holds per-CTA partial sums. */
@@ -398,7 +399,7 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
  * dloss, or dloss / count); NULL = 1.  dH / dW may be NULL when not wanted;
  * they are written, not added to.  f32 products are 3xTF32; with bf16, ds is
  * rounded to bf16 once (the products' operand type) and sums are fp32.
- * The gradients may not overlap the operands. */
+ * The results may not overlap the operands or one another, nor the workspace. */
 typedef enum silcu_reduction { SILCU_REDUCE_MEAN = 0, SILCU_REDUCE_SUM = 1, SILCU_REDUCE_NONE = 2 } silcu_reduction;
 typedef struct silcu_cross_entropy_args {
   const void *H, *W;

@@ -13,6 +13,34 @@ namespace silcu {
 inline size_t dtype_bytes(int dtype) { return dtype == SILCU_BF16 ? 2 : 4; }
 inline bool dtype_known(int dtype) { return dtype == SILCU_F32 || dtype == SILCU_BF16; }
 
+// Rows in memory: `width` bytes each, `stride` bytes apart.
+struct Span {
+  const void *p;
+  int64_t rows, width, stride;
+};
+// Whether two of them share a byte.  Rows of one stride that lie side by side
+// (column ranges of one matrix) do not; other interleaved rows count as sharing.
+inline bool overlap(const Span &a, const Span &b) {
+  if (!a.p || !b.p || a.rows * a.width == 0 || b.rows * b.width == 0) return false;
+  const int64_t a0 = int64_t(reinterpret_cast<uintptr_t>(a.p)), b0 = int64_t(reinterpret_cast<uintptr_t>(b.p));
+  if (a0 + (a.rows - 1) * a.stride + a.width <= b0 || b0 + (b.rows - 1) * b.stride + b.width <= a0) return false;
+  const int64_t stride = a.rows > 1 ? a.stride : b.stride;
+  if (stride <= 0 || (a.rows > 1 && b.rows > 1 && a.stride != b.stride)) return true;
+  const int64_t d = ((b0 - a0) % stride + stride) % stride;  // b's column in a's rows
+  return d < a.width || d + b.width > stride;
+}
+inline Span flat(const void *p, int64_t bytes) { return Span{p, 1, bytes, bytes}; }
+// Whether an output shares memory with an input or another output.
+inline bool outputs_overlap(const Span *outs, int nouts, const Span *ins, int nins) {
+  for (int i = 0; i < nouts; i++) {
+    for (int j = 0; j < nins; j++)
+      if (overlap(outs[i], ins[j])) return true;
+    for (int j = 0; j < i; j++)
+      if (overlap(outs[i], outs[j])) return true;
+  }
+  return false;
+}
+
 // VEC elements as they lie in memory: one 16-byte vector, or one element.
 template <typename T, int VEC> struct Raw;
 template <> struct Raw<float, 4> { float4 r; };

@@ -701,6 +701,11 @@ silcu_status silcu_layer_norm_forward(const void *in, void *out, float *mean, fl
   if (!in || !out || !gamma || !beta) return fail(SILCU_INVALID_ARGUMENT, "layer_norm_forward: null pointer");
   st = check_aligned("layer_norm_forward", dtype, {in, out}, {mean, rstd, gamma, beta});
   if (st != SILCU_OK) return st;
+  const int64_t bytes = int64_t(rows * cols * dtype_bytes(dtype)), row4 = int64_t(4 * rows), col4 = int64_t(4 * cols);
+  const Span outs[] = {flat(out, bytes), flat(mean, row4), flat(rstd, row4)};
+  const Span ins[] = {flat(gamma, col4), flat(beta, col4), flat(out == in ? nullptr : in, bytes)};
+  if (outputs_overlap(outs, 3, ins, 3))
+    return fail(SILCU_INVALID_ARGUMENT, "layer_norm_forward: overlapping operands");
   LnArgs a = {};
   a.in = in;
   a.out = out;
@@ -748,6 +753,12 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
     const size_t need = silcu_layer_norm_backward_workspace_bytes(rows, cols, dtype);
     if (!workspace || workspace_bytes < need)
       return fail(SILCU_WORKSPACE_TOO_SMALL, "layer_norm_backward: workspace %zu < %zu", workspace_bytes, need);
+    const int64_t bytes = int64_t(rows * cols * dtype_bytes(dtype)), row4 = int64_t(4 * rows), col4 = int64_t(4 * cols);
+    auto other = [&](const void *p) { return flat(p == din ? nullptr : p, bytes); };  // din may be one of these
+    const Span outs[] = {flat(din, bytes), flat(dgamma, col4), flat(dbeta, col4)};
+    const Span ins[] = {other(dout), other(in), other(dresidual), flat(gamma, col4), flat(mean, row4), flat(rstd, row4)};
+    if (outputs_overlap(outs, 3, ins, 6))
+      return fail(SILCU_INVALID_ARGUMENT, "layer_norm_backward: overlapping operands");
     LnArgs a = {};
     a.in = in;
     a.dout = dout;

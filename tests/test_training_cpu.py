@@ -188,3 +188,30 @@ def test_python_refuses_cpu_tensors():
         gpu.grad_norm([x])
     with pytest.raises(ValueError):
         gpu.TensorList([])
+
+
+def test_overlapping_operands_are_refused(lib):
+    """Results that share memory with an operand or with one another; an
+    operand written in place and column ranges of one matrix are another matter."""
+    at = lambda *offsets: [C.c_void_p((1 << 20) + o) for o in offsets]  # noqa: E731
+    f, b = lib.silcu_layer_norm_forward, lib.silcu_layer_norm_backward
+    n, far = 100 * 768 * 4, 1 << 22
+    x, near, out, mean, rstd, g, be = at(0, 768 * 4, far, 2 * far, 3 * far, 4 * far, 5 * far)
+    for args in [(x, near, mean, rstd, g, be), (x, out, mean, mean, g, be), (x, out, x, rstd, g, be), (x, out, mean, rstd, out, be)]:
+        assert f(*args, 100, 768, 1e-5, 0, None) == 1 and b"overlap" in lib.silcu_last_error()
+    ws = C.c_void_p(1 << 30)
+    dy, dg, db = at(6 * far, 7 * far, 8 * far)
+    for args in [(dy, x, mean, rstd, g, None, near, dg, db), (dy, x, mean, rstd, g, near, x, dg, db),
+                 (dy, x, mean, rstd, g, None, out, dg, dg), (dy, x, mean, rstd, g, None, out, mean, db),
+                 (dy, x, mean, rstd, g, None, out, out, db)]:
+        assert b(*args, 100, 768, 0, ws, n * 8, None) == 1 and b"overlap" in lib.silcu_last_error()
+
+    fwd, bwd = lib.silcu_linear_cross_entropy, lib.silcu_linear_cross_entropy_backward
+    base = _loss_args()
+    for kw in (dict(loss=base.H + 8), dict(loss=base.lse + 4), dict(lse=base.W), dict(lse=base.targets + 36)):
+        a = _loss_args(**kw)
+        assert fwd(C.byref(a), ws, far, None) == 1 and b"overlap" in lib.silcu_last_error(), kw
+    for kw in (dict(dH=base.H + 256), dict(dH=base.W - 4), dict(dW=base.W + 256), dict(dW=base.dH + 2304), dict(dH=base.lse),
+               dict(dloss=base.dW + 25596), dict(dH=base.H + 252, ldh=128, lddh=128), dict(dH=base.H + 256, ldh=128, lddh=130)):
+        a = _loss_args(**kw)
+        assert bwd(C.byref(a), ws, far, None) == 1 and b"overlap" in lib.silcu_last_error(), kw
