@@ -28,8 +28,8 @@
 // scores that become lse); the epilogue adds each chunk in fp32 registers, to
 // nearest, while the next one runs.  What is rounded to bf16 next takes one chunk.
 //
-// Every wait is bounded; on expiry the kernel records a code, unwinds, frees
-// its TMEM and exits.  No load is multicast.
+// Every wait is bounded; on expiry the kernel records a code, unwinds, lets what
+// is in flight land, frees its TMEM and exits.  No load is multicast.
 #pragma once
 
 #include <cuda.h>
@@ -63,6 +63,14 @@ __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, int *
     }
   }
   return true;
+}
+
+// After a wait that gave up: the loads and MMAs that this thread issued, or that
+// it no longer waits for, end within microseconds; a millisecond covers them.
+__device__ __forceinline__ void settle() {
+  const unsigned long long t0 = globaltimer();
+#pragma unroll 1
+  for (int i = 0; i < (1 << 16) && globaltimer() - t0 < 1000000ull; i++) asm volatile("nanosleep.u32 1000;");
 }
 
 // Adds to an earlier launch's sum.  Nothing else adds to this element in this
@@ -116,8 +124,8 @@ struct Cfg {
   // Columns that join the sums at a time: 32 leave the tf32 sums no registers, and
   // what spills there every chunk pays for (score gradients 660 -> 477 us with 16).
   static constexpr int LD = Ty::PARTS == 2 ? 16 : 32;
-  // The sum goes back to TMEM for an epilogue that has no registers beside it
-  // (with the 128 sums in registers the tf32 score gradients spill 2.8 KB a thread).
+  // The tf32 sums go back to TMEM for the epilogues that have no registers beside
+  // them (with the 128 sums in registers the score gradients spill 2.8 KB a thread).
   static constexpr bool BACK = MULTI && EPI != kStats;
   static constexpr int CHUNK = !MULTI ? 1 << 30 : (Ty::PARTS == 2 ? 128 : 1024) / BK;
   static constexpr int GROUP_M = EPI == kOut ? 8 : 16;
@@ -199,7 +207,8 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
   return Ty::PARTS == 1 ? make_desc_mn16(addr, C::MN_BOX) : make_desc_mn32(addr, C::MN_BOX);
 }
 
-// BMN: B is stored with the N index contiguous (kOut; A's order is Problem::amn).
+// The scores' operands both have k contiguous; of kOut's, B has the N index contiguous
+// (BMN) and A what Problem::amn says.
 //
 // RAW: B may be plain fp32.  Its tile is the hi operand as it stands (the
 // tensor core reads the upper 19 bits of a value), and the epilogue warps, idle
@@ -309,6 +318,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           }
         }
       }
+      if (!ok) settle();
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {  // the pair's MMAs are issued by the even CTA
@@ -373,6 +383,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           else mma_commit(tfull0 + 8 * j);
         }
       }
+      if (!ok) settle();
     }
   } else {
     const int qr = warp & 3, h = (warp - 2) >> 2;
@@ -436,7 +447,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       float lse = 0.f, g = 0.f;
       auto row_data = [&] {
         if (EPI != kOut && row < q.M) {
-          y = p.loss.targets[row];
+          y = max(p.loss.targets[row], -1);  // any negative one; differences with it do not overflow
           if (EPI == kScoreGrad) {
             lse = p.loss.lse[row] * kLog2e;
             g = p.loss.scale ? p.loss.scale[row] : 1.0f;
@@ -642,6 +653,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         release(cg - 1);
       }
     }
+    if (!ok) settle();
   }
   tc_fence_before();
   __syncthreads();

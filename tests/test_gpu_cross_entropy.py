@@ -191,6 +191,20 @@ def test_rows_left_out(cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [40, 300])
+def test_every_left_out_target_alike(cuda, rows, dtype):
+    """The vocabulary's size, the smallest and the largest int32 leave a row out just as -1 does."""
+    H, W, y = make(rows, 600, 72, dtype, 6, left_out=0.5)
+    out = ~((y >= 0) & (y < 600))
+    y[out] = -1
+    want = run(H, W, y)
+    for t in (600, -2 ** 31, 2 ** 31 - 1, -100):
+        y[out] = t
+        for p, q in zip(run(H, W, y), want):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 def test_bad_values_in_rows_that_count(cuda, dtype):
     H, W, y = make(130, 600, 72, dtype, 6, left_out=0.0)
     H[4, 5] = float("nan")
