@@ -37,40 +37,6 @@ namespace {
 using Args = silcu_cross_entropy_args;
 
 // ------------------------------------------------------------ small kernels
-// Joins a row's parts: lse = M + log sum l_i exp(m_i - M).  A CTA takes 32
-// rows, 32 warps the parts in 32 interleaved slices.
-__global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ part, int nparts, int64_t rows,
-                                                    const int32_t *__restrict__ targets, int V,
-                                                    const float *__restrict__ target_score, float *__restrict__ lse,
-                                                    float *__restrict__ loss) {
-  __shared__ float2 sm[32][33];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int64_t row = int64_t(blockIdx.x) * 32 + lane;
-  let_next_start();
-  wait_for_previous();
-  float m = -INFINITY, l = 0.f;
-  auto join = [&](float2 x) {
-    const float mx = fmaxf(m, x.x);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    l = l * ex2((m - ref) * kLog2e) + x.y * ex2((x.x - ref) * kLog2e);
-    m = mx;
-  };
-  if (row < rows) {
-#pragma unroll 4
-    for (int i = slice; i < nparts; i += 32) join(__ldcs(part + int64_t(i) * rows + row));
-  }
-  sm[slice][lane] = make_float2(m, l);
-  __syncthreads();
-  if (slice == 0 && row < rows) {
-#pragma unroll
-    for (int i = 1; i < 32; i++) join(sm[i][lane]);
-    const float v = m + logf(l);
-    lse[row] = v;
-    const int y = targets[row];
-    loss[row] = y >= 0 && y < V ? v - target_score[row] : 0.f;
-  }
-}
-
 __device__ __forceinline__ double cta_sum(double v, double *sm) {
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
@@ -81,9 +47,10 @@ __device__ __forceinline__ double cta_sum(double v, double *sm) {
   return s;
 }
 
-// Number of rows that count, in every thread of the (one) CTA.
+// Number of rows that count, in every thread of the CTA.
 __device__ __forceinline__ double count_rows(const int32_t *targets, int64_t rows, int V, double *sm) {
   int n = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) {
     const int y = targets[i];
     n += y >= 0 && y < V;
@@ -91,56 +58,122 @@ __device__ __forceinline__ double count_rows(const int32_t *targets, int64_t row
   return cta_sum(double(n), sm);
 }
 
-// The scalar loss: the sum of the rows' losses, or their mean over the rows
-// that count (0 when none does).
-__global__ void __launch_bounds__(1024) loss_reduce(const float *__restrict__ row_loss,
-                                                    const int32_t *__restrict__ targets, int64_t rows, int V, int mean,
-                                                    float *__restrict__ loss) {
-  __shared__ double sm[32];
+// Joins a row's parts, lse = M + log sum l_i exp(m_i - M), and with `total`
+// the rows' losses to their sum, or their mean over the rows that count (0 when
+// none does).  A CTA takes 8 rows and has 128 threads for the parts of each;
+// 8 rows of 294 parts took 4.6 us with 32 threads a row and a chain of 31 joins at its
+// end.  The CTA that finishes last adds the losses, in row order whichever it
+// is: `done` counts the CTAs, and the scores' launch has set it to 0.
+constexpr int kFinishRows = 8;
+__global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ part, int nparts, int64_t rows,
+                                                    const int32_t *__restrict__ targets, int V,
+                                                    const float *__restrict__ target_score, float *__restrict__ lse,
+                                                    float *loss, int mean, unsigned *done, float *__restrict__ total) {
+  __shared__ float2 sm[32][kFinishRows];
+  __shared__ double sums[32];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row0 = int64_t(blockIdx.x) * kFinishRows, row = row0 + (lane & 7);
   let_next_start();
   wait_for_previous();
+  // what the row's result needs of it, on its way early (an unwritten score is not used)
+  const int64_t mine = row0 + warp;
+  int y = -1;
+  float score = 0.f;
+  if (warp < kFinishRows && mine < rows) {
+    y = targets[mine];
+    score = target_score[mine];
+  }
+  float m = -INFINITY, l = 0.f;
+  auto join = [&](float om, float ol) {
+    const float mx = fmaxf(m, om);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    l = l * ex2((m - ref) * kLog2e) + ol * ex2((om - ref) * kLog2e);
+    m = mx;
+  };
+  if (row < rows) {
+#pragma unroll 4
+    for (int i = threadIdx.x >> 3; i < nparts; i += 128) {
+      const float2 x = __ldcs(part + int64_t(i) * rows + row);
+      join(x.x, x.y);
+    }
+  }
+  auto across = [&](int step) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, step), ol = __shfl_xor_sync(0xffffffffu, l, step);
+    join(om, ol);
+  };
+  across(8);
+  across(16);
+  if (lane < kFinishRows) sm[warp][lane] = make_float2(m, l);
+  __syncthreads();
+  if (warp < kFinishRows) {
+    m = sm[lane][warp].x, l = sm[lane][warp].y;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) across(step);
+    if (lane == 0 && mine < rows) {
+      const float v = m + logf(l);
+      lse[mine] = v;
+      loss[mine] = y >= 0 && y < V ? v - score : 0.f;
+    }
+  }
+  if (!total) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(done, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) s += double(row_loss[i]);
-  s = cta_sum(s, sm);
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) s += double(__ldcg(loss + i));
+  s = cta_sum(s, sums);
   if (mean) {
-    const double n = count_rows(targets, rows, V, sm);
+    const double n = count_rows(targets, rows, V, sums);
     s = n > 0.0 ? s / n : 0.0;
   }
-  if (threadIdx.x == 0) *loss = float(s);
+  if (threadIdx.x == 0) *total = float(s);
 }
 
 // The gradient of every row's loss.
-__global__ void __launch_bounds__(1024) row_scales(const float *__restrict__ dloss,
-                                                   const int32_t *__restrict__ targets, int64_t rows, int V,
-                                                   int reduction, float *__restrict__ scale) {
+struct Scales {
+  const float *dloss;
+  int reduction;
+  float *scale;
+};
+__device__ __forceinline__ void row_scales(const Scales &c, const int32_t *targets, int64_t rows, int V) {
   __shared__ double sm[32];
-  let_next_start();
-  wait_for_previous();
   float g = 1.0f;
-  if (reduction == SILCU_REDUCE_MEAN) {
+  if (c.reduction == SILCU_REDUCE_MEAN) {
     const double n = count_rows(targets, rows, V, sm);
-    g = float((dloss ? double(*dloss) : 1.0) / (n > 0.0 ? n : 1.0));
-  } else if (reduction == SILCU_REDUCE_SUM && dloss) {
-    g = *dloss;
+    g = float((c.dloss ? double(*c.dloss) : 1.0) / (n > 0.0 ? n : 1.0));
+  } else if (c.reduction == SILCU_REDUCE_SUM && c.dloss) {
+    g = *c.dloss;
   }
-  for (int64_t i = threadIdx.x; i < rows; i += 1024)
-    scale[i] = reduction == SILCU_REDUCE_NONE && dloss ? dloss[i] : g;
+  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+    c.scale[i] = c.reduction == SILCU_REDUCE_NONE && c.dloss ? c.dloss[i] : g;
 }
 
 // dst [rows, dp] = src [rows, D] (row stride ld), columns D.. zero; with
 // targets, rows that are left out are zero as well.  With `lo`, dst and lo
-// take the exact tf32 pair.
+// take the exact tf32 pair, with `scales` the first CTA writes the rows' scales.
 template <typename T>
 __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int64_t ld, int64_t rows, int D, int dp,
                                                  const int32_t *__restrict__ targets, int V, T *__restrict__ dst,
-                                                 float *__restrict__ lo) {
+                                                 float *__restrict__ lo, const Scales scales) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = dp / W;
   const bool vec = ld % W == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   const int64_t n = rows * per_row;
+  const int first = scales.scale ? 1 : 0;
   let_next_start();
   wait_for_previous();
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+  if (first && blockIdx.x == 0) {
+    row_scales(scales, targets, rows, V);
+    return;
+  }
+  for (int64_t i = int64_t(blockIdx.x - first) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x - first) * 256) {
     const int64_t r = i / per_row;
     const int c = int(i - r * per_row) * W;
     Raw<T, W> v = raw_zero<T, W>();
@@ -191,11 +224,19 @@ __global__ void __launch_bounds__(256) planes_finish(const float *__restrict__ p
     const int64_t r = i / per_row;
     const int c = int(i - r * per_row) * W;
     float f[W] = {};
-    for (int p = 0; p < nplanes; p++) {  // ldp is a multiple of W: the last vectors stay inside the row
-      float v[W];
-      load_f32<W>(planes + p * plane + r * ldp + c, v);
+    const float *src = planes + r * ldp + c;  // ldp is a multiple of W: the last vectors stay inside the row
+    constexpr int AHEAD = 32 / W;             // planes on their way at a time
+    for (int p = 0; p < nplanes; p += AHEAD) {
+      float v[AHEAD][W];
 #pragma unroll
-      for (int k = 0; k < W; k++) f[k] += v[k];
+      for (int j = 0; j < AHEAD; j++)
+        if (p + j < nplanes) load_f32<W>(src + (p + j) * plane, v[j]);
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++)
+        if (p + j < nplanes) {
+#pragma unroll
+          for (int k = 0; k < W; k++) f[k] += v[j][k];
+        }
     }
 #pragma unroll
     for (int k = 0; k < W; k++) f[k] *= k0;
@@ -283,9 +324,9 @@ bool rows16(const void *p, int64_t ld, int dtype) {
 
 // fp32 W is read as it is, and split inside the products, where few rows make
 // reading it the larger part of the work: forward and backward of 30 rows of
-// 60000 x 3000 took 2.18 ms with a split copy and take 1.15 without.  Every 128
-// rows split W again, so more rows are better off with the copy: 200 rows of the
-// same 1.30 ms with it, 1.34 without; 333 of 10007 x 768 173 and 256 us.
+// 60000 x 3000 took 2.18 ms with a split copy and 1.15 without (0.97 since dH is
+// transposed).  Every 128 rows split W again, so more rows are better off with the copy:
+// 200 rows of the same 1.30 ms with it, 1.34 without; 333 of 10007 x 768 173 and 256 us.
 constexpr int64_t kRawRows = 128;
 template <typename Ty>
 bool raw_w(const Args &a) {
@@ -317,10 +358,10 @@ struct Copy {
     if (Ty::PARTS == 2) lo = sp.take<float>(rows * dp);
   }
   silcu_status fill(const void *src, int64_t ld, int64_t rows, int64_t D, const int32_t *targets, int64_t V,
-                    cudaStream_t s) const {
+                    cudaStream_t s, const Scales &scales = {}) const {
     using T = typename Ty::T;
-    launch_after(copy_rows<T>, stream_grid(rows * dp * int64_t(sizeof(T)) / 16), 256, 0, s,
-                 static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo);
+    launch_after(copy_rows<T>, stream_grid(rows * dp * int64_t(sizeof(T)) / 16) + (scales.scale ? 1 : 0), 256, 0, s,
+                 static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo, scales);
     return check_launch("cross_entropy copy");
   }
   Operand operand(bool mn) const { return Operand{p, lo, dp, mn}; }
@@ -335,6 +376,7 @@ struct Forward {
   Copy<Ty> h, w;
   float2 *part;
   float *target_score, *row_loss;
+  unsigned *done;  // CTAs of loss_finish so far
 
   Forward(const Args &a, Space &sp) {
     copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
@@ -346,6 +388,7 @@ struct Forward {
     part = sp.take<float2>(int64_t(nparts) * a.rows);
     target_score = sp.take<float>(a.rows);
     row_loss = a.reduction == SILCU_REDUCE_NONE ? a.loss : sp.take<float>(a.rows);
+    done = sp.take<unsigned>(1);
     if (copy_h) h.take(sp, a.rows, a.D);
     if (copy_w) w.take(sp, piece, a.D);
   }
@@ -360,9 +403,10 @@ struct Gradient {
   int64_t M, N, K;
   int split = 1;
   bool wanted, direct;
+  bool transposed = false;    // computed as its transpose (kOutT): the N x M tiles hold all of M
   float *planes = nullptr;
   int tile = 2 * lossmm::BM;  // rows and columns of a tile (CTA pairs: 256; single CTAs: 128)
-  int64_t tiles() const { return ceil_div(M, tile) * ceil_div(N, tile); }
+  int64_t tiles() const { return (transposed ? 1 : ceil_div(M, tile)) * ceil_div(N, tile); }
   int64_t units() const { return tile == lossmm::BM ? sm_count() : sm_count() / 2; }
 };
 
@@ -442,7 +486,15 @@ struct Backward {
     dh.M = a.rows, dh.N = a.D, dh.K = piece, dh.wanted = a.dH;
     dw.M = piece, dw.N = a.D, dw.K = a.rows, dw.wanted = a.dW;
     if (score.raw) dh.tile = dw.tile = lossmm::BM;
-    choose_splits(dh, dw, Ty::PARTS == 2);
+    dh.transposed = a.rows <= lossmm::BM;
+    if (dh.transposed) {  // a launch of its own
+      Gradient none = {};
+      none.K = 1, none.wanted = false;
+      choose_splits(dh, none, Ty::PARTS == 2);
+      choose_splits(none, dw, Ty::PARTS == 2);
+    } else {
+      choose_splits(dh, dw, Ty::PARTS == 2);
+    }
     dh.direct = dh.split == 1 && piece == a.V;  // else pieces add up in the planes
     dw.direct = dw.split == 1;
     for (Gradient *g : {&dh, &dw})
@@ -478,11 +530,11 @@ silcu_status scores(lossmm::Params &p, const ScoreTiles &t, cudaStream_t s) {
   return t.pair ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
 }
 
-template <typename Ty>
+template <typename Ty, int EPI>
 silcu_status products(lossmm::Params &p, bool pairs, int count, cudaStream_t s) {
   if constexpr (Ty::PARTS == 2)
-    if (!pairs) return lossmm::launch<Ty, lossmm::kOut, false, true>(p, count, s);
-  return lossmm::launch<Ty, lossmm::kOut, true>(p, count, s);
+    if (!pairs) return lossmm::launch<Ty, EPI, false, true>(p, count, s);
+  return lossmm::launch<Ty, EPI, true>(p, count, s);
 }
 
 template <typename T>
@@ -518,15 +570,14 @@ silcu_status forward(const Args &a, const Forward<Ty> &f, cudaStream_t s) {
     p.loss.v0 = int32_t(v0);
     p.loss.part = f.part;
     p.loss.target_score = f.target_score;
+    p.loss.done = f.done;
     if ((st = scores<Ty, lossmm::kStats>(p, f.tiles, s)) != SILCU_OK) return st;
     part0 += f.parts(a, v0);
   }
-  launch_after(loss_finish, uint32_t((a.rows + 31) / 32), 1024, 0, s, f.part, f.nparts, a.rows, a.targets, int(a.V),
-               f.target_score, a.lse, f.row_loss);
-  if ((st = check_launch("cross_entropy finish")) != SILCU_OK || a.reduction == SILCU_REDUCE_NONE) return st;
-  launch_after(loss_reduce, 1, 1024, 0, s, f.row_loss, a.targets, a.rows, int(a.V),
-               int(a.reduction == SILCU_REDUCE_MEAN), a.loss);
-  return check_launch("cross_entropy reduce");
+  launch_after(loss_finish, uint32_t(ceil_div(a.rows, kFinishRows)), 1024, 0, s, f.part, f.nparts, a.rows, a.targets,
+               int(a.V), f.target_score, a.lse, f.row_loss, int(a.reduction == SILCU_REDUCE_MEAN), f.done,
+               a.reduction == SILCU_REDUCE_NONE ? nullptr : a.loss);
+  return check_launch("cross_entropy finish");
 }
 
 // Where a product of ds goes: the result itself, or planes that earlier
@@ -562,9 +613,8 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
   using T = typename Ty::T;
   constexpr int BK = lossmm::Cfg<Ty, lossmm::kOut, true>::BK;
   silcu_status st;
-  launch_after(row_scales, 1, 1024, 0, s, a.dloss, a.targets, a.rows, int(a.V), a.reduction, b.scale);
-  if ((st = check_launch("cross_entropy scales")) != SILCU_OK) return st;
-  if ((st = b.h.fill(a.H, a.ldh, a.rows, a.D, a.targets, a.V, s)) != SILCU_OK) return st;
+  if ((st = b.h.fill(a.H, a.ldh, a.rows, a.D, a.targets, a.V, s, Scales{a.dloss, a.reduction, b.scale})) != SILCU_OK)
+    return st;
   // A factor that all rows share leaves ds alone where ds is rounded.
   const bool shared = Ty::PARTS == 1 && a.reduction != SILCU_REDUCE_NONE;
   const float *alpha = shared ? b.scale : nullptr;
@@ -591,19 +641,28 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     p.loss.scale = shared ? nullptr : b.scale;
     if ((st = scores<Ty, lossmm::kScoreGrad>(p, b.score, s)) != SILCU_OK) return st;
 
-    // Both products of ds in one launch, the one with the longer items first.
-    memset(&p, 0, sizeof(p));
-    p.err = device_error_ptr();
     const bool pairs = !b.score.raw;
-    p.bn = pairs ? lossmm::BN : lossmm::BM;
-    p.rows_a = lossmm::BM;
-    p.alpha = alpha;
-    if (!pairs) set_raw(p);
-    int count = 0;
     w.mn = true;
+    auto clear = [&](int bn) {
+      memset(&p, 0, sizeof(p));
+      p.err = device_error_ptr();
+      p.bn = bn;
+      p.rows_a = lossmm::BM;
+      p.alpha = alpha;
+      if (!pairs) set_raw(p);
+    };
+    if (b.dh.wanted && b.dh.transposed) {
+      clear(int(up(a.rows, 32)));
+      if (!lossmm::set_problem<Ty>(p.p[0], pairs, p.bn, lossmm::BM, a.D, a.rows, n, w, b.ds.operand(false))) return map_error();
+      set_output(p.p[0], b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
+      if ((st = products<Ty, lossmm::kOutT>(p, pairs, 1, s)) != SILCU_OK) return st;
+    }
+    // Both products of ds in one launch, the one with the longer items first.
+    clear(pairs ? lossmm::BN : lossmm::BM);
+    int count = 0;
     const bool dw_first = b.dw.K / b.dw.split > b.dh.K / b.dh.split;
     for (const bool is_dw : {dw_first, !dw_first}) {
-      if (!(is_dw ? b.dw : b.dh).wanted) continue;
+      if (is_dw ? !b.dw.wanted : !b.dh.wanted || b.dh.transposed) continue;
       lossmm::Problem &q = p.p[count++];
       if (is_dw) {
         if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
@@ -615,7 +674,7 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
         set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
       }
     }
-    if ((st = products<Ty>(p, pairs, count, s)) != SILCU_OK) return st;
+    if (count && (st = products<Ty, lossmm::kOut>(p, pairs, count, s)) != SILCU_OK) return st;
     if (b.dw.wanted && !b.dw.direct) {
       st = finish_planes<Ty>(b.dw, n, a.D, alpha, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, s);
       if (st != SILCU_OK) return st;
@@ -699,8 +758,8 @@ silcu_status silcu_linear_cross_entropy(const silcu_cross_entropy_args *ap, void
     return fail(SILCU_INVALID_ARGUMENT, "linear_cross_entropy: null pointer");
   if (a.rows == 0) {
     if (a.reduction == SILCU_REDUCE_NONE) return SILCU_OK;
-    loss_reduce<<<1, 1024, 0, s>>>(nullptr, nullptr, 0, int(a.V), 0, a.loss);
-    return check_launch("linear_cross_entropy");
+    const cudaError_t r = cudaMemsetAsync(a.loss, 0, sizeof(float), s);
+    return r == cudaSuccess ? SILCU_OK : fail(SILCU_CUDA_ERROR, "linear_cross_entropy: %s", cudaGetErrorString(r));
   }
   if ((st = check_pointers("linear_cross_entropy", a)) != SILCU_OK) return st;
   const int64_t e = int64_t(dtype_bytes(a.dtype));

@@ -23,6 +23,7 @@ struct LossArgs {
   int32_t v0, V;           // vocabulary index of this launch's column 0; vocabulary size
   float2 *part;            // forward: [parts][rows] (m, l)
   float *target_score;     // forward: [rows], written for rows that count
+  unsigned *done;          // forward: set to 0 for what follows
   const float *lse;        // backward: [rows]
   const float *scale;      // backward: [rows] gradient of each row's loss, or null = 1
 };

@@ -44,7 +44,7 @@ using namespace tc;
 
 constexpr int BM = 128, BN = 256;
 
-enum Epilogue { kStats = 0, kScoreGrad = 1, kOut = 2 };
+enum Epilogue { kStats = 0, kScoreGrad = 1, kOut = 2, kOutT = 3 };
 enum OutMode { kDirect = 0, kPlane = 1, kPlaneAdd = 2 };
 
 // mbar_wait without its call: around a call the 128 sums of an epilogue thread
@@ -82,6 +82,13 @@ __device__ __forceinline__ void red_add4(float *p, const uint4 &v) {
                : "memory");
 }
 
+__device__ __forceinline__ void red_add(float *p, float v) {
+  asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ void store_as(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_as(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
 // x rounded to tf32 as cvt.rna.tf32 does (halves away from zero), on the
 // integer pipe: the conversion took 70 of 660 us of the score gradients.
 __device__ __forceinline__ float tf32_rna_bits(float x) {
@@ -107,6 +114,7 @@ struct Tf32 {
 template <typename Ty, int EPI, bool PAIR, bool RAW = false>
 struct Cfg {
   static_assert(!RAW || (Ty::PARTS == 2 && !PAIR), "raw operands: tf32 on single CTAs");
+  static_assert(RAW || PAIR || (EPI != kOut && EPI != kOutT), "only the scores run on single CTAs otherwise");
   static constexpr int TM = PAIR ? 2 * BM : BM;
   static constexpr int ROWS_B = PAIR ? BN / 2 : BN;  // B columns held per CTA
   static constexpr int SUBS = PAIR && Ty::PARTS == 1 ? 2 : 1;  // 128-byte-row tiles of each operand per stage
@@ -126,7 +134,7 @@ struct Cfg {
   static constexpr int LD = Ty::PARTS == 2 ? 16 : 32;
   // The tf32 sums go back to TMEM for the epilogues that have no registers beside
   // them (with the 128 sums in registers the score gradients spill 2.8 KB a thread).
-  static constexpr bool BACK = MULTI && EPI != kStats;
+  static constexpr bool BACK = MULTI && (EPI == kScoreGrad || EPI == kOut);
   static constexpr int CHUNK = !MULTI ? 1 << 30 : (Ty::PARTS == 2 ? 128 : 1024) / BK;
   static constexpr int GROUP_M = EPI == kOut ? 8 : 16;
   static constexpr uint32_t MN_BOX = Ty::KROW * 128;       // KROW elements of M / N x KROW k
@@ -135,12 +143,28 @@ struct Cfg {
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
+// Division of 0 <= n < 2^31 by a divisor known on the host: with 2^l >= d, m =
+// floor(2^(31 + l) / d) + 1 is off by less than 1 and n m / 2^(31 + l) by less than 1 / d.
+struct Divisor {
+  uint32_t m, shift;
+  void set(int d) {
+    int l = 0;
+    while ((int64_t(1) << l) < d) l++;
+    shift = uint32_t(31 + l);
+    m = uint32_t((uint64_t(1) << shift) / uint64_t(d) + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return int((uint64_t(uint32_t(n)) * m) >> shift); }
+};
+
 struct Problem {
   CUtensorMap a[2], b[2];  // [part]: hi, lo (tf32)
   int M, N, K, tiles_m, tiles_n;
+  // What tile_of divides by (set in launch): the epilogue of a short tile waits for it,
+  // and three divisions at run time take 900 cycles.
+  Divisor by_split, by_group, by_last;
   int ksplit;              // each tile's K range in this many parts (kOut; part i -> plane i)
-  int amn;                 // kOut: A is stored with the M index contiguous
-  int raw;                 // RAW kernels: B is plain fp32 (b[0]), split in shared memory
+  int amn;                 // kOut: A is stored with the M index contiguous (kOutT: it always is)
+  int raw;                 // RAW kernels: B (kOutT: A) is plain fp32, split in shared memory
   int mode, vec;           // vec: kDirect rows are 16-byte aligned
   void *out;
   int64_t ldo, plane;      // row stride; elements from one plane to the next
@@ -150,12 +174,12 @@ struct __align__(64) Params {
   Problem p[2];  // kOut: up to two products in one launch
   void *ds[2];       // score gradients [part]: [M, lds], lds a multiple of 64
   int64_t lds;
-  int bn;            // tile columns
+  int bn;            // tile columns (of the scores and kOut on CTA pairs: BN)
   int rows_a;        // rows of A's boxes (single CTAs; the rest of a tile is never stored)
   int half;          // columns of an epilogue warp (RAW; else 128)
   int stages;        // ring stages (RAW)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
-  int units, n0, n1, tail, extra;
+  int units, n0, n1, rounds, tail, extra;  // rounds = n0 / units, tail = n0 % units
   const float *alpha;  // kOut: factor of kDirect results in bf16, or null
   LossArgs loss;
   int part0;  // index of this launch's first part
@@ -171,12 +195,11 @@ struct Work {
 // the second product's (about one item of the first in cost), and the rest goes
 // round all units.
 __device__ __forceinline__ bool work_at(const Params &p, int u, int k, Work &w) {
-  const int q0 = u < p.n0 ? (p.n0 - u + p.units - 1) / p.units : 0;
-  if (k < q0) {
+  if (u + k * p.units < p.n0) {
     w = Work{0, u + k * p.units};
     return true;
   }
-  k -= q0;
+  k -= p.rounds + (u < p.tail);  // the unit's items of the first product
   const int low = p.units - p.tail;  // units short of one item
   int j;
   if (p.tail && u >= p.tail) j = k < p.extra ? k * low + u - p.tail : p.extra * low + (k - p.extra) * p.units + u;
@@ -191,14 +214,15 @@ struct Tile {
 
 template <typename C>
 __device__ __forceinline__ Tile tile_of(const Problem &q, int bn, int item) {
-  const int t = item / q.ksplit, part = item - t * q.ksplit;
-  const int group = t / (C::GROUP_M * q.tiles_n);
+  const int t = q.by_split(item), part = item - t * q.ksplit;
+  const int group = q.by_group(t);
   const int first = group * C::GROUP_M;
   const int gm = q.tiles_m - first < C::GROUP_M ? q.tiles_m - first : C::GROUP_M;
   const int r = t - group * C::GROUP_M * q.tiles_n;
   const int nk = (q.K + C::BK - 1) / C::BK;
-  return Tile{(first + r % gm) * C::TM, (r / gm) * bn, int(int64_t(part) * nk / q.ksplit),
-              int(int64_t(part + 1) * nk / q.ksplit), part};
+  const int col = gm == C::GROUP_M ? r / C::GROUP_M : q.by_last(r), row = first + r - col * gm;
+  // at most 32 parts of 2^24 k: the products stay below 2^31
+  return Tile{row * C::TM, col * bn, q.by_split(part * nk), q.by_split((part + 1) * nk), part};
 }
 
 template <typename Ty, typename C>
@@ -210,7 +234,13 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
 // The scores' operands both have k contiguous; of kOut's, B has the N index contiguous
 // (BMN) and A what Problem::amn says.
 //
-// RAW: B may be plain fp32.  Its tile is the hi operand as it stands (the
+// kOutT stores its result transposed, D[m, n] at out[n][m]: dH of few rows as
+// (W^T ds^T)^T.  W, with the M index contiguous, then fills the tile's 128 or 256 rows
+// and ds its few columns, and an MMA takes the time of the columns that exist.  As
+// ds . W the few rows were padded to a whole tile: 30 rows of 60000 x 3000
+// took 185 us of the tensor pipe's time in bf16 and 580 in fp32.
+//
+// RAW: one operand may be plain fp32.  Its tile is the hi operand as it stands (the
 // tensor core reads the upper 19 bits of a value), and the epilogue warps, idle
 // while the MMAs run, write the remainders beside it.  For few rows, where the
 // time is that of reading W, this spares writing and reading a split copy.
@@ -219,7 +249,7 @@ template <typename Ty, int EPI, bool PAIR, bool RAW>
 __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(const __grid_constant__ Params p) {
   using C = Cfg<Ty, EPI, PAIR, RAW>;
   using T = typename Ty::T;
-  constexpr bool BMN = EPI == kOut;
+  constexpr bool BMN = EPI == kOut, RAW_A = EPI == kOutT;
   constexpr int NBUF = C::NBUF, PARTS = Ty::PARTS, SUBS = C::SUBS;
   const int TILE_A = RAW ? p.rows_a * 128 : C::TILE_A, TILE_B = RAW ? p.bn * 128 : C::TILE_B;
   const int SUB_BYTES = PARTS * (TILE_A + TILE_B), STAGE_BYTES = SUBS * SUB_BYTES;
@@ -235,7 +265,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
-  const int bn = PAIR ? BN : p.bn;
+  const int bn = PAIR && EPI != kOutT ? BN : p.bn;
 
   let_next_start();
   if (threadIdx.x == 0) {
@@ -265,19 +295,21 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   wait_for_previous();
+  if (EPI == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.loss.done = 0u;
   Work w;
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t kbg = 0;
       bool ok = true;
-      const uint32_t bytes = SUBS * PARTS * ((PAIR ? TILE_A : p.rows_a * 128) + (PAIR ? TILE_B : bn * 128)) * (PAIR ? 2 : 1);
+      const uint32_t bytes =
+          SUBS * PARTS * ((PAIR ? TILE_A : p.rows_a * 128) * (PAIR ? 2 : 1) + bn * 128);  // a pair's, on the even CTA
       const int boxes_b = RAW ? bn / Ty::KROW : C::MN_BOXES_B;
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
         const Problem &q = p.p[w.prob];
         const Tile tl = tile_of<C>(q, bn, w.item);
-        const int am = tl.m0 + BM * int(rank), nb = tl.n0 + C::ROWS_B * int(rank);
-        const bool amn = EPI == kOut && q.amn;
+        const int am = tl.m0 + BM * int(rank), nb = tl.n0 + (PAIR ? bn / 2 : 0) * int(rank);
+        const bool amn = EPI == kOutT || (EPI == kOut && q.amn);
         for (int kb = tl.kb0; kb < tl.kb1; kb++, kbg++) {
           const uint32_t s = kbg % STAGES, ph = (kbg / STAGES) & 1;
           if (kbg >= STAGES && !mbar_try_wait(empty0 + 8 * s, ph ^ 1) &&
@@ -287,7 +319,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           }
           // a pair's bytes all complete on the even CTA's barrier
           const uint32_t bar = PAIR ? mapa_shared(full0 + 8 * s, 0) : full0 + 8 * s;
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, RAW && q.raw ? bytes - TILE_B : bytes);
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, RAW && q.raw ? bytes - (RAW_A ? TILE_A : TILE_B) : bytes);
           auto load = [&](uint32_t dst, const CUtensorMap *map, int c0, int c1) {
             if (PAIR) tma_load_2d_pair(dst, map, bar, c0, c1);
             else tma_load_2d(dst, map, bar, c0, c1);
@@ -298,6 +330,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
             uint32_t dst = smem_u32(smem + s * STAGE_BYTES + u * SUB_BYTES);
 #pragma unroll
             for (int h = 0; h < PARTS; h++, dst += TILE_A) {
+              if (RAW && RAW_A && q.raw && h == 1) continue;
               if (amn) {
 #pragma unroll
                 for (int i = 0; i < C::MN_BOXES_A; i++) load(dst + i * C::MN_BOX, &q.a[h], am + Ty::KROW * i, kc);
@@ -307,7 +340,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
             }
 #pragma unroll
             for (int h = 0; h < PARTS; h++, dst += TILE_B) {
-              if (RAW && q.raw && h == 1) break;
+              if (RAW && !RAW_A && q.raw && h == 1) break;
               if (BMN) {
 #pragma unroll
                 for (int i = 0; i < boxes_b; i++) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
@@ -328,7 +361,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
         const Problem &q = p.p[w.prob];
         const Tile tl = tile_of<C>(q, bn, w.item);
-        const bool amn = EPI == kOut && q.amn;
+        const bool amn = EPI == kOutT || (EPI == kOut && q.amn);
         const uint64_t adesc = operand_desc<Ty, C>(base, amn), bdesc = operand_desc<Ty, C>(base + PARTS * TILE_A, BMN);
         const uint32_t astep = (amn ? C::MN_STEP : 32u) >> 4, bstep = (BMN ? C::MN_STEP : 32u) >> 4;
         const uint32_t idesc = (1u << 4) | Ty::FORMAT | (uint32_t(amn) << 15) | (uint32_t(BMN) << 16) |
@@ -389,7 +422,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
     const int qr = warp & 3, h = (warp - 2) >> 2;
     float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
     const int half = RAW ? p.half : 128;
-    const float alpha = EPI == kOut && p.alpha ? *p.alpha : 1.0f;
+    const float alpha = (EPI == kOut || EPI == kOutT) && p.alpha ? *p.alpha : 1.0f;
     uint32_t cg = 0, kbe = 0;
     bool ok = true;
     for (int k = 0; ok && work_at(p, unit, k, w); k++) {
@@ -399,7 +432,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       const int row = r0 + lane;
       // this warp's columns of the tile (may be <= 0)
       const int cols = min(min(q.N, tl.n0 + bn), c0 + half) - c0;
-      // RAW: the next `n` stages' remainders x - tf32(x) of a raw B, for the MMAs.
+      // RAW: the next `n` stages' remainders x - tf32(x) of the raw operand, for the MMAs.
       // Every warp sees every raw use of a slot, so no barrier is ever more than
       // one phase ahead of it.
       auto remainders = [&](int n) {
@@ -410,8 +443,9 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         for (int i = 0; i < n; i++, kbe++) {
           const uint32_t s = kbe % STAGES;
           if (!__all_sync(0xffffffffu, wait_inline(full0 + 8 * s, (kbe / STAGES) & 1, p.err, 25))) return false;
-          float4 *hi = reinterpret_cast<float4 *>(smem + s * STAGE_BYTES + 2 * TILE_A), *lo = hi + TILE_B / 16;
-          for (int e = int(threadIdx.x) - 64; e < TILE_B / 16; e += 32 * C::EPI_WARPS) {
+          const int tile = RAW_A ? TILE_A : TILE_B;
+          float4 *hi = reinterpret_cast<float4 *>(smem + s * STAGE_BYTES + (RAW_A ? 0 : 2 * TILE_A)), *lo = hi + tile / 16;
+          for (int e = int(threadIdx.x) - 64; e < tile / 16; e += 32 * C::EPI_WARPS) {
             float4 x = hi[e];
             x.x = __fsub_rn(x.x, tf32_trunc(x.x));
             x.y = __fsub_rn(x.y, tf32_trunc(x.y));
@@ -436,7 +470,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         __syncwarp();
         if (lane == 0) {
           const uint32_t bar = tempty0 + 8 * (t % NBUF);
-          if (PAIR) mbar_arrive_cluster(mapa_shared(bar, 0));
+          if (PAIR) mbar_arrive_cluster_relaxed(mapa_shared(bar, 0));
           else mbar_arrive(bar);
         }
       };
@@ -446,7 +480,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       int y = -1;
       float lse = 0.f, g = 0.f;
       auto row_data = [&] {
-        if (EPI != kOut && row < q.M) {
+        if ((EPI == kStats || EPI == kScoreGrad) && row < q.M) {
           y = max(p.loss.targets[row], -1);  // any negative one; differences with it do not overflow
           if (EPI == kScoreGrad) {
             lse = p.loss.lse[row] * kLog2e;
@@ -479,6 +513,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           if (ok && cols > 0) {
 #pragma unroll
             for (int cb = 0; cb < 128; cb += C::LD) {
+              if (EPI == kOutT && cb >= cols) break;
               float r[C::LD];
               tmem_ld_cols<C::LD>(src0 + (cg % NBUF) * BN + cb, r);
               tmem_ld_done(r);
@@ -529,22 +564,38 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       auto put = [&](int i, uint4 v) {
         *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(st) + lane * 128 + 16 * (i ^ (lane & 7))) = v;
       };
-      // The staged block to rows r0.. of `out` from column col0 on, 8 lanes a row:
-      // write(address, 16 bytes, columns that exist from there on), where any do.
+      // The staged block to rows r0.. of `out` from column col0 on, 8 lanes a row.  A
+      // lane with at least `whole` columns from its own on writes vector(address, 16
+      // bytes), one with fewer single(address, 16 bytes, columns).  Several vectors are
+      // read before the first is written: one by one they took 150 cycles each, and
+      // the epilogue of a short product was all there was (dW of 30 rows of 60000 x
+      // 3000, bf16: 156 us).
+      constexpr int AT_ONCE = PARTS == 2 && EPI == kScoreGrad ? 4 : 8;  // eight spill there
       const int rows_left = q.M - r0 - (lane >> 3);
-      auto send = [&](auto *out, int64_t ld, int col0, auto &&write) {
+      auto send = [&](auto *out, int64_t ld, int col0, int whole, auto &&vector, auto &&single) {
         constexpr int W = 16 / int(sizeof(*out));
         const int ch = lane & 7, left = c0 + cols - col0 - W * ch;
         auto *dst = out + int64_t(r0 + (lane >> 3)) * ld + col0 + W * ch;
         const char *src = reinterpret_cast<const char *>(st) + (lane >> 3) * 128;
         const int even = 16 * (ch ^ (lane >> 3)), odd = 16 * (ch ^ ((lane >> 3) + 4));
         __syncwarp();
-        if (left > 0) {
 #pragma unroll
-          for (int i = 0; i < 8; i++, dst += 4 * ld)
-            if (4 * i < rows_left) write(dst, *reinterpret_cast<const uint4 *>(src + 512 * i + (i & 1 ? odd : even)), left);
+        for (int i0 = 0; i0 < 8; i0 += AT_ONCE) {
+          uint4 x[AT_ONCE];
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; i++)
+            x[i] = *reinterpret_cast<const uint4 *>(src + 512 * (i0 + i) + (i & 1 ? odd : even));
+          if (i0 + AT_ONCE == 8) __syncwarp();
+          if (left >= whole) {
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++, dst += 4 * ld)
+              if (4 * (i0 + i) < rows_left) vector(dst, x[i]);
+          } else if (left > 0) {
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++, dst += 4 * ld)
+              if (4 * (i0 + i) < rows_left) single(dst, x[i], left);
+          }
         }
-        __syncwarp();
       };
       constexpr int UNROLL = IN_REGS ? 4 : 1;
 
@@ -566,7 +617,8 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           const bool counts = y >= 0 && y < p.loss.V;
           const int at = y - p.loss.v0 - c0;
           // plain stores need no wait before the next block; rows of ds end on whole vectors
-          auto whole = [](T *dst, const uint4 &x, int) { *reinterpret_cast<uint4 *>(dst) = x; };
+          auto store = [](T *dst, const uint4 &x) { *reinterpret_cast<uint4 *>(dst) = x; };
+          auto none = [](T *, const uint4 &, int) {};
 #pragma unroll UNROLL
           for (int cb = 0; cb < 4; cb++) {
             if (32 * cb < cols) {
@@ -579,7 +631,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
                   put(4 * (cb & 1) + i, make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
                                                    pack_bf16(v[8 * i + 4], v[8 * i + 5]),
                                                    pack_bf16(v[8 * i + 6], v[8 * i + 7])));
-                if ((cb & 1) || 32 * (cb + 1) >= cols) send(static_cast<T *>(p.ds[0]), p.lds, c0 + 32 * (cb & ~1), whole);
+                if ((cb & 1) || 32 * (cb + 1) >= cols) send(static_cast<T *>(p.ds[0]), p.lds, c0 + 32 * (cb & ~1), 1, store, none);
               } else {  // the exact tf32 pair, 32 columns per row each
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
@@ -593,15 +645,38 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
                     }
                     put(i, make_uint4(e[0], e[1], e[2], e[3]));
                   }
-                  send(static_cast<T *>(p.ds[part]), p.lds, c0 + 32 * cb, whole);
+                  send(static_cast<T *>(p.ds[part]), p.lds, c0 + 32 * cb, 1, store, none);
+                }
+              }
+            }
+          }
+        }
+      } else if constexpr (EPI == kOutT) {  // 32 lanes hold 32 neighbours of an output row
+#pragma unroll UNROLL
+        for (int cb = 0; cb < 4; cb++) {
+          if (32 * cb < cols) {
+            float v[32];
+            block(cb, v);
+            if (row < q.M) {
+              const int64_t at = int64_t(c0 + 32 * cb) * q.ldo + row;
+#pragma unroll
+              for (int i = 0; i < 32; i++) {
+                if (32 * cb + i < cols) {
+                  if (q.mode == kDirect) store_as(static_cast<T *>(q.out) + at + i * q.ldo, alpha * v[i]);
+                  else if (q.mode == kPlane) static_cast<float *>(q.out)[tl.part * q.plane + at + i * q.ldo] = v[i];
+                  else red_add(static_cast<float *>(q.out) + tl.part * q.plane + at + i * q.ldo, v[i]);
                 }
               }
             }
           }
         }
       } else if (r0 < q.M) {
-        const bool direct16 = q.mode == kDirect && PARTS == 1;
+        const int mode = q.mode;
+        const bool direct16 = mode == kDirect && PARTS == 1;
+        const int64_t ldo = q.ldo;
         float *out = static_cast<float *>(q.out) + tl.part * q.plane;
+        // planes' rows hold whole vectors; results' may end or lie elsewhere
+        const int whole = mode != kDirect ? 1 : q.vec ? 16 / int(sizeof(T)) : 1 << 30;
 #pragma unroll UNROLL
         for (int cb = 0; cb < 4; cb++) {
           if (32 * cb < cols) {
@@ -616,34 +691,31 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
                                pack_bf16(alpha * v[8 * i + 4], alpha * v[8 * i + 5]),
                                pack_bf16(alpha * v[8 * i + 6], alpha * v[8 * i + 7])));
               if ((cb & 1) || 32 * (cb + 1) >= cols)
-                send(static_cast<unsigned short *>(q.out), q.ldo, c0 + 32 * (cb & ~1),
-                     [&](unsigned short *dst, const uint4 &x, int left) {
-                       if (q.vec && left >= 8) {
-                         *reinterpret_cast<uint4 *>(dst) = x;
-                       } else {
-                         const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+                send(
+                    static_cast<unsigned short *>(q.out), ldo, c0 + 32 * (cb & ~1), whole,
+                    [](unsigned short *dst, const uint4 &x) { *reinterpret_cast<uint4 *>(dst) = x; },
+                    [](unsigned short *dst, const uint4 &x, int left) {
+                      const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                         for (int t = 0; t < 8; t++)
-                           if (t < left) dst[t] = static_cast<unsigned short>(e[t >> 1] >> (16 * (t & 1)));
-                       }
-                     });
+                      for (int t = 0; t < 8; t++)
+                        if (t < left) dst[t] = static_cast<unsigned short>(e[t >> 1] >> (16 * (t & 1)));
+                    });
             } else {  // 32 fp32 columns
 #pragma unroll
               for (int i = 0; i < 8; i++)
                 put(i, make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
                                   __float_as_uint(v[4 * i + 3])));
-              send(out, q.ldo, c0 + 32 * cb, [&](float *dst, const uint4 &x, int left) {
-                if (q.mode == kPlaneAdd) {
-                  red_add4(dst, x);
-                } else if (q.mode == kPlane || (q.vec && left >= 4)) {  // a plane's rows hold whole vectors
-                  *reinterpret_cast<uint4 *>(dst) = x;
-                } else {
-                  const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+              auto single = [](float *dst, const uint4 &x, int left) {
+                const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                  for (int t = 0; t < 4; t++)
-                    if (t < left) dst[t] = __uint_as_float(e[t]);
-                }
-              });
+                for (int t = 0; t < 4; t++)
+                  if (t < left) dst[t] = __uint_as_float(e[t]);
+              };
+              if (mode == kPlaneAdd)
+                send(out, ldo, c0 + 32 * cb, whole, [](float *dst, const uint4 &x) { red_add4(dst, x); }, single);
+              else
+                send(out, ldo, c0 + 32 * cb, whole, [](float *dst, const uint4 &x) { *reinterpret_cast<uint4 *>(dst) = x; },
+                     single);
             }
           }
         }
@@ -696,8 +768,8 @@ bool set_problem(Problem &q, bool pair, int bn, int rows_a, int64_t M, int64_t N
   q.tiles_n = int((N + bn - 1) / bn);
   q.ksplit = 1;
   q.amn = a.mn;
-  q.raw = Ty::PARTS == 2 && !b.lo;
-  return operand_map<Ty>(q.a, a, M, K, rows_a) && operand_map<Ty>(q.b, b, N, K, pair ? BN / 2 : bn);
+  q.raw = Ty::PARTS == 2 && (!a.lo || !b.lo);
+  return operand_map<Ty>(q.a, a, M, K, rows_a) && operand_map<Ty>(q.b, b, N, K, pair ? bn / 2 : bn);
 }
 
 inline int64_t items_of(const Problem &q) { return int64_t(q.tiles_m) * q.tiles_n * q.ksplit; }
@@ -720,7 +792,14 @@ silcu_status launch(Params &p, int problems, cudaStream_t s) {
   p.n0 = int(n0);
   p.n1 = int(n1);
   p.units = int(n0 + n1 < most ? n0 + n1 : most);
+  p.rounds = int(n0 / p.units);
   p.tail = int(n0 % p.units);
+  for (int i = 0; i < problems; i++) {
+    Problem &q = p.p[i];
+    q.by_split.set(q.ksplit);
+    q.by_group.set(C::GROUP_M * q.tiles_n);
+    q.by_last.set(q.tiles_m % C::GROUP_M ? q.tiles_m % C::GROUP_M : C::GROUP_M);
+  }
   p.extra = 0;
   if (n1 && p.tail) {  // an item of the first product in items of the second, by their k
     const double c0 = double(p.p[0].K) / p.p[0].ksplit, c1 = double(p.p[1].K) / p.p[1].ksplit;

@@ -138,12 +138,28 @@ def test_reductions(cuda, reduction, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows,V,D,piece", [(300, 1500, 200, 256), (130, 1025, 64, 512), (40, 5000, 65, 1024),
-                                            (600, 900, 520, 256)])
+                                            (600, 900, 520, 256), (100, 3000, 64, 512), (1, 2000, 160, 256)])
 def test_vocabulary_pieces(cuda, monkeypatch, rows, V, D, piece, dtype):
     """The same result from several pieces, a short last one among them."""
     H, W, y = make(rows, V, D, dtype, V)
     monkeypatch.setenv("SILCU_LOSS_PIECE", str(piece))
     check(H, W, y, *run(H, W, y))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,V,D", [(31, 1200, 100), (128, 600, 264), (129, 600, 264)])
+def test_one_gradient_alone(cuda, rows, V, D, dtype):
+    """dH or dW by itself is what both together give, and nothing past its rows or columns is written."""
+    H, W, y = make(rows, V, D, dtype, 8)
+    _, lse, dH, dW = run(H, W, y)
+    for i, full in enumerate((dH, dW)):
+        wide = torch.full((full.shape[0] + 2, D + 24), 7.0, device="cuda", dtype=dtype)
+        out = wide[1:-1, 8:-16]
+        kw = {"need_dW": False, "dH": out} if i == 0 else {"need_dH": False, "dW": out}
+        got = gpu.linear_cross_entropy_backward(H, W, y, lse, **kw)
+        assert got[1 - i] is None and torch.equal(out, full)
+        out.fill_(7.0)
+        assert bool((wide == 7.0).all())
 
 
 @pytest.mark.parametrize("dtype,rows,V,D", [(torch.bfloat16, 8192, 70001, 64), (torch.float32, 8192, 20011, 64)])
