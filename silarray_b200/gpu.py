@@ -489,6 +489,14 @@ def _at(what, t, dtype, n, index):
     raise ValueError(f"{what}: expected {n} elements, got {t.numel()}")
 
 
+def _out(what, t, like, n, index):
+    """An output and its address: t itself, or (None) a new tensor like `like`."""
+    if t is None:
+        t = torch.empty_like(like)
+        return t, t.data_ptr()
+    return t, _at(what, t, like.dtype, n, index)
+
+
 def _scratch(nbytes, device):
     """Scratch of one call (the tensor and its address).  It comes from torch's
     caching allocator each time, so calls on several streams or in several
@@ -524,11 +532,10 @@ def layer_norm_forward(IN, OUT=None, gamma=None, beta=None, rows=None, cols=None
     x = _at("layer_norm IN", IN, IN.dtype, n, index)
     g = _at("layer_norm gamma", gamma, _F32, cols, index)
     b = _at("layer_norm beta", beta, _F32, cols, index)
-    OUT = torch.empty_like(IN) if OUT is None else OUT
-    mean = torch.empty(rows, dtype=_F32, device=IN.device)
-    rstd = torch.empty(rows, dtype=_F32, device=IN.device)
-    _launch(lib().silcu_layer_norm_forward, index, x, _at("layer_norm OUT", OUT, IN.dtype, n, index),
-            mean.data_ptr(), rstd.data_ptr(), g, b, rows, cols, eps, dt)
+    OUT, out = _out("layer_norm OUT", OUT, IN, n, index)
+    mean = gamma.new_empty(rows)
+    rstd = torch.empty_like(mean)
+    _launch(lib().silcu_layer_norm_forward, index, x, out, mean.data_ptr(), rstd.data_ptr(), g, b, rows, cols, eps, dt)
     return OUT, mean, rstd
 
 
@@ -543,14 +550,12 @@ def layer_norm_backward(dout, IN, mean, rstd, gamma, dresidual=None, din=None, d
            _at("layer_norm mean", mean, _F32, rows, index), _at("layer_norm rstd", rstd, _F32, rows, index),
            _at("layer_norm gamma", gamma, _F32, cols, index),
            None if dresidual is None else _at("layer_norm dresidual", dresidual, t, n, index))
-    din = torch.empty_like(IN) if din is None else din
-    dgamma = torch.empty(cols, dtype=_F32, device=IN.device) if dgamma is None else dgamma
-    dbeta = torch.empty(cols, dtype=_F32, device=IN.device) if dbeta is None else dbeta
+    din, p = _out("layer_norm din", din, IN, n, index)
+    dgamma, pg = _out("layer_norm dgamma", dgamma, gamma, cols, index)
+    dbeta, pb = _out("layer_norm dbeta", dbeta, gamma, cols, index)
     nbytes = lib().silcu_layer_norm_backward_workspace_bytes(rows, cols, dt)
     buf, ws = _scratch(nbytes, IN.device)
-    _launch(lib().silcu_layer_norm_backward, index, *ops, _at("layer_norm din", din, t, n, index),
-            _at("layer_norm dgamma", dgamma, _F32, cols, index), _at("layer_norm dbeta", dbeta, _F32, cols, index),
-            rows, cols, dt, ws, nbytes)
+    _launch(lib().silcu_layer_norm_backward, index, *ops, p, pg, pb, rows, cols, dt, ws, nbytes)
     return din, dgamma, dbeta
 
 
@@ -596,7 +601,7 @@ def linear_cross_entropy(H, W, targets, reduction="mean", loss=None, lse=None):
     lse = torch.empty(n, dtype=_F32, device=H.device) if lse is None else lse
     a, index = _cross_entropy_args(H, W, targets, lse, reduction)
     each = reduction == "none"
-    loss = torch.empty(n if each else (), dtype=_F32, device=H.device) if loss is None else loss
+    loss = (torch.empty_like(lse) if each else lse.new_empty(())) if loss is None else loss
     a.loss = _at("linear_cross_entropy loss", loss, _F32, n if each else 1, index)
     nbytes = lib().silcu_linear_cross_entropy_workspace_bytes(a, 0)
     buf, ws = _scratch(nbytes, H.device)
@@ -624,6 +629,9 @@ def linear_cross_entropy_backward(H, W, targets, lse, dloss=None, reduction="mea
     return dH if need_dH else None, dW if need_dW else None
 
 
+_data_ptr, _numel, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+
+
 class TensorList:
     """The gradients of a model as grad_norm and clip_grad_norm take them: a
     list of fp32 / bf16 CUDA tensors, laid out once for the C call (and again
@@ -633,15 +641,16 @@ class TensorList:
         self.tensors = list(tensors)
         if not self.tensors:
             raise ValueError("TensorList: no tensors")
-        self._addresses = self._counts = None
+        self._addresses = self._counts = self._dtypes = None
         self._layout()
 
     def _layout(self):
         """Checks the tensors and fills the C arrays, unless nothing moved."""
-        addresses = [t.data_ptr() for t in self.tensors]
-        counts = [t.numel() for t in self.tensors]
-        if addresses == self._addresses and counts == self._counts \
-                and all(t.dtype is d and t.is_contiguous() for t, (d, _) in zip(self.tensors, self.shapes)):
+        ts = self.tensors  # map: half the time of a loop, and small lists are bound by it
+        addresses, counts = list(map(_data_ptr, ts)), list(map(_numel, ts))
+        dtypes = [t.dtype for t in ts]
+        if addresses == self._addresses and counts == self._counts and dtypes == self._dtypes \
+                and all(map(_is_contiguous, ts)):
             return self
         n = len(self.tensors)
         array = (_lib.Tensor * n)()
@@ -652,11 +661,11 @@ class TensorList:
             array[i] = _lib.Tensor(addresses[i], counts[i], k)
         self.array, self.pointers = array, (ct.c_void_p * n)(*addresses)
         self.device, self.index = self.tensors[0].device, index
-        self.shapes = [(t.dtype, c) for t, c in zip(self.tensors, counts)]
+        self.scalar = torch.empty((), dtype=_F32, device=self.device)
         self.spans = sorted((a, a + c * t.element_size())
                             for a, c, t in zip(addresses, counts, self.tensors) if c)
         self.nbytes = lib().silcu_grad_norm_workspace_bytes(self.array, n)
-        self._addresses, self._counts = addresses, counts
+        self._addresses, self._counts, self._dtypes = addresses, counts, dtypes
         self._clips_into = None
         return self
 
@@ -667,7 +676,8 @@ class TensorList:
         """Refuses to clip into `out` (a TensorList, maybe this one) where tensors overlap."""
         if self._clips_into is out.spans:
             return  # these two have been checked
-        if out is not self and (self.shapes != out.shapes or self.index != out.index):
+        if out is not self and (self._counts != out._counts or self._dtypes != out._dtypes
+                                or self.index != out.index):
             raise ValueError("clip_grad_norm: OUT must match the tensors in number, size, dtype and device")
         # an output may be its own input; apart from that all spans are disjoint
         mine, theirs = set(self.spans), set(out.spans)
@@ -687,7 +697,7 @@ def _list(tensors):
 def grad_norm(tensors):
     """2-norm over a list of tensors (or a TensorList) as a 0-d device tensor."""
     tl = _list(tensors)
-    norm = torch.empty((), dtype=_F32, device=tl.device)
+    norm = torch.empty_like(tl.scalar)
     buf, ws = _scratch(tl.nbytes, tl.device)
     _launch(lib().silcu_grad_norm, tl.index, tl.array, len(tl), norm.data_ptr(), ws, tl.nbytes)
     return norm
@@ -701,7 +711,7 @@ def clip_grad_norm(tensors, max_norm, OUT=None, eps=1e-6):
     out = tl if OUT is None else _list(OUT)
     tl._check_clip(out)
     pointers = None if OUT is None else out.pointers
-    norm = torch.empty((), dtype=_F32, device=tl.device)
+    norm = torch.empty_like(tl.scalar)
     buf, ws = _scratch(tl.nbytes, tl.device)
     _launch(lib().silcu_clip_grad_norm, tl.index, tl.array, pointers, len(tl), max_norm, eps, norm.data_ptr(), ws,
             tl.nbytes)
