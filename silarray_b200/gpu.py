@@ -575,6 +575,14 @@ def _matrix(what, t, rows, cols, dtype, index):
     return t.data_ptr(), ld
 
 
+def _gradient(what, t, like, index):
+    """The gradient of a checked matrix, t or a new one, its address and row stride."""
+    if t is None:
+        t = torch.empty_like(like, memory_format=torch.contiguous_format)
+        return t, t.data_ptr(), t.shape[1]
+    return t, *_matrix(what, t, *like.shape, like.dtype, index)
+
+
 def _cross_entropy_args(H, W, targets, lse, reduction):
     if reduction not in REDUCTION:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
@@ -618,11 +626,9 @@ def linear_cross_entropy_backward(H, W, targets, lse, dloss=None, reduction="mea
     if dloss is not None:
         a.dloss = _at("linear_cross_entropy dloss", dloss, _F32, H.shape[0] if reduction == "none" else 1, index)
     if need_dH:
-        dH = torch.empty(H.shape, dtype=H.dtype, device=H.device) if dH is None else dH
-        a.dH, a.lddh = _matrix("linear_cross_entropy dH", dH, *H.shape, H.dtype, index)
+        dH, a.dH, a.lddh = _gradient("linear_cross_entropy dH", dH, H, index)
     if need_dW:
-        dW = torch.empty(W.shape, dtype=W.dtype, device=W.device) if dW is None else dW
-        a.dW, a.lddw = _matrix("linear_cross_entropy dW", dW, *W.shape, W.dtype, index)
+        dW, a.dW, a.lddw = _gradient("linear_cross_entropy dW", dW, W, index)
     nbytes = lib().silcu_linear_cross_entropy_workspace_bytes(a, 1)
     buf, ws = _scratch(nbytes, H.device)
     _launch(lib().silcu_linear_cross_entropy_backward, index, a, ws, nbytes)
