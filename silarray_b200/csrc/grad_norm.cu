@@ -186,6 +186,7 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) sum_squares(const __grid_constant__ ListArgs<CAP> a) {
   __shared__ double sm[kWarps];
   let_next_start();
+  wait_for_previous();
   double acc = 0.0;
   for_span(a, uint64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5), [&](int t, uint64_t first, uint64_t n) {
     if (a.dtype[t] == SILCU_BF16) {
@@ -223,6 +224,7 @@ __device__ __forceinline__ double total_norm(const double *part, int nparts) {
 }
 
 __global__ void __launch_bounds__(kThreads) norm_finish(const double *part, int nparts, float *norm) {
+  let_next_start();
   wait_for_previous();
   const double n = total_norm(part, nparts);
   if (threadIdx.x == 0) *norm = float(n);
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(kThreads) norm_finish(const double *part, int 
 
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) clip_scale(const __grid_constant__ ListArgs<CAP> a) {
+  let_next_start();
   wait_for_previous();
   const double norm = total_norm(a.all, a.nparts);
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm) *a.norm = float(norm);
@@ -329,7 +332,7 @@ void launch_sum(const silcu_tensor *t, const Piece &p, double *part, cudaStream_
   ListArgs<CAP> a = {};
   fill(a, t, nullptr, p);
   a.part = part + p.part0;
-  sum_squares<CAP><<<p.grid, kThreads, 0, s>>>(a);
+  launch_after(sum_squares<CAP>, p.grid, kThreads, 0, s, a);
 }
 
 template <int CAP>

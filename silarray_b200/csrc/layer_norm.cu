@@ -22,6 +22,9 @@
 //                      row, and read from global memory with a 32-byte lane
 //                      stride they keep the L1 77 % busy: 4096 x 8192 39.2 us
 //                      with ln_forward, 31.4 persistent, 28.5 with shared memory.
+//                      Started early behind its predecessor (launch_after) 24.9, 26.8
+//                      without; for ln_forward's many CTAs the waits cost more than
+//                      that gives (16384 x 768 19.4 us, 16.5 without).
 //   ln_backward        persistent, prefetching; each thread adds its columns'
 //                      dgamma / dbeta terms in registers over all rows of its CTA,
 //                      one partial row per CTA, added in CTA order by ln_finish.
@@ -153,6 +156,8 @@ __global__ void __launch_bounds__(NT, MIN_CTAS) ln_forward_stream(const LnArgs a
   __shared__ float sm[2][2][NW];
   const float4 *gs = ps, *bs = ps + VPT * NT * VEC / 4;
   const uint32_t t = threadIdx.x;
+  let_next_start();
+  wait_for_previous();
   params_to_smem<VEC, VPT, NT>(ps, a.gamma, a.cols, t);  // each thread reads back what it wrote
   params_to_smem<VEC, VPT, NT>(ps + VPT * NT * VEC / 4, a.beta, a.cols, t);
   const float inv_n = 1.0f / float(a.cols);
@@ -303,6 +308,8 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
     if constexpr (Cfg::PARAMS) params_from_smem<VEC, VPT, NT>(gs, j, t, f);
     else load_f32<VEC>(a.gamma + (t + j * NT) * VEC, f);
   };
+  let_next_start();
+  wait_for_previous();
   if constexpr (Cfg::PARAMS) params_to_smem<VEC, VPT, NT>(reinterpret_cast<float4 *>(dyn), a.gamma, a.cols, t);
   float ag[ACCREG ? E : 1], ab[ACCREG ? E : 1];
   if (ACCREG) {
@@ -312,7 +319,6 @@ __global__ void __launch_bounds__(NT *GROUPS) ln_backward(const LnArgs a) {
     for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NT * GROUPS) acc_s[c] = 0.f;
     __syncthreads();
   }
-  let_next_start();
   const float inv_n = 1.0f / float(a.cols);
   const uint64_t step = uint64_t(gridDim.x) * GROUPS;
   int buf = 0;
@@ -494,26 +500,34 @@ __global__ void __launch_bounds__(512) ln_backward_long(const LnArgs a) {
   }
 }
 
-// dgamma / dbeta: the partial rows added in CTA order, in 32 interleaved
-// slices per column (one warp each) that then add in slice order.
+// dgamma / dbeta: the partial rows added in an order that only their number
+// decides.  COLS columns a CTA, 1024 / COLS threads for the rows of each.  Few columns
+// spread over more SMs with 8 of them (768 columns, 888 partial rows: 4.7 us with 32).
+template <int COLS>
 __global__ void __launch_bounds__(1024) ln_finish(const float *__restrict__ part, uint32_t nparts, uint32_t cols,
                                                   float *__restrict__ dgamma, float *__restrict__ dbeta) {
+  constexpr uint32_t SLICES = 1024 / COLS;
   __shared__ float sm[32][33];
-  const uint32_t lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const uint32_t c = blockIdx.x * 32 + lane;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t c = blockIdx.x * COLS + threadIdx.x % COLS;
   float s = 0.f;
+  let_next_start();
   wait_for_previous();
   if (c < 2 * cols) {
 #pragma unroll 8
-    for (uint32_t i = slice; i < nparts; i += 32) s += __ldcs(part + uint64_t(i) * 2 * cols + c);
+    for (uint32_t i = threadIdx.x / COLS; i < nparts; i += SLICES) s += __ldcs(part + uint64_t(i) * 2 * cols + c);
   }
-  sm[slice][lane] = s;
-  __syncthreads();
-  if (slice == 0 && c < 2 * cols) {
 #pragma unroll
-    for (int i = 1; i < 32; i++) s += sm[i][lane];
-    if (c < cols) dgamma[c] = s;
-    else dbeta[c - cols] = s;
+  for (int step = COLS; step < 32; step *= 2) s += __shfl_xor_sync(0xffffffffu, s, step);
+  if (lane < COLS) sm[warp][lane] = s;
+  __syncthreads();
+  if (warp < COLS) {  // the warps' sums of column `warp`
+    s = warp_sum(sm[lane][warp]);
+    const uint32_t col = blockIdx.x * COLS + warp;
+    if (lane == 0 && col < 2 * cols) {
+      if (col < cols) dgamma[col] = s;
+      else dbeta[col - cols] = s;
+    }
   }
 }
 
@@ -583,7 +597,7 @@ struct Forward {
         allow_smem(ln_forward_stream<T, 8, VPT, NT, CTAS>, smem, configured, "layer_norm_forward");
     if (st != SILCU_OK) return st;
     const uint64_t cap = uint64_t(sm_count()) * CTAS;
-    ln_forward_stream<T, 8, VPT, NT, CTAS><<<uint32_t(a.rows < cap ? a.rows : cap), NT, smem, s>>>(a);
+    launch_after(ln_forward_stream<T, 8, VPT, NT, CTAS>, uint32_t(a.rows < cap ? a.rows : cap), NT, smem, s, a);
     return check_launch("layer_norm_forward");
   }
 };
@@ -621,7 +635,7 @@ struct Backward {
     const silcu_status st = allow_smem(kernel, Cfg::smem(Cfg::E * NT), configured, "layer_norm_backward");
     if (st != SILCU_OK) return st;
     *grid = BackwardGrid{a.rows}.run<VEC, VPT, NT, GROUPS>();
-    kernel<<<*grid, NT * GROUPS, Cfg::smem(a.cols), s>>>(a);
+    launch_after(kernel, *grid, NT * GROUPS, Cfg::smem(a.cols), s, a);
     return check_launch("layer_norm_backward");
   }
 };
@@ -776,8 +790,9 @@ silcu_status silcu_layer_norm_backward(const void *dout, const void *in, const f
       st = dresidual ? backward<float, true>(a, s, &grid) : backward<float, false>(a, s, &grid);
     if (st != SILCU_OK) return st;
   }
-  launch_after(ln_finish, uint32_t((2 * cols + 31) / 32), 1024, 0, s, static_cast<const float *>(workspace), grid,
-               uint32_t(cols), dgamma, dbeta);
+  const bool few = 2 * cols <= 8 * 2 * size_t(sm_count());  // 8 columns a CTA, two CTAs an SM
+  launch_after(few ? ln_finish<8> : ln_finish<32>, uint32_t((2 * cols + (few ? 7 : 31)) / (few ? 8 : 32)), 1024, 0, s,
+               static_cast<const float *>(workspace), grid, uint32_t(cols), dgamma, dbeta);
   return check_launch("layer_norm_backward finish");
 }
 
