@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ p
                                                     float *loss, int mean, unsigned *done, float *__restrict__ total) {
   __shared__ float2 sm[32][kFinishRows];
   __shared__ double sums[32];
+  __shared__ int counts[32];
   __shared__ bool last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row0 = int64_t(blockIdx.x) * kFinishRows, row = row0 + (lane & 7);
@@ -126,14 +127,23 @@ __global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ p
   __syncthreads();
   if (!last) return;
   double s = 0.0;
+  int n = 0;
 #pragma unroll 4
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) s += double(__ldcg(loss + i));
-  s = cta_sum(s, sums);
-  if (mean) {
-    const double n = count_rows(targets, rows, V, sums);
-    s = n > 0.0 ? s / n : 0.0;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    const int t = targets[i];
+    s += double(__ldcg(loss + i));
+    n += t >= 0 && t < V;
   }
-  if (threadIdx.x == 0) *total = float(s);
+  s = warp_sum(s);
+  n = warp_sum(n);
+  if (lane == 0) sums[warp] = s, counts[warp] = n;
+  __syncthreads();
+  if (warp == 0) {
+    s = warp_sum(sums[lane]);
+    n = warp_sum(counts[lane]);
+    if (mean) s = n > 0 ? s / double(n) : 0.0;
+    if (lane == 0) *total = float(s);
+  }
 }
 
 // The gradient of every row's loss.
@@ -485,8 +495,8 @@ struct Backward {
     lds = ds.dp;
     dh.M = a.rows, dh.N = a.D, dh.K = piece, dh.wanted = a.dH;
     dw.M = piece, dw.N = a.D, dw.K = a.rows, dw.wanted = a.dW;
-    if (score.raw) dh.tile = dw.tile = lossmm::BM;
     dh.transposed = a.rows <= lossmm::BM;
+    if (score.raw) dh.tile = lossmm::BM;  // and transposed, having few rows
     if (dh.transposed) {  // a launch of its own
       Gradient none = {};
       none.K = 1, none.wanted = false;
@@ -528,13 +538,6 @@ silcu_status scores(lossmm::Params &p, const ScoreTiles &t, cudaStream_t s) {
   if constexpr (Ty::PARTS == 2)
     if (t.raw) return lossmm::launch<Ty, EPI, false, true>(p, 1, s);
   return t.pair ? lossmm::launch<Ty, EPI, true>(p, 1, s) : lossmm::launch<Ty, EPI, false>(p, 1, s);
-}
-
-template <typename Ty, int EPI>
-silcu_status products(lossmm::Params &p, bool pairs, int count, cudaStream_t s) {
-  if constexpr (Ty::PARTS == 2)
-    if (!pairs) return lossmm::launch<Ty, EPI, false, true>(p, count, s);
-  return lossmm::launch<Ty, EPI, true>(p, count, s);
 }
 
 template <typename T>
@@ -649,32 +652,36 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
       p.bn = bn;
       p.rows_a = lossmm::BM;
       p.alpha = alpha;
-      if (!pairs) set_raw(p);
     };
     if (b.dh.wanted && b.dh.transposed) {
       clear(int(up(a.rows, 32)));
+      if (!pairs) set_raw(p);
       if (!lossmm::set_problem<Ty>(p.p[0], pairs, p.bn, lossmm::BM, a.D, a.rows, n, w, b.ds.operand(false))) return map_error();
       set_output(p.p[0], b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
-      if ((st = products<Ty, lossmm::kOutT>(p, pairs, 1, s)) != SILCU_OK) return st;
+      if constexpr (Ty::PARTS == 2)
+        st = pairs ? lossmm::launch<Ty, lossmm::kOutT, true>(p, 1, s) : lossmm::launch<Ty, lossmm::kOutT, false, true>(p, 1, s);
+      else
+        st = lossmm::launch<Ty, lossmm::kOutT, true>(p, 1, s);
+      if (st != SILCU_OK) return st;
     }
     // Both products of ds in one launch, the one with the longer items first.
-    clear(pairs ? lossmm::BN : lossmm::BM);
+    clear(lossmm::BN);
     int count = 0;
     const bool dw_first = b.dw.K / b.dw.split > b.dh.K / b.dh.split;
     for (const bool is_dw : {dw_first, !dw_first}) {
       if (is_dw ? !b.dw.wanted : !b.dh.wanted || b.dh.transposed) continue;
       lossmm::Problem &q = p.p[count++];
       if (is_dw) {
-        if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
+        if (!lossmm::set_problem<Ty>(q, true, p.bn, lossmm::BM, n, a.D, a.rows, b.ds.operand(true), b.h.operand(true)))
           return map_error();
         set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, a.D,
                    ceil_div(a.rows, BK));
       } else {
-        if (!lossmm::set_problem<Ty>(q, pairs, p.bn, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
+        if (!lossmm::set_problem<Ty>(q, true, p.bn, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
         set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
       }
     }
-    if (count && (st = products<Ty, lossmm::kOut>(p, pairs, count, s)) != SILCU_OK) return st;
+    if (count && (st = lossmm::launch<Ty, lossmm::kOut, true>(p, count, s)) != SILCU_OK) return st;
     if (b.dw.wanted && !b.dw.direct) {
       st = finish_planes<Ty>(b.dw, n, a.D, alpha, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, s);
       if (st != SILCU_OK) return st;
