@@ -114,7 +114,7 @@ struct Tf32 {
 template <typename Ty, int EPI, bool PAIR, bool RAW = false>
 struct Cfg {
   static_assert(!RAW || (Ty::PARTS == 2 && !PAIR), "raw operands: tf32 on single CTAs");
-  static_assert(RAW || PAIR || (EPI != kOut && EPI != kOutT), "only the scores run on single CTAs otherwise");
+  static_assert(PAIR || EPI == kStats || EPI == kScoreGrad || (EPI == kOutT && RAW), "single CTAs");
   static constexpr int TM = PAIR ? 2 * BM : BM;
   static constexpr int ROWS_B = PAIR ? BN / 2 : BN;  // B columns held per CTA
   static constexpr int SUBS = PAIR && Ty::PARTS == 1 ? 2 : 1;  // 128-byte-row tiles of each operand per stage
@@ -164,7 +164,6 @@ struct Problem {
   Divisor by_split, by_group, by_last;
   int ksplit;              // each tile's K range in this many parts (kOut; part i -> plane i)
   int amn;                 // kOut: A is stored with the M index contiguous (kOutT: it always is)
-  int raw;                 // RAW kernels: B (kOutT: A) is plain fp32, split in shared memory
   int mode, vec;           // vec: kDirect rows are 16-byte aligned
   void *out;
   int64_t ldo, plane;      // row stride; elements from one plane to the next
@@ -238,11 +237,13 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
 // (W^T ds^T)^T.  W, with the M index contiguous, then fills the tile's 128 or 256 rows
 // and ds its few columns, and an MMA takes the time of the columns that exist.  As
 // ds . W the few rows were padded to a whole tile: 30 rows of 60000 x 3000
-// took 185 us of the tensor pipe's time in bf16 and 580 in fp32.
+// took 185 us in bf16 and 580 in fp32; so they take 56 (6.4 TB/s) and 280.
 //
 // RAW: one operand may be plain fp32.  Its tile is the hi operand as it stands (the
 // tensor core reads the upper 19 bits of a value), and the epilogue warps, idle
-// while the MMAs run, write the remainders beside it.  For few rows, where the
+// while the MMAs run, write the remainders beside it.  Two buffers for those and more
+// stages in their place gave nothing, nor did halves of the warps that take turns: twelve
+// MMAs per 32 k that each read 128 rows of A are what a stage costs.  For few rows, where the
 // time is that of reading W, this spares writing and reading a split copy.
 // Stages are as large as the tile needs.
 template <typename Ty, int EPI, bool PAIR, bool RAW>
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           }
           // a pair's bytes all complete on the even CTA's barrier
           const uint32_t bar = PAIR ? mapa_shared(full0 + 8 * s, 0) : full0 + 8 * s;
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, RAW && q.raw ? bytes - (RAW_A ? TILE_A : TILE_B) : bytes);
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, RAW ? bytes - (RAW_A ? TILE_A : TILE_B) : bytes);
           auto load = [&](uint32_t dst, const CUtensorMap *map, int c0, int c1) {
             if (PAIR) tma_load_2d_pair(dst, map, bar, c0, c1);
             else tma_load_2d(dst, map, bar, c0, c1);
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
             uint32_t dst = smem_u32(smem + s * STAGE_BYTES + u * SUB_BYTES);
 #pragma unroll
             for (int h = 0; h < PARTS; h++, dst += TILE_A) {
-              if (RAW && RAW_A && q.raw && h == 1) continue;
+              if (RAW && RAW_A && h == 1) continue;
               if (amn) {
 #pragma unroll
                 for (int i = 0; i < C::MN_BOXES_A; i++) load(dst + i * C::MN_BOX, &q.a[h], am + Ty::KROW * i, kc);
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
             }
 #pragma unroll
             for (int h = 0; h < PARTS; h++, dst += TILE_B) {
-              if (RAW && !RAW_A && q.raw && h == 1) break;
+              if (RAW && !RAW_A && h == 1) break;
               if (BMN) {
 #pragma unroll
                 for (int i = 0; i < boxes_b; i++) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {  // the pair's MMAs are issued by the even CTA
-      uint32_t kbg = 0, cg = 0, raw_uses = 0;  // raw_uses: parity of each slot's raw uses so far
+      uint32_t kbg = 0, cg = 0;
       bool ok = true;
       const uint32_t base = smem_u32(smem);
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
@@ -378,12 +379,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           for (int kb = c0; kb < c1; kb++, kbg++) {
             const uint32_t s = kbg % STAGES, ph = (kbg / STAGES) & 1;
             if ((!mbar_try_wait(full0 + 8 * s, ph) && !mbar_wait(full0 + 8 * s, ph, p.err, 22)) ||
-                (RAW && q.raw && !mbar_try_wait(ready0 + 8 * s, (raw_uses >> s) & 1) &&
-                 !mbar_wait(ready0 + 8 * s, (raw_uses >> s) & 1, p.err, 26))) {
+                (RAW && !mbar_try_wait(ready0 + 8 * s, ph) && !mbar_wait(ready0 + 8 * s, ph, p.err, 26))) {
               ok = false;
               break;
             }
-            if (RAW && q.raw) raw_uses ^= 1u << s;
             tc_fence_after();
 #pragma unroll
             for (int u = 0; u < SUBS; u++) {
@@ -433,13 +432,9 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       // this warp's columns of the tile (may be <= 0)
       const int cols = min(min(q.N, tl.n0 + bn), c0 + half) - c0;
       // RAW: the next `n` stages' remainders x - tf32(x) of the raw operand, for the MMAs.
-      // Every warp sees every raw use of a slot, so no barrier is ever more than
-      // one phase ahead of it.
+      // Every warp sees every use of a slot, so no barrier is ever more than one phase ahead
+      // of it.
       auto remainders = [&](int n) {
-        if (!q.raw) {
-          kbe += n;
-          return true;
-        }
         for (int i = 0; i < n; i++, kbe++) {
           const uint32_t s = kbe % STAGES;
           if (!__all_sync(0xffffffffu, wait_inline(full0 + 8 * s, (kbe / STAGES) & 1, p.err, 25))) return false;
@@ -768,7 +763,6 @@ bool set_problem(Problem &q, bool pair, int bn, int rows_a, int64_t M, int64_t N
   q.tiles_n = int((N + bn - 1) / bn);
   q.ksplit = 1;
   q.amn = a.mn;
-  q.raw = Ty::PARTS == 2 && (!a.lo || !b.lo);
   return operand_map<Ty>(q.a, a, M, K, rows_a) && operand_map<Ty>(q.b, b, N, K, pair ? bn / 2 : bn);
 }
 
