@@ -522,6 +522,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           if (ok && cols > 0) {
 #pragma unroll
             for (int cb = 0; cb < 4; cb++) {
+              if (32 * cb >= cols) break;  // the other warp's columns may still hold its last chunk
               uint32_t r[32];
 #pragma unroll
               for (int i = 0; i < 32; i++) r[i] = __float_as_uint(acc[32 * cb + i]);
