@@ -219,35 +219,46 @@ __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int6
   }
 }
 
-// out [rows, D] = alpha times the sum of the fp32 planes [rows, ldp], in plane order.
-template <typename T>
+// out [rows, D] = alpha times the sum of the fp32 planes [rows, ldp], in plane order, or
+// for few elements of many planes by WAYS neighbouring lanes that take turns at the planes
+// (16 planes of 100 x 1024: 9 us by one thread).
+template <typename T, int WAYS>
 __global__ void __launch_bounds__(256) planes_finish(const float *__restrict__ planes, int nplanes, int64_t plane,
                                                      int64_t rows, int D, int ldp, const float *__restrict__ alpha,
                                                      T *__restrict__ out, int64_t ldo, int vec) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = (D + W - 1) / W;
   const int64_t n = rows * per_row;
+  const int way = threadIdx.x % WAYS;
   let_next_start();
   wait_for_previous();
   const float k0 = alpha ? *alpha : 1.0f;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-    const int64_t r = i / per_row;
+  for (int64_t i0 = int64_t(blockIdx.x) * (256 / WAYS); i0 < n; i0 += int64_t(gridDim.x) * (256 / WAYS)) {
+    const int64_t i = i0 + threadIdx.x / WAYS, r = i / per_row;
     const int c = int(i - r * per_row) * W;
     float f[W] = {};
-    const float *src = planes + r * ldp + c;  // ldp is a multiple of W: the last vectors stay inside the row
-    constexpr int AHEAD = 32 / W;             // planes on their way at a time
-    for (int p = 0; p < nplanes; p += AHEAD) {
-      float v[AHEAD][W];
+    if (i < n) {
+      const float *src = planes + r * ldp + c;  // ldp is a multiple of W: the last vectors stay inside the row
+      constexpr int AHEAD = 32 / W;             // planes on their way at a time
+      for (int p = way; p < nplanes; p += AHEAD * WAYS) {
+        float v[AHEAD][W];
 #pragma unroll
-      for (int j = 0; j < AHEAD; j++)
-        if (p + j < nplanes) load_f32<W>(src + (p + j) * plane, v[j]);
+        for (int j = 0; j < AHEAD; j++)
+          if (p + j * WAYS < nplanes) load_f32<W>(src + (p + j * WAYS) * plane, v[j]);
 #pragma unroll
-      for (int j = 0; j < AHEAD; j++)
-        if (p + j < nplanes) {
+        for (int j = 0; j < AHEAD; j++)
+          if (p + j * WAYS < nplanes) {
 #pragma unroll
-          for (int k = 0; k < W; k++) f[k] += v[j][k];
-        }
+            for (int k = 0; k < W; k++) f[k] += v[j][k];
+          }
+      }
     }
+#pragma unroll
+    for (int step = 1; step < WAYS; step *= 2) {
+#pragma unroll
+      for (int k = 0; k < W; k++) f[k] += __shfl_xor_sync(0xffffffffu, f[k], step);
+    }
+    if (i >= n || way) continue;
 #pragma unroll
     for (int k = 0; k < W; k++) f[k] *= k0;
     T *dst = out + r * ldo + c;
@@ -415,8 +426,9 @@ struct Gradient {
   bool wanted, direct;
   bool transposed = false;    // computed as its transpose (kOutT): the N x M tiles hold all of M
   float *planes = nullptr;
-  int tile = 2 * lossmm::BM;  // rows and columns of a tile (CTA pairs: 256; single CTAs: 128)
-  int64_t tiles() const { return (transposed ? 1 : ceil_div(M, tile)) * ceil_div(N, tile); }
+  int tile = 2 * lossmm::BM;  // rows of a tile (CTA pairs: 256; single CTAs: 128)
+  int bn = lossmm::BN;        // and its columns
+  int64_t tiles() const { return transposed ? ceil_div(N, tile) : ceil_div(M, tile) * ceil_div(N, bn); }
   int64_t units() const { return tile == lossmm::BM ? sm_count() : sm_count() / 2; }
 };
 
@@ -432,7 +444,7 @@ double out_time(const Gradient &first, const Gradient &second, bool tf32) {
   if (n0 + n1 == 0) return 0.0;
   const int64_t u = n0 + n1 < units ? n0 + n1 : units, tail = n0 % u, low = u - tail;
   const double epilogue = tf32 ? 128.0 : 512.0;
-  const double ns = (tf32 ? 42.0 : 7.0) * (first.tile == lossmm::BM ? 0.5 : 1.0);
+  const double ns = (tf32 ? 42.0 : 7.0) * (first.tile == lossmm::BM ? 0.5 : first.bn / 256.0);
   const double c0 = double(first.K) / first.split, c1 = double(second.K) / second.split;
   const int64_t extra = n1 && tail ? int64_t(c0 / c1 + 0.5) : 0;
   auto rounds = [&](int64_t begin, int64_t step) { return begin < n1 ? ceil_div(n1 - begin, step) : 0; };
@@ -450,17 +462,27 @@ double out_time(const Gradient &first, const Gradient &second, bool tf32) {
   return time * ns + bytes / 6500.0;
 }
 
+// Columns of the products' tiles, whose N is D: the width that wastes the fewest
+// columns of D (16 more stand for a tile's fixed share).  Each CTA of a pair loads half
+// of them in boxes of 32 fp32 or 64 bf16 columns.
+int columns_of_tile(int64_t D, bool tf32) {
+  int best = lossmm::BN;
+  for (int bn = lossmm::BN; bn >= 64; bn -= tf32 ? 64 : 128)
+    if (ceil_div(D, bn) * (bn + 16) < ceil_div(D, best) * (best + 16)) best = bn;
+  return best;
+}
+
 // Cuts the products' K so that the launch ends evenly: long sums of few tiles
 // (few rows, or a short vocabulary) and the last round of many.  At least 512 k
-// a part.
+// a part, and 32 parts at most but for the few tiles of a transposed product.
 void choose_splits(Gradient &dh, Gradient &dw, bool tf32) {
-  static const int counts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
+  static const int counts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64};
   double best = -1.0;
   int bh = 1, bw = 1;
   for (const int h : counts) {
-    if (h > 1 && (!dh.wanted || dh.K < 512 * int64_t(h))) break;
+    if (h > 1 && (!dh.wanted || dh.K < 512 * int64_t(h) || (h > 32 && !dh.transposed))) break;
     for (const int w : counts) {
-      if (w > 1 && (!dw.wanted || dw.K < 512 * int64_t(w))) break;
+      if (w > 1 && (!dw.wanted || dw.K < 512 * int64_t(w) || w > 32)) break;
       dh.split = h;
       dw.split = w;
       const bool dw_first = dw.K / w > dh.K / h;
@@ -495,6 +517,7 @@ struct Backward {
     lds = ds.dp;
     dh.M = a.rows, dh.N = a.D, dh.K = piece, dh.wanted = a.dH;
     dw.M = piece, dw.N = a.D, dw.K = a.rows, dw.wanted = a.dW;
+    dh.bn = dw.bn = columns_of_tile(a.D, Ty::PARTS == 2);
     dh.transposed = a.rows <= lossmm::BM;
     if (score.raw) dh.tile = lossmm::BM;  // and transposed, having few rows
     if (dh.transposed) {  // a launch of its own
@@ -606,8 +629,10 @@ silcu_status finish_planes(const Gradient &g, int64_t rows, int64_t D, const flo
                            int vec, cudaStream_t s) {
   using T = typename Ty::T;
   const int64_t ldp = up(D, 8);
-  launch_after(planes_finish<T>, stream_grid(rows * ceil_div(D * int64_t(sizeof(T)), 16)), 256, 0, s, g.planes, g.split,
-               g.M * ldp, rows, int(D), int(ldp), alpha, static_cast<T *>(out), ldo, vec);
+  const int64_t vectors = rows * ceil_div(D * int64_t(sizeof(T)), 16);
+  const bool few = g.split >= 8 && vectors * 8 <= int64_t(sm_count()) * 2048;  // eight lanes each fill the SMs at most once
+  launch_after(few ? planes_finish<T, 8> : planes_finish<T, 1>, stream_grid(vectors * (few ? 8 : 1)), 256, 0, s, g.planes,
+               g.split, g.M * ldp, rows, int(D), int(ldp), alpha, static_cast<T *>(out), ldo, vec);
   return check_launch("cross_entropy planes");
 }
 
@@ -665,7 +690,8 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
       if (st != SILCU_OK) return st;
     }
     // Both products of ds in one launch, the one with the longer items first.
-    clear(lossmm::BN);
+    clear(b.dw.bn);
+    p.half = int(up(p.bn / 2, 32));
     int count = 0;
     const bool dw_first = b.dw.K / b.dw.split > b.dh.K / b.dh.split;
     for (const bool is_dw : {dw_first, !dw_first}) {

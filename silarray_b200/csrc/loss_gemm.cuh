@@ -173,9 +173,9 @@ struct __align__(64) Params {
   Problem p[2];  // kOut: up to two products in one launch
   void *ds[2];       // score gradients [part]: [M, lds], lds a multiple of 64
   int64_t lds;
-  int bn;            // tile columns (of the scores and kOut on CTA pairs: BN)
+  int bn;            // tile columns (of the scores on CTA pairs: BN)
   int rows_a;        // rows of A's boxes (single CTAs; the rest of a tile is never stored)
-  int half;          // columns of an epilogue warp (RAW; else 128)
+  int half;          // columns of an epilogue warp (RAW and kOut; else 128)
   int stages;        // ring stages (RAW)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, rounds, tail, extra;  // rounds = n0 / units, tail = n0 % units
@@ -220,7 +220,7 @@ __device__ __forceinline__ Tile tile_of(const Problem &q, int bn, int item) {
   const int r = t - group * C::GROUP_M * q.tiles_n;
   const int nk = (q.K + C::BK - 1) / C::BK;
   const int col = gm == C::GROUP_M ? r / C::GROUP_M : q.by_last(r), row = first + r - col * gm;
-  // at most 32 parts of 2^24 k: the products stay below 2^31
+  // at most 64 parts of 2^24 k, 32 or more to a block: the products stay below 2^31
   return Tile{row * C::TM, col * bn, q.by_split(part * nk), q.by_split((part + 1) * nk), part};
 }
 
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = PAIR ? int(blockIdx.x >> 1) : int(blockIdx.x);
-  const int bn = PAIR && EPI != kOutT ? BN : p.bn;
+  const int bn = PAIR && (EPI == kStats || EPI == kScoreGrad) ? BN : p.bn;
 
   let_next_start();
   if (threadIdx.x == 0) {
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       bool ok = true;
       const uint32_t bytes =
           SUBS * PARTS * ((PAIR ? TILE_A : p.rows_a * 128) * (PAIR ? 2 : 1) + bn * 128);  // a pair's, on the even CTA
-      const int boxes_b = RAW ? bn / Ty::KROW : C::MN_BOXES_B;
+      const int boxes_b = (PAIR ? bn / 2 : bn) / Ty::KROW;
       for (int k = 0; ok && work_at(p, unit, k, w); k++) {
         const Problem &q = p.p[w.prob];
         const Tile tl = tile_of<C>(q, bn, w.item);
@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
               if (RAW && !RAW_A && h == 1) break;
               if (BMN) {
 #pragma unroll
-                for (int i = 0; i < boxes_b; i++) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
+                for (int i = 0; i < C::MN_BOXES_B; i++)
+                  if (i < boxes_b) load(dst + i * C::MN_BOX, &q.b[h], nb + Ty::KROW * i, kc);
               } else {
                 load(dst, &q.b[h], kc, nb);
               }
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
   } else {
     const int qr = warp & 3, h = (warp - 2) >> 2;
     float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
-    const int half = RAW ? p.half : 128;
+    const int half = RAW || EPI == kOut ? p.half : 128;
     const float alpha = (EPI == kOut || EPI == kOutT) && p.alpha ? *p.alpha : 1.0f;
     uint32_t cg = 0, kbe = 0;
     bool ok = true;
