@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
 // stride in elements.  Pointers and row strides are multiples of 16 bytes.
 struct Operand {
   const void *p, *lo;  // lo: the tf32 pair's (null for bf16 and raw fp32)
-  int64_t ld;
+  int64_t ld, ldlo;
   bool mn;
 };
 
@@ -747,8 +747,9 @@ template <typename Ty>
 bool operand_map(CUtensorMap (&m)[2], const Operand &o, int64_t extent, int64_t K, int rows) {
   for (int h = 0; h < (o.lo ? 2 : 1); h++) {
     const void *p = h ? o.lo : o.p;
-    const bool ok = o.mn ? make_map2<typename Ty::T>(&m[h], p, extent, K, o.ld, Ty::KROW, Ty::KROW, Ty::PARTS == 2)
-                         : make_map2<typename Ty::T>(&m[h], p, K, extent, o.ld, Ty::KROW, rows, false);
+    const int64_t ld = h ? o.ldlo : o.ld;
+    const bool ok = o.mn ? make_map2<typename Ty::T>(&m[h], p, extent, K, ld, Ty::KROW, Ty::KROW, Ty::PARTS == 2)
+                         : make_map2<typename Ty::T>(&m[h], p, K, extent, ld, Ty::KROW, rows, false);
     if (!ok) return false;
   }
   return true;
