@@ -291,7 +291,7 @@ using lossmm::Tf32;
 
 // Of a piece's ds (and of its copied weights).
 // Larger pieces add to dH's planes less often, smaller ones stay nearer to the
-// L2's size: 8192 rows of bf16 (131072 columns, D 2048) 13.4 ms at 256 MB, 13.0 at
+// L2's size (when chosen): 8192 rows of bf16 (131072 columns, D 2048) 13.4 ms at 256 MB, 13.0 at
 // 128, 13.7 at 64; 16384 fp32 rows (32768 columns, D 768) 15.6 ms at 512 MB, 16.4 at 256.
 constexpr int64_t kPieceBytes[2] = {int64_t(512) << 20, int64_t(128) << 20};  // by silcu_dtype
 
