@@ -359,7 +359,9 @@ silcu_status silcu_sgemv(const float *x, const float *W, float *y, const float *
 /* ------------------------------------------------------------ training ops
  * No counterpart in the reference, whose backward pass has gpu::sigmoid_backward
  * only: the gradient of layer_norm, the loss of a vocabulary projection with its
- * gradients, and the norm of a list of gradients. */
+ * gradients, and the norm of a list of gradients.  A workspace belongs to one call until
+ * that has ended on the GPU: calls on two streams, or graphs replayed at the same
+ * time, take one each. */
 typedef enum silcu_dtype { SILCU_F32 = 0, SILCU_BF16 = 1 } silcu_dtype;
 
 /* layer_norm of a contiguous [rows, cols] matrix of `dtype` that also keeps
