@@ -298,15 +298,21 @@ constexpr int64_t kPieceBytes[2] = {int64_t(512) << 20, int64_t(128) << 20};  //
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 
+// Columns per piece at most, from SILCU_LOSS_PIECE (tests, tuning).  An entry point reads
+// it once and plans once: the plan whose size it checks is the one it runs.
+int64_t piece_limit() {
+  const char *e = getenv("SILCU_LOSS_PIECE");
+  if (!e) return INT64_MAX;
+  const int64_t want = atoll(e);
+  return up(want < 1 ? 1 : want < (1 << 24) ? want : 1 << 24, 256);
+}
+
 // Vocabulary columns per piece: a multiple of 256 whose `bytes` per column
 // stay within the limit, and pieces of about equal size.
-int64_t piece_of(int64_t V, int64_t bytes, int dtype) {
+int64_t piece_of(int64_t V, int64_t bytes, int dtype, int64_t limit) {
   int64_t p = kPieceBytes[dtype] / bytes / 256 * 256;
   if (p < 256) p = 256;
-  if (const char *e = getenv("SILCU_LOSS_PIECE")) {  // columns per piece at most (tests, tuning)
-    const int64_t want = up(atoll(e) > 0 ? atoll(e) : 256, 256);
-    if (want < p) p = want;
-  }
+  if (limit < p) p = limit;
   if (p >= V) return V;
   return up(ceil_div(V, ceil_div(V, p)), 256);
 }
@@ -407,10 +413,10 @@ struct Forward {
   float *target_score, *row_loss;
   unsigned *done;  // CTAs of loss_finish so far
 
-  Forward(const Args &a, Space &sp) {
+  Forward(const Args &a, Space &sp, int64_t limit) {
     copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
     copy_w = Ty::PARTS == 2 ? !raw_w<Ty>(a) : !rows16(a.W, a.ldw, a.dtype);
-    piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype) : a.V;
+    piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype, limit) : a.V;
     tiles = score_tiles(a.rows, piece, raw_w<Ty>(a));
     nparts = 0;
     for (int64_t v0 = 0; v0 < a.V; v0 += piece) nparts += parts(a, v0);
@@ -512,11 +518,11 @@ struct Backward {
   Copy<Ty> ds;
   Gradient dh, dw;
 
-  Backward(const Args &a, Space &sp) {
+  Backward(const Args &a, Space &sp, int64_t limit) {
     const int64_t e = int64_t(Ty::PARTS) * sizeof(typename Ty::T);
     copy_w = Ty::PARTS == 2 ? !raw_w<Ty>(a) : !rows16(a.W, a.ldw, a.dtype);
     const int64_t of_ds = e * a.rows, of_w = copy_w ? e * up(a.D, 8) : 0;
-    piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype);
+    piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype, limit);
     score = score_tiles(a.rows, piece, raw_w<Ty>(a));
     scale = sp.take<float>(a.rows);
     h.take(sp, a.rows, a.D);
@@ -760,14 +766,19 @@ silcu_status check_pointers(const char *what, const Args &a) {
   return SILCU_OK;
 }
 
-silcu_status check_space(const char *what, const Args &a, int backward, void *ws, size_t bytes) {
-  const size_t need = silcu_linear_cross_entropy_workspace_bytes(&a, backward);
+constexpr size_t kAlign = 256;  // the caller's workspace need not be aligned
+char *aligned(void *p) { return reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(p) + kAlign - 1) & ~uintptr_t(kAlign - 1)); }
+
+// The plan of a call, Forward or Backward, laid out in its workspace, once that is known to hold it.
+template <template <typename> class Plan, typename Ty, typename F>
+silcu_status with_plan(const char *what, const Args &a, void *ws, size_t bytes, F &&run) {
+  Space sp{aligned(ws)};
+  const Plan<Ty> plan(a, sp, piece_limit());
+  const size_t need = sp.used + kAlign;
   if (!ws || bytes < need) return fail(SILCU_WORKSPACE_TOO_SMALL, "%s: workspace %zu < %zu", what, bytes, need);
   if (!device_error_ptr()) return fail(SILCU_CUDA_ERROR, "%s: no device error word", what);
-  return SILCU_OK;
+  return run(plan);
 }
-
-char *align256(void *p) { return reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(p) + 255) & ~uintptr_t(255)); }
 
 }  // namespace
 }  // namespace silcu
@@ -778,14 +789,15 @@ size_t silcu_linear_cross_entropy_workspace_bytes(const silcu_cross_entropy_args
   using namespace silcu;
   if (check_shape("linear_cross_entropy_workspace_bytes", ap) != SILCU_OK || ap->rows == 0) return 0;
   Space f{nullptr}, b{nullptr};
+  const int64_t limit = piece_limit();
   if (ap->dtype == SILCU_BF16) {
-    Forward<Bf16> plan(*ap, f);
-    if (backward) Backward<Bf16> plan_b(*ap, b);
+    Forward<Bf16> plan(*ap, f, limit);
+    if (backward) Backward<Bf16> plan_b(*ap, b, limit);
   } else {
-    Forward<Tf32> plan(*ap, f);
-    if (backward) Backward<Tf32> plan_b(*ap, b);
+    Forward<Tf32> plan(*ap, f, limit);
+    if (backward) Backward<Tf32> plan_b(*ap, b, limit);
   }
-  return (f.used > b.used ? f.used : b.used) + 256;  // the caller's pointer need not be aligned
+  return (f.used > b.used ? f.used : b.used) + kAlign;
 }
 
 silcu_status silcu_linear_cross_entropy(const silcu_cross_entropy_args *ap, void *workspace, size_t workspace_bytes,
@@ -808,9 +820,9 @@ silcu_status silcu_linear_cross_entropy(const silcu_cross_entropy_args *ap, void
   const Span ins[] = {{a.H, a.rows, a.D * e, a.ldh * e}, {a.W, a.V, a.D * e, a.ldw * e}, flat(a.targets, 4 * a.rows)};
   if (outputs_overlap(outs, 2, ins, 3))
     return fail(SILCU_INVALID_ARGUMENT, "linear_cross_entropy: a result overlaps an operand");
-  if ((st = check_space("linear_cross_entropy", a, 0, workspace, workspace_bytes)) != SILCU_OK) return st;
-  Space sp{align256(workspace)};
-  return a.dtype == SILCU_BF16 ? forward(a, Forward<Bf16>(a, sp), s) : forward(a, Forward<Tf32>(a, sp), s);
+  auto run = [&](const auto &plan) { return forward(a, plan, s); };
+  return a.dtype == SILCU_BF16 ? with_plan<Forward, Bf16>("linear_cross_entropy", a, workspace, workspace_bytes, run)
+                               : with_plan<Forward, Tf32>("linear_cross_entropy", a, workspace, workspace_bytes, run);
 }
 
 silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args *ap, void *workspace,
@@ -840,9 +852,9 @@ silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args 
                       flat(a.lse, 4 * a.rows),
                       flat(a.dloss, a.reduction == SILCU_REDUCE_NONE ? 4 * a.rows : 4)};
   if (outputs_overlap(outs, 2, ins, 5)) return fail(SILCU_INVALID_ARGUMENT, "%s: a gradient overlaps an operand", what);
-  if ((st = check_space(what, a, 1, workspace, workspace_bytes)) != SILCU_OK) return st;
-  Space sp{align256(workspace)};
-  return a.dtype == SILCU_BF16 ? backward(a, Backward<Bf16>(a, sp), s) : backward(a, Backward<Tf32>(a, sp), s);
+  auto run = [&](const auto &plan) { return backward(a, plan, s); };
+  return a.dtype == SILCU_BF16 ? with_plan<Backward, Bf16>(what, a, workspace, workspace_bytes, run)
+                               : with_plan<Backward, Tf32>(what, a, workspace, workspace_bytes, run);
 }
 
 }  // extern "C"
