@@ -33,6 +33,9 @@ inline bool aligned16(const void *p) {
 // has ended (programmatic dependent launch): its start-up overlaps the other's
 // tail.  It calls wait_for_previous() before it reads or writes anything that
 // others touch; the one ahead calls let_next_start() early on.
+// Such a kernel's life overlaps the writes of its predecessors, so nothing it reads is
+// constant for that life: no read-only loads, and no const parameters declared free of
+// aliases, which let the compiler choose such loads or move them above the wait.
 template <typename... Params, typename... Args>
 cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};

@@ -65,10 +65,9 @@ __device__ __forceinline__ double count_rows(const int32_t *targets, int64_t row
 // end.  The CTA that finishes last adds the losses, in row order whichever it
 // is: `done` counts the CTAs, and the scores' launch has set it to 0.
 constexpr int kFinishRows = 8;
-__global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ part, int nparts, int64_t rows,
-                                                    const int32_t *__restrict__ targets, int V,
-                                                    const float *__restrict__ target_score, float *__restrict__ lse,
-                                                    float *loss, int mean, unsigned *done, float *__restrict__ total) {
+__global__ void __launch_bounds__(1024) loss_finish(const float2 *part, int nparts, int64_t rows, const int32_t *targets,
+                                                    int V, const float *target_score, float *lse, float *loss, int mean,
+                                                    unsigned *done, float *total) {
   __shared__ float2 sm[32][kFinishRows];
   __shared__ double sums[32];
   __shared__ int counts[32];
@@ -95,7 +94,7 @@ __global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ p
   if (row < rows) {
 #pragma unroll 4
     for (int i = threadIdx.x >> 3; i < nparts; i += 128) {
-      const float2 x = __ldcs(part + int64_t(i) * rows + row);
+      const float2 x = load_streaming(part + int64_t(i) * rows + row);
       join(x.x, x.y);
     }
   }
@@ -131,7 +130,7 @@ __global__ void __launch_bounds__(1024) loss_finish(const float2 *__restrict__ p
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < rows; i += 1024) {
     const int t = targets[i];
-    s += double(__ldcg(loss + i));
+    s += double(load_l2(loss + i));
     n += t >= 0 && t < V;
   }
   s = warp_sum(s);
@@ -171,9 +170,8 @@ __device__ __forceinline__ void row_scales(const Scales &c, const int32_t *targe
 // tensor core reads its upper 19 bits) and lo takes what that leaves.  With `scales`
 // the first CTA writes the rows' scales.
 template <typename T>
-__global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int64_t ld, int64_t rows, int D, int dp,
-                                                 const int32_t *__restrict__ targets, int V, T *__restrict__ dst,
-                                                 float *__restrict__ lo, const Scales scales) {
+__global__ void __launch_bounds__(256) copy_rows(const T *src, int64_t ld, int64_t rows, int D, int dp,
+                                                 const int32_t *targets, int V, T *dst, float *lo, const Scales scales) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = dp / W;
   const bool vec = ld % W == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
@@ -191,7 +189,7 @@ __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int6
     Raw<T, W> v = raw_zero<T, W>();
     bool keep = true;
     if (targets) {
-      const int y = __ldg(targets + r);
+      const int y = targets[r];
       keep = y >= 0 && y < V;
     }
     if (keep) {
@@ -226,9 +224,8 @@ __global__ void __launch_bounds__(256) copy_rows(const T *__restrict__ src, int6
 // for few elements of many planes by WAYS neighbouring lanes that take turns at the planes
 // (16 planes of 100 x 1024: 9 us by one thread).
 template <typename T, int WAYS>
-__global__ void __launch_bounds__(256) planes_finish(const float *__restrict__ planes, int nplanes, int64_t plane,
-                                                     int64_t rows, int D, int ldp, const float *__restrict__ alpha,
-                                                     T *__restrict__ out, int64_t ldo, int vec) {
+__global__ void __launch_bounds__(256) planes_finish(const float *planes, int nplanes, int64_t plane, int64_t rows, int D,
+                                                     int ldp, const float *alpha, T *out, int64_t ldo, int vec) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = (D + W - 1) / W;
   const int64_t n = rows * per_row;

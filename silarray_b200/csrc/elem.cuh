@@ -49,11 +49,50 @@ template <> struct Raw<__nv_bfloat16, 8> { uint4 r; };
 template <> struct Raw<__nv_bfloat16, 1> { unsigned short r; };
 
 // Streaming loads and stores (the data is not read again by this kernel).
-// Not the read-only path: outputs may be one of the inputs.
+// The loads are volatile, so they stay behind wait_for_previous(), and not of the read-only
+// path: an earlier kernel that is still running may write what they read (see
+// launch_after), and outputs may be one of the inputs.
+__device__ __forceinline__ float load_streaming(const float *p) {
+  float v;
+  asm volatile("ld.global.cs.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned short load_streaming(const unsigned short *p) {
+  unsigned short v;
+  asm volatile("ld.global.cs.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_streaming(const float2 *p) {
+  float2 v;
+  asm volatile("ld.global.cs.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_streaming(const float4 *p) {
+  float4 v;
+  asm volatile("ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 load_streaming(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+// The same from the L2: what other CTAs of this kernel have written.
+__device__ __forceinline__ float load_l2(const float *p) {
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> raw_load(const T *p) {
   Raw<T, VEC> v;
-  v.r = __ldcs(reinterpret_cast<const decltype(v.r) *>(p));
+  v.r = load_streaming(reinterpret_cast<const decltype(v.r) *>(p));
   return v;
 }
 template <typename T, int VEC>

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(512) ln_forward_long(const LnArgs a) {
     if (a.rstd_out) a.rstd_out[row] = rstd;
   }
   for (uint32_t c = threadIdx.x; c < a.cols; c += 512) {
-    float v[1] = {fmaf((at(c) - mu) * rstd, __ldg(a.gamma + c), __ldg(a.beta + c))};
+    float v[1] = {fmaf((at(c) - mu) * rstd, a.gamma[c], a.beta[c])};
     Raw<T, 1> o;
     pack(v, o);
     raw_store<T, 1>(dst + c, o);
@@ -277,8 +277,8 @@ struct LnRow {
       dy[j] = in ? raw_load<T, VEC>(py + c) : raw_zero<T, VEC>();
       if (RES) res[j] = in ? raw_load<T, VEC>(pr + c) : raw_zero<T, VEC>();
     }
-    mean = __ldg(a.mean + row);
-    rstd = __ldg(a.rstd + row);
+    mean = a.mean[row];
+    rstd = a.rstd[row];
   }
 };
 
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(256) ln_backward_cols(const LnArgs a) {
     float x[1], dy[1];
     unpack(raw_load<T, 1>(px + row * a.cols + c), x);
     unpack(raw_load<T, 1>(py + row * a.cols + c), dy);
-    g = fmaf(dy[0], (x[0] - __ldg(a.mean + row)) * __ldg(a.rstd + row), g);
+    g = fmaf(dy[0], (x[0] - a.mean[row]) * a.rstd[row], g);
     b += dy[0];
   }
   float *part = a.part + uint64_t(blockIdx.y) * 2 * a.cols;
@@ -485,14 +485,14 @@ __global__ void __launch_bounds__(512) ln_backward_long(const LnArgs a) {
   };
   float c1 = 0.f, c2 = 0.f;
   for (uint32_t c = threadIdx.x; c < a.cols; c += 512) {
-    const float w = at(py, c) * __ldg(a.gamma + c);
+    const float w = at(py, c) * a.gamma[c];
     c1 += w;
     c2 = fmaf(w, (at(px, c) - mean) * rstd, c2);
   }
   c1 = group_sum<512>(c1, sm[0]) * inv_n;
   c2 = group_sum<512>(c2, sm[1]) * inv_n;
   for (uint32_t c = threadIdx.x; c < a.cols; c += 512) {
-    float v[1] = {rstd * (at(py, c) * __ldg(a.gamma + c) - c1 - (at(px, c) - mean) * rstd * c2)};
+    float v[1] = {rstd * (at(py, c) * a.gamma[c] - c1 - (at(px, c) - mean) * rstd * c2)};
     if (RES) v[0] += at(pr, c);
     Raw<T, 1> o;
     pack(v, o);
@@ -504,8 +504,8 @@ __global__ void __launch_bounds__(512) ln_backward_long(const LnArgs a) {
 // decides.  COLS columns a CTA, 1024 / COLS threads for the rows of each.  Few columns
 // spread over more SMs with 8 of them (768 columns, 888 partial rows: 4.7 us with 32).
 template <int COLS>
-__global__ void __launch_bounds__(1024) ln_finish(const float *__restrict__ part, uint32_t nparts, uint32_t cols,
-                                                  float *__restrict__ dgamma, float *__restrict__ dbeta) {
+__global__ void __launch_bounds__(1024) ln_finish(const float *part, uint32_t nparts, uint32_t cols, float *dgamma,
+                                                  float *dbeta) {
   constexpr uint32_t SLICES = 1024 / COLS;
   __shared__ float sm[32][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(1024) ln_finish(const float *__restrict__ part
   wait_for_previous();
   if (c < 2 * cols) {
 #pragma unroll 8
-    for (uint32_t i = threadIdx.x / COLS; i < nparts; i += SLICES) s += __ldcs(part + uint64_t(i) * 2 * cols + c);
+    for (uint32_t i = threadIdx.x / COLS; i < nparts; i += SLICES) s += load_streaming(part + uint64_t(i) * 2 * cols + c);
   }
 #pragma unroll
   for (int step = COLS; step < 32; step *= 2) s += __shfl_xor_sync(0xffffffffu, s, step);
