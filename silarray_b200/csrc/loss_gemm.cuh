@@ -24,9 +24,12 @@
 // same times, and prefetching operands to the L2 made them worse.
 //
 // Sums: the tensor core truncates as it accumulates, so sums that need more
-// than its 2^-22 per step are cut into chunks (128 k of tf32, 1024 k of the bf16
-// scores that become lse); the epilogue adds each chunk in fp32 registers, to
-// nearest, while the next one runs.  What is rounded to bf16 next takes one chunk.
+// than its 2^-22 per step are cut into chunks (128 k of tf32, 1024 k of bf16 scores);
+// the epilogue adds each chunk in fp32 registers, to nearest, while the next one runs.
+// The backward's bf16 scores take the forward's chunks although ds is rounded to bf16
+// next: 8 x 10^-4 of a sum of 131072 products of one sign is lost in one chunk, 10^-5 of
+// one of 4096, and where p is near 1 that much is left in p - 1.  It costs steps of D above
+// 1024 up to 1 % (4096 rows of 32768 x 4096 3.14 -> 3.18 ms).
 //
 // Every wait is bounded; on expiry the kernel records a code, unwinds, lets what
 // is in flight land, frees its TMEM and exits.  No load is multicast.
@@ -127,15 +130,19 @@ struct Cfg {
   static constexpr int SMEM_BYTES = RING_BYTES + EPI_WARPS * 4096 + 1024 + 512;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int NBUF = 2;
-  // stages per accumulation chunk; MULTI: a tile may take several, which meet in registers
-  static constexpr bool MULTI = Ty::PARTS == 2 || EPI == kStats;
+  // Stages per accumulation chunk; a tile may take several, which meet in registers.
+  // SUMS: every tile's sums pass through registers; else those of one chunk stay in TMEM.
+  static constexpr bool SUMS = Ty::PARTS == 2 || EPI == kStats;
   // Columns that join the sums at a time: 32 leave the tf32 sums no registers, and
   // what spills there every chunk pays for (score gradients 660 -> 477 us with 16).
-  static constexpr int LD = Ty::PARTS == 2 ? 16 : 32;
-  // The tf32 sums go back to TMEM for the epilogues that have no registers beside
-  // them (with the 128 sums in registers the score gradients spill 2.8 KB a thread).
-  static constexpr bool BACK = MULTI && (EPI == kScoreGrad || EPI == kOut);
-  static constexpr int CHUNK = !MULTI ? 1 << 30 : (Ty::PARTS == 2 ? 128 : 1024) / BK;
+  static constexpr int LD = EPI == kStats && Ty::PARTS == 1 ? 32 : 16;
+  // The sums go back to TMEM for the epilogues that have no registers beside
+  // them (with the 128 sums in registers the tf32 score gradients spill 2.8 KB a thread).
+  static constexpr bool BACK = !SUMS || EPI == kScoreGrad || EPI == kOut;
+  // The scores' chunks are the same in both passes, which so see the same scores:
+  // (p - 1) of a target that is all but certain is what is left of them.
+  static constexpr int CHUNK =
+      (Ty::PARTS == 2 ? 128 : EPI == kStats || EPI == kScoreGrad ? 1024 : 1 << 24) / BK;
   // Rows of tiles that are walked together, column by column.  The scores read W once
   // (their H stays in the L2); kOut's tiles of one row of them follow one another and share its
   // ds: against groups of 8 the DRAM reads of 4096 x 8192 x 768 fp32 fall from 1018 to 783 MB,
@@ -477,7 +484,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       };
       // What the epilogue needs of the row: asked for while the MMAs run, where
       // three registers are left beside the sums.
-      constexpr bool EARLY = !C::BACK;
+      constexpr bool EARLY = PARTS == 1 || !C::BACK;
       int y = -1;
       float lse = 0.f, g = 0.f;
       auto row_data = [&] {
@@ -491,10 +498,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       };
       if (EARLY) row_data();
       const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + half * h;
-      float acc[C::MULTI ? 128 : 1];
-      if constexpr (C::MULTI) {
+      float acc[128];
+      if (C::SUMS || tl.kb1 - tl.kb0 > C::CHUNK) {
         int kc = tl.kb0;
-        if constexpr (PARTS == 1) {  // the first chunk lands in the sums' registers
+        if constexpr (C::SUMS && PARTS == 1) {  // the first chunk lands in the sums' registers
           ok = finished(cg);
           if (ok && cols > 0) {
 #pragma unroll
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
       cg++;
       if (!ok) break;  // a wait gave up; ok is the same in all lanes
       if (!EARLY) row_data();
-      constexpr bool IN_REGS = C::MULTI && !C::BACK;
+      constexpr bool IN_REGS = !C::BACK;
       // Columns 32 cb .. 32 cb + 31 of this thread's row, for cb = 0, 1, 2, 3 in
       // turn; from TMEM the next ones are on their way while these are used.
       float ahead[IN_REGS ? 1 : 32];
