@@ -24,8 +24,10 @@
 // same times, and prefetching operands to the L2 made them worse.
 //
 // Sums: the tensor core truncates as it accumulates, so sums that need more
-// than its 2^-22 per step are cut into chunks (128 k of tf32, 1024 k of bf16 scores);
-// the epilogue adds each chunk in fp32 registers, to nearest, while the next one runs.
+// than its 2^-22 per step are cut into chunks; the epilogue adds each chunk in fp32
+// registers, to nearest, while the next one runs.  Chunks are 128 k of tf32, 1024 k of bf16
+// scores, and 16384 k of the products of bf16 ds, whose results are rounded to bf16: of a sum of
+// one sign such a chunk loses 3 x 10^-5 (2^-13 at most), where 211000 terms in one lost 1.2 x 10^-3.
 // The backward's bf16 scores take the forward's chunks although ds is rounded to bf16
 // next: 8 x 10^-4 of a sum of 131072 products of one sign is lost in one chunk, 10^-5 of
 // one of 4096, and where p is near 1 that much is left in p - 1.  It costs steps of D above
@@ -142,7 +144,7 @@ struct Cfg {
   // The scores' chunks are the same in both passes, which so see the same scores:
   // (p - 1) of a target that is all but certain is what is left of them.
   static constexpr int CHUNK =
-      (Ty::PARTS == 2 ? 128 : EPI == kStats || EPI == kScoreGrad ? 1024 : 1 << 24) / BK;
+      (Ty::PARTS == 2 ? 128 : EPI == kStats || EPI == kScoreGrad ? 1024 : 16384) / BK;
   // Rows of tiles that are walked together, column by column.  The scores read W once
   // (their H stays in the L2); kOut's tiles of one row of them follow one another and share its
   // ds: against groups of 8 the DRAM reads of 4096 x 8192 x 768 fp32 fall from 1018 to 783 MB,

@@ -43,3 +43,67 @@ def test_both_passes_see_the_same_scores(cuda, rows, V, D, score):
         ref = -1.0 / (1.0 + torch.exp(s) / (V - 1))
         one = s * (D / 1024 / 2 * U + 32.5 * 2.0 ** -22)  # of a score, in each pass
         assert bool(((ds - ref).abs() <= 2 * one + tol).all()), float((ds - ref).abs().max())
+
+
+# ------------------------------------------------------- long sums of one sign
+# All scores are 0 here, so p is 1 / V everywhere.  The target's term comes last in its sum and
+# takes away what the others add up to, as bf16 holds it: what is left is rounded to bf16
+# so finely that the error of the sum itself shows.
+def tiles_of_every_pair():
+    """As many tiles of 256 columns as there are pairs of SMs: no reason to split a sum for them."""
+    return torch.cuda.get_device_properties(0).multi_processor_count // 2
+
+
+def positive(rows, cols, seed):
+    """bf16 values of [0.5, 1.5)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    out = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    for i in range(0, rows, 8192):
+        part = out[i:i + 8192]
+        part.copy_(torch.rand(part.shape, generator=g, device="cuda").add_(0.5))
+    return out
+
+
+def ds_of(V):
+    """p and p - 1 as ds holds them.  p has bits enough for products that fill the sums' last
+    ones, and lies where an error of 2^-20 does not round it another way."""
+    p = float(torch.tensor(1.0 / V, dtype=torch.float64).bfloat16())
+    assert abs(1.0 / V - p) * V < 2.0 ** -11 and not p.hex().startswith("0x1.0")
+    return p, float(torch.tensor(1.0 / V - 1.0, dtype=torch.float64).bfloat16())
+
+
+def check_sum(got, others, target):
+    """Against `others` + `target` (fp64): 1024 additions (16384 k) truncated by 2^-22 of the chunk's
+    sum so far, half of it on average, then a few rounded joins, and the result's rounding."""
+    ref = others + target
+    tol = (512 * 2.0 ** -22 + 40 * U) * others + 2.0 ** -8 * ref.abs()
+    err = (got.double() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("rows", [128, 256])
+def test_long_sums_over_the_vocabulary(cuda, rows):
+    V, D = 211000, 256 * tiles_of_every_pair()
+    p, p1 = ds_of(V)
+    W = positive(V, D, 1)
+    others = p * W[:-1].sum(0, dtype=torch.float64)
+    W[-1] = (-others / p1).bfloat16()
+    H = torch.zeros(rows, D, device="cuda", dtype=torch.bfloat16)
+    y = torch.full((rows,), V - 1, device="cuda", dtype=torch.int32)
+    _, lse = gpu.linear_cross_entropy(H, W, y)
+    dH, _ = gpu.linear_cross_entropy_backward(H, W, y, lse, reduction="sum", need_dW=False)
+    check_sum(dH, others, p1 * W[-1].double())
+
+
+def test_long_sums_over_the_rows(cuda):
+    rows, V, D = 262144, 217, 256 * tiles_of_every_pair()
+    p, p1 = ds_of(V)
+    H = positive(rows, D, 2)
+    others = p * H[:-1].sum(0, dtype=torch.float64)
+    H[-1] = (-others / p1).bfloat16()
+    W = torch.zeros(V, D, device="cuda", dtype=torch.bfloat16)
+    y = torch.full((rows,), 1, device="cuda", dtype=torch.int32)
+    y[-1] = 0
+    _, lse = gpu.linear_cross_entropy(H, W, y)
+    _, dW = gpu.linear_cross_entropy_backward(H, W, y, lse, reduction="sum", need_dH=False)
+    check_sum(dW[0], others, p1 * H[-1].double())
