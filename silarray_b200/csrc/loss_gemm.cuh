@@ -179,6 +179,10 @@ struct Problem {
   int ksplit;              // each tile's K range in this many parts (kOut; part i -> plane i)
   int amn;                 // kOut: A is stored with the M index contiguous (kOutT: it always is)
   int mode, vec;           // vec: kDirect rows are 16-byte aligned
+  // Factor of kDirect results in bf16, or null: one, or with per_row one for each row of
+  // the result; kOutT has one for each of the N rows that it writes.
+  const float *alpha;
+  int per_row;
   void *out;
   int64_t ldo, plane;      // row stride; elements from one plane to the next
 };
@@ -193,7 +197,6 @@ struct __align__(64) Params {
   int stages;        // ring stages (RAW)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, rounds, tail, extra;  // rounds = n0 / units, tail = n0 % units
-  const float *alpha;  // kOut: factor of kDirect results in bf16, or null
   LossArgs loss;
   int part0;  // index of this launch's first part
   int *err;
@@ -436,7 +439,6 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
     const int qr = warp & 3, h = (warp - 2) >> 2;
     float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
     const int half = RAW || EPI == kOut ? p.half : 128;
-    const float alpha = (EPI == kOut || EPI == kOutT) && p.alpha ? *p.alpha : 1.0f;
     uint32_t cg = 0, kbe = 0;
     bool ok = true;
     for (int k = 0; ok && work_at(p, unit, k, w); k++) {
@@ -497,6 +499,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
             g = p.loss.scale ? p.loss.scale[row] : 1.0f;
           }
         }
+        if (EPI == kOut && PARTS == 1) g = q.alpha && row < q.M ? q.alpha[q.per_row ? row : 0] : 1.0f;
       };
       if (EARLY) row_data();
       const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + half * h;
@@ -673,7 +676,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
 #pragma unroll
               for (int i = 0; i < 32; i++) {
                 if (32 * cb + i < cols) {
-                  if (q.mode == kDirect) store_as(static_cast<T *>(q.out) + at + i * q.ldo, alpha * v[i]);
+                  if (q.mode == kDirect) store_as(static_cast<T *>(q.out) + at + i * q.ldo, q.alpha ? q.alpha[c0 + 32 * cb + i] * v[i] : v[i]);
                   else if (q.mode == kPlane) static_cast<float *>(q.out)[tl.part * q.plane + at + i * q.ldo] = v[i];
                   else red_add(static_cast<float *>(q.out) + tl.part * q.plane + at + i * q.ldo, v[i]);
                 }
@@ -697,10 +700,8 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
 #pragma unroll
               for (int i = 0; i < 4; i++)
                 put(4 * (cb & 1) + i,
-                    make_uint4(pack_bf16(alpha * v[8 * i], alpha * v[8 * i + 1]),
-                               pack_bf16(alpha * v[8 * i + 2], alpha * v[8 * i + 3]),
-                               pack_bf16(alpha * v[8 * i + 4], alpha * v[8 * i + 5]),
-                               pack_bf16(alpha * v[8 * i + 6], alpha * v[8 * i + 7])));
+                    make_uint4(pack_bf16(g * v[8 * i], g * v[8 * i + 1]), pack_bf16(g * v[8 * i + 2], g * v[8 * i + 3]),
+                               pack_bf16(g * v[8 * i + 4], g * v[8 * i + 5]), pack_bf16(g * v[8 * i + 6], g * v[8 * i + 7])));
               if ((cb & 1) || 32 * (cb + 1) >= cols)
                 send(
                     static_cast<unsigned short *>(q.out), ldo, c0 + 32 * (cb & ~1), whole,
