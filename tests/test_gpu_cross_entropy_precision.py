@@ -107,3 +107,22 @@ def test_long_sums_over_the_rows(cuda):
     _, lse = gpu.linear_cross_entropy(H, W, y)
     _, dW = gpu.linear_cross_entropy_backward(H, W, y, lse, reduction="sum", need_dH=False)
     check_sum(dW[0], others, p1 * H[-1].double())
+
+
+# ------------------------------------------------ operands with the low bits set
+@pytest.mark.parametrize("rows", [8, 200])  # W as it lies in memory, W with a copy of its remainders
+@pytest.mark.parametrize("h,w", [(1.0 + 2.0 ** -10 - 2.0 ** -20,) * 2])
+def test_fp32_operands_keep_their_low_bits(cuda, rows, h, w):
+    """One product per score, 64 h w, so lse is the score.  x = hi + lo, and lo rounds to tf32: 13 bits
+    to 11, off by 2^-22 of w at most.  What lo lo would add is below 2^-21 of the product where one
+    factor is cut to hi (lo < 2^-10) and the other rounded (2^-11); where both are cut and
+    have their low bits set it would be 2^-20.  Here h rounds to 2^-20 of itself: lo lo is 2^-30.
+    The sum of the three terms may lose its last bit, 2^-23."""
+    V, D = 300, 64
+    H, W = torch.zeros(rows, D, device="cuda"), torch.zeros(V, D, device="cuda")
+    H[:, 0] = h
+    W[:, 0] = -64.0
+    W[5, 0] = 64.0 * w
+    _, lse = gpu.linear_cross_entropy(H, W, torch.full((rows,), 5, device="cuda", dtype=torch.int32))
+    err = (lse.double() / (64.0 * H[:, 0].double() * (W[5, 0].double() / 64.0)) - 1.0).abs()
+    assert float(err.max()) <= (2.0 ** -22 if h == 1.0 else 2.0 ** -30 + 2.0 ** -23) + 2.0 ** -28
