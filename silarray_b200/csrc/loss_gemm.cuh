@@ -105,6 +105,15 @@ __device__ __forceinline__ float tf32_trunc(float x) {
   return __uint_as_float(__float_as_uint(x) & 0xffffe000u);
 }
 
+// x - tf32_trunc(x) for the tensor core, which cuts it to 11 bits of 13: 2^-12 of itself more is a
+// quarter to half a step of those, so that what is cut is off by half a step at most and an
+// eighth on average, as if it had been rounded (three eighths without, all of them toward
+// zero).  The epilogue warps' instructions are what a stage of few rows waits for: 4 rows of 50000 x
+// 2048 take 154 us with this, 152 without, 162 with a conversion that rounds.
+__device__ __forceinline__ float remainder_of(float x) {
+  return __fmul_rn(__fsub_rn(x, tf32_trunc(x)), 1.0f + 1.0f / 4096.0f);
+}
+
 struct Bf16 {
   using T = __nv_bfloat16;
   static constexpr int PARTS = 1, KROW = 64, KMMA = 16;  // k in a 128-byte row, and of one MMA
@@ -459,10 +468,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           float4 *hi = reinterpret_cast<float4 *>(smem + s * STAGE_BYTES + (RAW_A ? 0 : 2 * TILE_A)), *lo = hi + tile / 16;
           for (int e = int(threadIdx.x) - 64; e < tile / 16; e += 32 * C::EPI_WARPS) {
             float4 x = hi[e];
-            x.x = __fsub_rn(x.x, tf32_trunc(x.x));
-            x.y = __fsub_rn(x.y, tf32_trunc(x.y));
-            x.z = __fsub_rn(x.z, tf32_trunc(x.z));
-            x.w = __fsub_rn(x.w, tf32_trunc(x.w));
+            x.x = remainder_of(x.x);
+            x.y = remainder_of(x.y);
+            x.z = remainder_of(x.z);
+            x.w = remainder_of(x.w);
             lo[e] = x;
           }
           fence_proxy_async_smem();

@@ -111,7 +111,7 @@ def test_long_sums_over_the_rows(cuda):
 
 # ------------------------------------------------ operands with the low bits set
 @pytest.mark.parametrize("rows", [8, 200])  # W as it lies in memory, W with a copy of its remainders
-@pytest.mark.parametrize("h,w", [(1.0 + 2.0 ** -10 - 2.0 ** -20,) * 2])
+@pytest.mark.parametrize("h,w", [(1.0, 1.0 + 2.0 ** -10 - 2.0 ** -23), (1.0 + 2.0 ** -10 - 2.0 ** -20,) * 2])
 def test_fp32_operands_keep_their_low_bits(cuda, rows, h, w):
     """One product per score, 64 h w, so lse is the score.  x = hi + lo, and lo rounds to tf32: 13 bits
     to 11, off by 2^-22 of w at most.  What lo lo would add is below 2^-21 of the product where one
