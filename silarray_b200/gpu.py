@@ -507,13 +507,17 @@ def _scratch(nbytes, device):
     return buf, buf.data_ptr()
 
 
+def _on(index, fn, *args):
+    """fn(*args) with GPU `index` as the current one: workspace sizes depend on it, too."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def _launch(fn, index, *args):
     """fn(*args, stream) on GPU `index` and its current stream."""
-    if torch._C._cuda_getDevice() == index:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
-    else:
-        with torch.cuda.device(index):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    check(_on(index, fn, *args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _rows_cols(IN, rows, cols):
@@ -553,7 +557,7 @@ def layer_norm_backward(dout, IN, mean, rstd, gamma, dresidual=None, din=None, d
     din, p = _out("layer_norm din", din, IN, n, index)
     dgamma, pg = _out("layer_norm dgamma", dgamma, gamma, cols, index)
     dbeta, pb = _out("layer_norm dbeta", dbeta, gamma, cols, index)
-    nbytes = lib().silcu_layer_norm_backward_workspace_bytes(rows, cols, dt)
+    nbytes = _on(index, lib().silcu_layer_norm_backward_workspace_bytes, rows, cols, dt)
     buf, ws = _scratch(nbytes, IN.device)
     _launch(lib().silcu_layer_norm_backward, index, *ops, p, pg, pb, rows, cols, dt, ws, nbytes)
     return din, dgamma, dbeta
@@ -611,7 +615,7 @@ def linear_cross_entropy(H, W, targets, reduction="mean", loss=None, lse=None):
     each = reduction == "none"
     loss = (torch.empty_like(lse) if each else lse.new_empty(())) if loss is None else loss
     a.loss = _at("linear_cross_entropy loss", loss, _F32, n if each else 1, index)
-    nbytes = lib().silcu_linear_cross_entropy_workspace_bytes(a, 0)
+    nbytes = _on(index, lib().silcu_linear_cross_entropy_workspace_bytes, a, 0)
     buf, ws = _scratch(nbytes, H.device)
     _launch(lib().silcu_linear_cross_entropy, index, a, ws, nbytes)
     return loss, lse
@@ -629,7 +633,7 @@ def linear_cross_entropy_backward(H, W, targets, lse, dloss=None, reduction="mea
         dH, a.dH, a.lddh = _gradient("linear_cross_entropy dH", dH, H, index)
     if need_dW:
         dW, a.dW, a.lddw = _gradient("linear_cross_entropy dW", dW, W, index)
-    nbytes = lib().silcu_linear_cross_entropy_workspace_bytes(a, 1)
+    nbytes = _on(index, lib().silcu_linear_cross_entropy_workspace_bytes, a, 1)
     buf, ws = _scratch(nbytes, H.device)
     _launch(lib().silcu_linear_cross_entropy_backward, index, a, ws, nbytes)
     return dH if need_dH else None, dW if need_dW else None
@@ -670,7 +674,7 @@ class TensorList:
         self.scalar = torch.empty((), dtype=_F32, device=self.device)
         self.spans = sorted((a, a + c * t.element_size())
                             for a, c, t in zip(addresses, counts, self.tensors) if c)
-        self.nbytes = lib().silcu_grad_norm_workspace_bytes(self.array, n)
+        self.nbytes = _on(index, lib().silcu_grad_norm_workspace_bytes, self.array, n)
         self._addresses, self._counts, self._dtypes = addresses, counts, dtypes
         self._clips_into = None
         return self
