@@ -291,11 +291,13 @@ using lossmm::Bf16;
 using lossmm::Operand;
 using lossmm::Tf32;
 
-// Of a piece's ds (and of its copied weights).
-// Larger pieces add to dH's planes less often, smaller ones stay nearer to the
-// L2's size (when chosen): 8192 rows of bf16 (131072 columns, D 2048) 13.4 ms at 256 MB, 13.0 at
-// 128, 13.7 at 64; 16384 fp32 rows (32768 columns, D 768) 15.6 ms at 512 MB, 16.4 at 256.
-constexpr int64_t kPieceBytes[2] = {int64_t(512) << 20, int64_t(128) << 20};  // by silcu_dtype
+// Elements of a piece's ds, and of its copied weights: 128 MB of bf16, 512 MB of tf32 pairs.
+// Each piece ends its two launches on a round of tiles that is not full, and adds to dH's planes;
+// 2^26 scores are 1024 tiles of 256 x 256, 14 rounds of 74 pairs.  The L2 plays no part.  The
+// backward passes of 16 shapes (both types, 512 to 32768 rows, 20000 to 131072 columns, D 512
+// to 4096) took, against each one's best piece, 6 % more on average with 2^25 scores, 3 % with 2^26
+// (11 % at most), 2 % with 2^27, which would double the memory.
+constexpr int64_t kPieceElements = int64_t(1) << 26;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
@@ -309,10 +311,10 @@ int64_t piece_limit() {
   return up(want < 1 ? 1 : want < (1 << 24) ? want : 1 << 24, 256);
 }
 
-// Vocabulary columns per piece: a multiple of 256 whose `bytes` per column
-// stay within the limit, and pieces of about equal size.
-int64_t piece_of(int64_t V, int64_t bytes, int dtype, int64_t limit) {
-  int64_t p = kPieceBytes[dtype] / bytes / 256 * 256;
+// Vocabulary columns per piece: a multiple of 256 that stays within the limit at
+// `elements` per column, and pieces of about equal size.
+int64_t piece_of(int64_t V, int64_t elements, int64_t limit) {
+  int64_t p = kPieceElements / elements / 256 * 256;
   if (p < 256) p = 256;
   if (limit < p) p = limit;
   if (p >= V) return V;
@@ -420,7 +422,7 @@ struct Forward {
   Forward(const Args &a, Space &sp, int64_t limit) {
     copy_h = Ty::PARTS == 2 || !rows16(a.H, a.ldh, a.dtype);
     copy_w = Ty::PARTS == 2 ? !raw_w<Ty>(a) : !rows16(a.W, a.ldw, a.dtype);
-    piece = copy_w ? piece_of(a.V, int64_t(Ty::PARTS) * sizeof(typename Ty::T) * up(a.D, 8), a.dtype, limit) : a.V;
+    piece = copy_w ? piece_of(a.V, up(a.D, 8), limit) : a.V;
     tiles = score_tiles(a.rows, piece, raw_w<Ty>(a));
     nparts = 0;
     for (int64_t v0 = 0; v0 < a.V; v0 += piece) nparts += parts(a, v0);
@@ -523,10 +525,9 @@ struct Backward {
   Gradient dh, dw;
 
   Backward(const Args &a, Space &sp, int64_t limit) {
-    const int64_t e = int64_t(Ty::PARTS) * sizeof(typename Ty::T);
     copy_w = Ty::PARTS == 2 ? !raw_w<Ty>(a) : !rows16(a.W, a.ldw, a.dtype);
-    const int64_t of_ds = e * a.rows, of_w = copy_w ? e * up(a.D, 8) : 0;
-    piece = piece_of(a.V, of_ds > of_w ? of_ds : of_w, a.dtype, limit);
+    const int64_t of_w = copy_w ? up(a.D, 8) : 0;
+    piece = piece_of(a.V, a.rows > of_w ? a.rows : of_w, limit);
     score = score_tiles(a.rows, piece, raw_w<Ty>(a));
     scale = sp.take<float>(a.rows + 1);
     h.take(sp, a.rows, a.D);
