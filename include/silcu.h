@@ -429,8 +429,9 @@ silcu_status silcu_linear_cross_entropy_backward(const silcu_cross_entropy_args 
  * min(1, max_norm / (norm + eps)), a factor rounded to fp32: in place when outputs_host is
  * NULL, else into outputs_host[i], a tensor of the same size and dtype that
  * either is tensors[i] or overlaps none of the list.  Clipped tensors do not
- * overlap one another (for the norm alone they may: each counts).  A norm that is NaN makes
- * every element NaN; an infinite one makes finite elements 0. */
+ * overlap one another (for the norm alone they may: each counts), and neither norm nor the
+ * workspace overlaps any of them.  A norm that is NaN makes every element NaN; an infinite one
+ * makes finite elements 0, or with an infinite max_norm NaN (inf / inf). */
 typedef struct silcu_tensor {
   void *data;
   uint64_t n;
