@@ -414,8 +414,12 @@ typedef struct silcu_cross_entropy_args {
   void *dH, *dW;       /* backward */
   int64_t lddh, lddw;
 } silcu_cross_entropy_args;
-/* Workspace for both directions, or (backward = 0) for the forward pass alone.
- * Queried with the dH and dW (NULL or not) of the call. */
+/* Workspace for both directions, or (backward = 0) for the forward pass alone.  Queried with
+ * the call's own arguments: it depends on rows, V, D, dtype, reduction, on which of dH and dW are
+ * wanted, and on H, W, ldh and ldw, since operands whose rows do not start on 16-byte
+ * boundaries are copied (a query with NULL counts as aligned).  Of V it grows with 16 bytes
+ * for each row and tile of the scores (256 columns, fewer for few rows).  SILCU_LOSS_PIECE in the
+ * environment bounds the vocabulary entries that are worked on at a time. */
 size_t silcu_linear_cross_entropy_workspace_bytes(const silcu_cross_entropy_args *args_host, int backward);
 silcu_status silcu_linear_cross_entropy(const silcu_cross_entropy_args *args_host, void *workspace,
                                         size_t workspace_bytes, silcu_stream stream);

@@ -1,5 +1,6 @@
 """linear_cross_entropy's plan: the pieces that a call works in are the ones its
 workspace was checked for."""
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -55,3 +56,46 @@ def test_the_piece_limit_is_read_once_per_call(tmp_path):
     assert r.returncode == 0, r.stderr
     counts = [line.split() for line in r.stdout.splitlines()]
     assert len(counts) == 6 and all(int(n) <= 1 for _, n in counts), r.stdout
+
+
+def args(**kw):
+    a = _lib.CrossEntropyArgs()
+    for i, k in enumerate(("dH", "W", "targets", "loss", "lse", "H", "dW")):
+        setattr(a, k, (i + 1) << 34)
+    a.rows, a.V, a.D = 4096, 1 << 17, 768
+    for k, v in kw.items():
+        setattr(a, k, v)
+    for k in ("ldh", "ldw", "lddh", "lddw"):
+        setattr(a, k, getattr(a, k) or a.D)
+    return a
+
+
+def test_what_the_workspace_grows_with():
+    """Of the vocabulary only the forward's parts: two of 8 bytes for a tile of 256 columns (for 16
+    at least, where few rows have narrow tiles).  Pieces of about the same size hold the rest."""
+    _build.build()
+    size = _lib.lib().silcu_linear_cross_entropy_workspace_bytes
+    vocabularies = [1 << 17, 1 << 18, 1 << 20]
+    for rows in (1024, 4096):
+        parts = [16 * rows * v // 256 for v in vocabularies]
+        bf16, f32 = ([[size(C.byref(args(rows=rows, V=v, dtype=d)), b) for v in vocabularies] for b in (0, 1)] for d in (1, 0))
+        for s, n in zip(bf16[0], parts):  # its operands are read in place
+            assert abs((s - bf16[0][0]) - (n - parts[0])) <= n // 32, rows
+        for sizes in (bf16[1], *f32):
+            for s, n in zip(sizes, parts):
+                assert s <= 1.5 * sizes[0] + 1.1 * n, rows
+
+
+def test_the_workspace_of_another_layout():
+    """A query holds for operands laid out as they are in the call: unaligned ones are copied."""
+    _build.build()
+    lib = _lib.lib()
+    aligned = args(dtype=1)
+    for kw in (dict(H=(6 << 34) + 2), dict(W=(2 << 34) + 2), dict(ldw=769), dict(ldh=769)):
+        other = args(dtype=1, **kw)
+        for f, backward in ((lib.silcu_linear_cross_entropy, 0), (lib.silcu_linear_cross_entropy_backward, 1)):
+            need, own = (lib.silcu_linear_cross_entropy_workspace_bytes(C.byref(a), backward) for a in (aligned, other))
+            assert own >= need
+            if own > need:
+                assert f(C.byref(other), C.c_void_p(1 << 40), need, None) == 4
+            assert f(C.byref(other), C.c_void_p(1 << 40), own - 1, None) in (4, 2)

@@ -45,6 +45,22 @@ def test_both_passes_see_the_same_scores(cuda, rows, V, D, score):
         assert bool(((ds - ref).abs() <= 2 * one + tol).all()), float((ds - ref).abs().max())
 
 
+@pytest.mark.parametrize("rows,V,D,score", [(40, 300, 4096, 12), (300, 300, 4096, 12), (2048, 4096, 1024, 14)])
+def test_both_passes_see_the_same_fp32_scores(cuda, rows, V, D, score):
+    """The same in fp32, whose ds and dH keep 2^-19 and 2^-24 of themselves."""
+    H, W, y = certain(rows, V, D, score, 2)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    H = H.float() + torch.rand(H.shape, generator=g, device="cuda") * 2.0 ** -9  # low bits set
+    W = W.float()
+    W[0] *= 1.0 + torch.rand(D, generator=g, device="cuda") * 2.0 ** -9
+    loss, lse = gpu.linear_cross_entropy(H, W, y, reduction="none")
+    dH, _ = gpu.linear_cross_entropy_backward(H, W, y, lse, reduction="sum", need_dW=False)
+    w = W[0].double()
+    ds, want = dH.double() @ w / (w @ w), torch.expm1(-loss.double())
+    tol = U * lse.double() + 2.0 ** -22 + 2.0 ** -18 * want.abs()
+    assert bool(((ds - want).abs() <= tol).all()), float(((ds - want).abs() / tol).max())
+
+
 # ------------------------------------------------------- long sums of one sign
 # All scores are 0 here, so p is 1 / V everywhere.  The target's term comes last in its sum and
 # takes away what the others add up to, as bf16 holds it: what is left is rounded to bf16
