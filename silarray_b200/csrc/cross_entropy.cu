@@ -4,9 +4,10 @@
 //   s = H . W^T,  lse_t = log sum_v exp(s_tv),  loss_t = lse_t - s_t,y(t)
 //   ds_tv = g_t (exp(s_tv - lse_t) - [v = y(t)]),  dH = ds . W,  dW = ds^T . H
 //
-// Forward: one tensor-core product whose epilogue keeps, for every row and
-// every 128 columns, the maximum and the sum of exponentials (8 bytes in place
-// of 128 scores) and the target's score; loss_finish joins them.
+// Forward: one tensor-core product whose epilogue keeps, for every row and each half of a
+// tile's columns, the maximum and the sum of exponentials (8 bytes in place of 128
+// scores; tiles of fewer than 256 columns keep the same two parts) and the target's score;
+// loss_finish joins them.
 // Backward: piece by piece of the vocabulary, the same product again with the
 // score gradients as its epilogue (ds of one piece is all that is kept), then
 // dH += ds . W_piece and dW_piece = ds^T . H.  Recomputing the scores costs

@@ -283,7 +283,10 @@ struct LnRow {
 };
 
 // Rows of more than 8192 columns (32 elements a thread) have no registers for
-// the sums and the next row: the sums then live in shared memory.
+// the sums and the next row: the sums then live in shared memory.  512 threads have 128
+// registers each, and rows of 4097 to 8192 columns (16 elements) spill some of theirs: 104
+// bytes a thread of fp32 vectors with a residual gradient, up to 306 where elements move one
+// by one.
 template <int VEC, int VPT, int NT, int GROUPS>
 struct BwdCfg {
   static constexpr int E = VEC * VPT;

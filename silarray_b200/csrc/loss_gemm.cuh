@@ -11,8 +11,8 @@
 //               issues the MMAs from one thread;
 //   warps 2-9   epilogue, two per TMEM lane quarter, 128 columns each.
 // A tile is 256 x 256 on a CTA pair (cta_group::2: each CTA loads its 128 rows
-// of A and 128 columns of B), or 128 x bn on one CTA for the scores of at most
-// 128 rows, where reading W is all and bn spreads it evenly over the SMs.
+// of A and 128 columns of B), or for the scores 128 x bn on one CTA, where that takes fewer
+// rounds of all SMs (score_tiles): few rows, where reading W is all, and few tiles.
 //
 // What bounds it: the tensor pipe and, over many milliseconds, the card's
 // power.  The one thread that issues the MMAs was the limit at first: with a
@@ -27,7 +27,8 @@
 // than its 2^-22 per step are cut into chunks; the epilogue adds each chunk in fp32
 // registers, to nearest, while the next one runs.  Chunks are 128 k of tf32, 1024 k of bf16
 // scores, and 16384 k of the products of bf16 ds, whose results are rounded to bf16: of a sum of
-// one sign such a chunk loses 3 x 10^-5 (2^-13 at most), where 211000 terms in one lost 1.2 x 10^-3.
+// one sign such chunks lose 9 x 10^-5 (2^-13 at most, a chunk's sum growing evenly), where
+// 211000 terms in one chunk lost 1.2 x 10^-3 and 262144 1.7 x 10^-3.
 // The backward's bf16 scores take the forward's chunks although ds is rounded to bf16
 // next: 8 x 10^-4 of a sum of 131072 products of one sign is lost in one chunk, 10^-5 of
 // one of 4096, and where p is near 1 that much is left in p - 1.  It costs steps of D above
@@ -145,7 +146,9 @@ struct Cfg {
   // SUMS: every tile's sums pass through registers; else those of one chunk stay in TMEM.
   static constexpr bool SUMS = Ty::PARTS == 2 || EPI == kStats;
   // Columns that join the sums at a time: 32 leave the tf32 sums no registers, and
-  // what spills there every chunk pays for (score gradients 660 -> 477 us with 16).
+  // what spills there every chunk pays for (score gradients 660 -> 477 us with 16).  What
+  // still spills, outside that loop: 48 bytes a thread of the tf32 score gradients
+  // (not RAW), 36 of the bf16 scores.
   static constexpr int LD = EPI == kStats && Ty::PARTS == 1 ? 32 : 16;
   // The sums go back to TMEM for the epilogues that have no registers beside
   // them (with the 128 sums in registers the tf32 score gradients spill 2.8 KB a thread).
@@ -156,9 +159,10 @@ struct Cfg {
       (Ty::PARTS == 2 ? 128 : EPI == kStats || EPI == kScoreGrad ? 1024 : 16384) / BK;
   // Rows of tiles that are walked together, column by column.  The scores read W once
   // (their H stays in the L2); kOut's tiles of one row of them follow one another and share its
-  // ds: against groups of 8 the DRAM reads of 4096 x 8192 x 768 fp32 fall from 1018 to 783 MB,
-  // and steps at the power limit take 1 to 3 % less (16384 x 32768 x 768 fp32, 8192 x 131072 x
-  // 2048 bf16; 200 x 32768 x 1024 fp32 1 % more).
+  // ds: against groups of 8 the DRAM reads of 4096 x 8192 x 768 fp32 fall from 1018 to 783 MB.
+  // Backward passes of 19 shapes (both types, 200 to 32768 rows, D 512 to 4096) take 1 to 3 %
+  // less than with groups of 16 where ds is the larger operand, as long where tiles are few, and
+  // 1 to 2.4 % more where W is much the larger one (bf16, 1024 and 2048 rows, D 2048 and 4096).
   static constexpr int GROUP_M = EPI == kOut ? 1 : 16;
   static constexpr uint32_t MN_BOX = Ty::KROW * 128;       // KROW elements of M / N x KROW k
   static constexpr uint32_t MN_STEP = Ty::KMMA * 128;      // one MMA's k inside it

@@ -344,7 +344,11 @@ class LossHead:
 
     Activations and W are fp32, or bf16 with dtype=torch.bfloat16 (gamma, beta
     and their gradients stay fp32).  Targets are int32; one outside
-    [0, vocab) leaves its row out.  A whole step can be captured in a CUDA graph."""
+    [0, vocab) leaves its row out.  A whole step can be captured in a CUDA graph.
+
+    forward keeps x and targets themselves for backward, not copies: their buffers (a block's
+    output may be written again by its next forward) stay as they are until then.  backward
+    writes self.grads, it does not add to them."""
 
     def __init__(self, params, device="cuda", dtype=torch.float32, eps=1e-5):
         t = lambda a, dt: torch.from_numpy(np.ascontiguousarray(a)).to(device, dt)  # noqa: E731
