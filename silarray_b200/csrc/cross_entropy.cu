@@ -146,46 +146,41 @@ __global__ void __launch_bounds__(1024) loss_finish(const float2 *part, int npar
   }
 }
 
-// The gradient of every row's loss, 0 for a row that is left out, and behind them the one
-// that all rows share (mean, sum), 0 when none counts: where it multiplies finished sums, which
-// are zero for what is left out, a factor that is not finite must not turn them into NaN.
-struct Scales {
+// The factor that the gradients of a mean or a sum share: 0 when no row counts.
+struct Shared {
   const float *dloss;
   int reduction;
-  float *scale;  // [rows + 1]
+  float *factor;  // null: not wanted
 };
-__device__ __forceinline__ void row_scales(const Scales &c, const int32_t *targets, int64_t rows, int V) {
+__device__ __forceinline__ void shared_factor(const Shared &c, const int32_t *targets, int64_t rows, int V) {
   __shared__ double sm[32];
-  const bool each = c.reduction == SILCU_REDUCE_NONE;
-  float g = 1.0f;
-  if (!each) {
-    const double n = count_rows(targets, rows, V, sm), d = c.dloss ? double(*c.dloss) : 1.0;
-    g = n > 0.0 ? float(c.reduction == SILCU_REDUCE_MEAN ? d / n : d) : 0.0f;
-    if (threadIdx.x == 0) c.scale[rows] = g;
+  const double d = c.dloss ? double(*c.dloss) : 1.0;
+  double f = d;
+  // of a sum only a factor that is not finite would make something of the zeros of no rows
+  if (c.reduction == SILCU_REDUCE_MEAN || !isfinite(d)) {
+    const double n = count_rows(targets, rows, V, sm);
+    f = n == 0.0 ? 0.0 : c.reduction == SILCU_REDUCE_MEAN ? d / n : d;
   }
-  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) {
-    const int y = targets[i];
-    c.scale[i] = y < 0 || y >= V ? 0.0f : each && c.dloss ? c.dloss[i] : g;
-  }
+  if (threadIdx.x == 0) *c.factor = float(f);
 }
 
 // dst [rows, dp] = src [rows, D] (row stride ld), columns D.. zero; with
 // targets, rows that are left out are zero as well.  With `lo`, dst and lo
 // take the exact tf32 pair; with `lo` alone, src itself is to be the hi operand (the
-// tensor core reads its upper 19 bits) and lo takes what that leaves.  With `scales`
-// the first CTA writes the rows' scales.
+// tensor core reads its upper 19 bits) and lo takes what that leaves.  The first CTA
+// writes the shared factor where it is wanted.
 template <typename T>
 __global__ void __launch_bounds__(256) copy_rows(const T *src, int64_t ld, int64_t rows, int D, int dp,
-                                                 const int32_t *targets, int V, T *dst, float *lo, const Scales scales) {
+                                                 const int32_t *targets, int V, T *dst, float *lo, const Shared shared) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = dp / W;
   const bool vec = ld % W == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   const int64_t n = rows * per_row;
-  const int first = scales.scale ? 1 : 0;
+  const int first = shared.factor ? 1 : 0;
   let_next_start();
   wait_for_previous();
   if (first && blockIdx.x == 0) {
-    row_scales(scales, targets, rows, V);
+    shared_factor(shared, targets, rows, V);
     return;
   }
   for (int64_t i = int64_t(blockIdx.x - first) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x - first) * 256) {
@@ -225,25 +220,27 @@ __global__ void __launch_bounds__(256) copy_rows(const T *src, int64_t ld, int64
   }
 }
 
-// out [rows, D] = alpha (with per_row_alpha each row's own) times the sum of the fp32 planes
-// [rows, ldp], in plane order, or for few elements of many planes by WAYS neighbouring lanes
+// out [rows, D] = alpha times the sum of the fp32 planes [rows, ldp] (with targets, 0 for rows
+// that are left out, whatever alpha is), in plane order, or for few elements of many planes by WAYS neighbouring lanes
 // that take turns at the planes (16 planes of 100 x 1024: 9 us by one thread).
 template <typename T, int WAYS>
 __global__ void __launch_bounds__(256) planes_finish(const float *planes, int nplanes, int64_t plane, int64_t rows, int D,
-                                                     int ldp, const float *alpha, int per_row_alpha, T *out, int64_t ldo,
-                                                     int vec) {
+                                                     int ldp, const float *alpha, const int32_t *targets, int V, T *out,
+                                                     int64_t ldo, int vec) {
   constexpr int W = 16 / sizeof(T);
   const int per_row = (D + W - 1) / W;
   const int64_t n = rows * per_row;
   const int way = threadIdx.x % WAYS;
   let_next_start();
   wait_for_previous();
+  const float k0 = alpha ? *alpha : 1.0f;
   for (int64_t i0 = int64_t(blockIdx.x) * (256 / WAYS); i0 < n; i0 += int64_t(gridDim.x) * (256 / WAYS)) {
     const int64_t i = i0 + threadIdx.x / WAYS, r = i / per_row;
     const int c = int(i - r * per_row) * W;
-    float f[W] = {}, k0 = 1.0f;
+    float f[W] = {};
+    int y = 0;
     if (i < n) {
-      if (alpha) k0 = alpha[per_row_alpha ? r : 0];
+      if (targets) y = targets[r];
       const float *src = planes + r * ldp + c;  // ldp is a multiple of W: the last vectors stay inside the row
       constexpr int AHEAD = 32 / W;             // planes on their way at a time
       for (int p = way; p < nplanes; p += AHEAD * WAYS) {
@@ -265,8 +262,9 @@ __global__ void __launch_bounds__(256) planes_finish(const float *planes, int np
       for (int k = 0; k < W; k++) f[k] += __shfl_xor_sync(0xffffffffu, f[k], step);
     }
     if (i >= n || way) continue;
+    const float factor = lossmm::counts(y, V) ? k0 : 0.0f;
 #pragma unroll
-    for (int k = 0; k < W; k++) f[k] *= k0;
+    for (int k = 0; k < W; k++) f[k] *= factor;
     T *dst = out + r * ldo + c;
     Raw<T, W> o;
     pack(f, o);
@@ -397,10 +395,10 @@ struct Copy {
     if (Ty::PARTS == 2) lo = sp.take<float>(rows * dp);
   }
   silcu_status fill(const void *src, int64_t ld, int64_t rows, int64_t D, const int32_t *targets, int64_t V,
-                    cudaStream_t s, const Scales &scales = {}) const {
+                    cudaStream_t s, const Shared &shared = {}) const {
     using T = typename Ty::T;
-    launch_after(copy_rows<T>, stream_grid(rows * dp * int64_t(sizeof(T)) / 16) + (scales.scale ? 1 : 0), 256, 0, s,
-                 static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo, scales);
+    launch_after(copy_rows<T>, stream_grid(rows * dp * int64_t(sizeof(T)) / 16) + (shared.factor ? 1 : 0), 256, 0, s,
+                 static_cast<const T *>(src), ld, rows, int(D), int(dp), targets, int(V), p, lo, shared);
     return check_launch("cross_entropy copy");
   }
   Operand operand(bool mn) const { return Operand{p, lo, dp, dp, mn}; }
@@ -520,7 +518,7 @@ struct Backward {
   int64_t piece, lds;  // lds: row stride of ds
   ScoreTiles score;
   bool copy_w;
-  float *scale;
+  float *factor;       // that all rows share (mean, sum)
   Copy<Ty> h, w;       // H with left-out rows zero; a piece of W
   Copy<Ty> ds;
   Gradient dh, dw;
@@ -530,7 +528,7 @@ struct Backward {
     const int64_t of_w = copy_w ? up(a.D, 8) : 0;
     piece = piece_of(a.V, a.rows > of_w ? a.rows : of_w, limit);
     score = score_tiles(a.rows, piece, raw_w<Ty>(a));
-    scale = sp.take<float>(a.rows + 1);
+    factor = a.reduction == SILCU_REDUCE_NONE ? nullptr : sp.take<float>(1);
     h.take(sp, a.rows, a.D);
     if (copy_w) w.take(sp, piece, a.D, Ty::PARTS == 2 && rows16(a.W, a.ldw, a.dtype));
     ds.take(sp, a.rows, up(piece, 64));
@@ -645,14 +643,14 @@ void set_output(lossmm::Problem &q, const Gradient &g, bool add, void *out, int6
 }
 
 template <typename Ty>
-silcu_status finish_planes(const Gradient &g, int64_t rows, int64_t D, const float *alpha, bool per_row, void *out,
-                           int64_t ldo, int vec, cudaStream_t s) {
+silcu_status finish_planes(const Gradient &g, int64_t rows, int64_t D, const float *alpha, const int32_t *targets, int64_t V,
+                           void *out, int64_t ldo, int vec, cudaStream_t s) {
   using T = typename Ty::T;
   const int64_t ldp = up(D, 8);
   const int64_t vectors = rows * ceil_div(D * int64_t(sizeof(T)), 16);
   const bool few = g.split >= 8 && vectors * 8 <= int64_t(sm_count()) * 2048;  // eight lanes each fill the SMs at most once
   launch_after(few ? planes_finish<T, 8> : planes_finish<T, 1>, stream_grid(vectors * (few ? 8 : 1)), 256, 0, s, g.planes,
-               g.split, g.M * ldp, rows, int(D), int(ldp), alpha, int(per_row), static_cast<T *>(out), ldo, vec);
+               g.split, g.M * ldp, rows, int(D), int(ldp), alpha, targets, int(V), static_cast<T *>(out), ldo, vec);
   return check_launch("cross_entropy planes");
 }
 
@@ -661,11 +659,11 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
   using T = typename Ty::T;
   constexpr int BK = lossmm::Cfg<Ty, lossmm::kOut, true>::BK;
   silcu_status st;
-  if ((st = b.h.fill(a.H, a.ldh, a.rows, a.D, a.targets, a.V, s, Scales{a.dloss, a.reduction, b.scale})) != SILCU_OK)
+  if ((st = b.h.fill(a.H, a.ldh, a.rows, a.D, a.targets, a.V, s, Shared{a.dloss, a.reduction, b.factor})) != SILCU_OK)
     return st;
-  // A factor that all rows share leaves ds alone where ds is rounded.
-  const bool shared = Ty::PARTS == 1 && a.reduction != SILCU_REDUCE_NONE;
-  const float *dh_alpha = shared ? b.scale : nullptr, *dw_alpha = shared ? b.scale + a.rows : nullptr;
+  // A factor that all rows share leaves ds alone where ds is rounded, and multiplies the results;
+  // dH's rows that are left out stay 0 whatever it is.
+  const float *alpha = Ty::PARTS == 1 ? b.factor : nullptr;
   const int dh_vec = rows16(a.dH, a.lddh, a.dtype), dw_vec = rows16(a.dW, a.lddw, a.dtype);
   for (int64_t v0 = 0; v0 < a.V; v0 += b.piece) {
     const int64_t n = a.V - v0 < b.piece ? a.V - v0 : b.piece;
@@ -686,7 +684,8 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
     p.loss.V = int32_t(a.V);
     p.loss.v0 = int32_t(v0);
     p.loss.lse = a.lse;
-    p.loss.scale = shared ? nullptr : b.scale;
+    p.loss.scale = a.reduction == SILCU_REDUCE_NONE ? a.dloss : alpha ? nullptr : b.factor;
+    p.loss.per_row = a.reduction == SILCU_REDUCE_NONE;
     if ((st = scores<Ty, lossmm::kScoreGrad>(p, b.score, s)) != SILCU_OK) return st;
 
     const bool pairs = !b.score.raw;
@@ -696,13 +695,15 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
       p.err = device_error_ptr();
       p.bn = bn;
       p.rows_a = lossmm::BM;
+      p.alpha = alpha;
+      p.loss.targets = a.targets;
+      p.loss.V = int32_t(a.V);
     };
     if (b.dh.wanted && b.dh.transposed) {
       clear(int(up(a.rows, 32)));
       if (!pairs) set_raw(p);
       if (!lossmm::set_problem<Ty>(p.p[0], pairs, p.bn, lossmm::BM, a.D, a.rows, n, w, b.ds.operand(false))) return map_error();
       set_output(p.p[0], b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
-      p.p[0].alpha = dh_alpha;
       if constexpr (Ty::PARTS == 2)
         st = pairs ? lossmm::launch<Ty, lossmm::kOutT, true>(p, 1, s) : lossmm::launch<Ty, lossmm::kOutT, false, true>(p, 1, s);
       else
@@ -722,21 +723,19 @@ silcu_status backward(const Args &a, const Backward<Ty> &b, cudaStream_t s) {
           return map_error();
         set_output(q, b.dw, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, a.D,
                    ceil_div(a.rows, BK));
-        q.alpha = dw_alpha;
       } else {
         if (!lossmm::set_problem<Ty>(q, true, p.bn, lossmm::BM, a.rows, a.D, n, b.ds.operand(false), w)) return map_error();
         set_output(q, b.dh, v0 != 0, a.dH, a.lddh, dh_vec, a.D, ceil_div(n, BK));
-        q.alpha = dh_alpha;
-        q.per_row = 1;
+        q.of_rows = 1;
       }
     }
     if (count && (st = lossmm::launch<Ty, lossmm::kOut, true>(p, count, s)) != SILCU_OK) return st;
     if (b.dw.wanted && !b.dw.direct) {
-      st = finish_planes<Ty>(b.dw, n, a.D, dw_alpha, false, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, s);
+      st = finish_planes<Ty>(b.dw, n, a.D, alpha, nullptr, a.V, static_cast<T *>(a.dW) + v0 * a.lddw, a.lddw, dw_vec, s);
       if (st != SILCU_OK) return st;
     }
   }
-  if (b.dh.wanted && !b.dh.direct) return finish_planes<Ty>(b.dh, a.rows, a.D, dh_alpha, true, a.dH, a.lddh, dh_vec, s);
+  if (b.dh.wanted && !b.dh.direct) return finish_planes<Ty>(b.dh, a.rows, a.D, alpha, alpha ? a.targets : nullptr, a.V, a.dH, a.lddh, dh_vec, s);
   return SILCU_OK;
 }
 

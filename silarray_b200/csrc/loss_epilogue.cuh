@@ -25,7 +25,8 @@ struct LossArgs {
   float *target_score;     // forward: [rows], written for rows that count
   unsigned *done;          // forward: set to 0 for what follows
   const float *lse;        // backward: [rows]
-  const float *scale;      // backward: [rows] gradient of each row's loss, or null = 1
+  const float *scale;      // backward: gradient of the rows' loss, one or (per_row) [rows], or null = 1
+  int per_row;
 };
 
 // (m, l) of 128 scores, of which the first `valid` exist.  The terms are

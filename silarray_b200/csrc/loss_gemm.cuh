@@ -115,6 +115,9 @@ __device__ __forceinline__ float remainder_of(float x) {
   return __fmul_rn(__fsub_rn(x, tf32_trunc(x)), 1.0f + 1.0f / 4096.0f);
 }
 
+// Whether a row with this target is not left out.
+__device__ __forceinline__ bool counts(int y, int V) { return y >= 0 && y < V; }
+
 struct Bf16 {
   using T = __nv_bfloat16;
   static constexpr int PARTS = 1, KROW = 64, KMMA = 16;  // k in a 128-byte row, and of one MMA
@@ -192,10 +195,7 @@ struct Problem {
   int ksplit;              // each tile's K range in this many parts (kOut; part i -> plane i)
   int amn;                 // kOut: A is stored with the M index contiguous (kOutT: it always is)
   int mode, vec;           // vec: kDirect rows are 16-byte aligned
-  // Factor of kDirect results in bf16, or null: one, or with per_row one for each row of
-  // the result; kOutT has one for each of the N rows that it writes.
-  const float *alpha;
-  int per_row;
+  int of_rows;             // kOut: the result is dH, with a row for each target (kOutT: always)
   void *out;
   int64_t ldo, plane;      // row stride; elements from one plane to the next
 };
@@ -210,6 +210,7 @@ struct __align__(64) Params {
   int stages;        // ring stages (RAW)
   // Work items n0 of p[0] and n1 of p[1] over `units` CTAs (pairs); see work_at.
   int units, n0, n1, rounds, tail, extra;  // rounds = n0 / units, tail = n0 % units
+  const float *alpha;  // kOut, kOutT: factor of kDirect results in bf16, 0 for rows that are left out; or null = 1
   LossArgs loss;
   int part0;  // index of this launch's first part
   int *err;
@@ -452,6 +453,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
     const int qr = warp & 3, h = (warp - 2) >> 2;
     float *st = reinterpret_cast<float *>(smem + C::RING_BYTES) + (warp - 2) * 1024;
     const int half = RAW || EPI == kOut ? p.half : 128;
+    const float alpha = (EPI == kOut || EPI == kOutT) && p.alpha ? *p.alpha : 1.0f;
     uint32_t cg = 0, kbe = 0;
     bool ok = true;
     for (int k = 0; ok && work_at(p, unit, k, w); k++) {
@@ -509,10 +511,10 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           y = max(p.loss.targets[row], -1);  // any negative one; differences with it do not overflow
           if (EPI == kScoreGrad) {
             lse = p.loss.lse[row] * kLog2e;
-            g = p.loss.scale ? p.loss.scale[row] : 1.0f;
+            g = p.loss.scale ? p.loss.scale[p.loss.per_row ? row : 0] : 1.0f;
           }
         }
-        if (EPI == kOut && PARTS == 1) g = q.alpha && row < q.M ? q.alpha[q.per_row ? row : 0] : 1.0f;
+        if (EPI == kOut && PARTS == 1) y = p.alpha && q.of_rows && row < q.M ? p.loss.targets[row] : 0;
       };
       if (EARLY) row_data();
       const uint32_t src0 = tmem + (uint32_t(32 * qr) << 16) + half * h;
@@ -632,7 +634,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           if (cols >= 128) softmax_part(acc, 128, m, l);
           else softmax_part(acc, cols, m, l);
           const int at = y - p.loss.v0 - c0;  // the target among this thread's columns
-          if (y >= 0 && y < p.loss.V && at >= 0 && at < min(cols, 128)) {
+          if (counts(y, p.loss.V) && at >= 0 && at < min(cols, 128)) {
 #pragma unroll
             for (int i = 0; i < 128; i++)
               if (i == at) p.loss.target_score[row] = acc[i];
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         }
       } else if constexpr (EPI == kScoreGrad) {
         if (r0 < q.M) {
-          const bool counts = y >= 0 && y < p.loss.V;
+          const bool used = counts(y, p.loss.V);
           const int at = y - p.loss.v0 - c0;
           // plain stores need no wait before the next block; rows of ds end on whole vectors
           auto store = [](T *dst, const uint4 &x) { *reinterpret_cast<uint4 *>(dst) = x; };
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
             if (32 * cb < cols) {
               float v[32];
               block(cb, v);
-              score_gradient(v, lse, g, at - 32 * cb, counts);
+              score_gradient(v, lse, g, at - 32 * cb, used);
               if constexpr (PARTS == 1) {  // 64 bf16 columns per 128-byte row: two blocks a store
 #pragma unroll
                 for (int i = 0; i < 4; i++)
@@ -684,12 +686,16 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
           if (32 * cb < cols) {
             float v[32];
             block(cb, v);
+            uint32_t left_out = 0;  // of the block's 32 output rows
+            if (PARTS == 1 && q.mode == kDirect && p.alpha)
+              left_out = __ballot_sync(0xffffffffu, lane < cols - 32 * cb &&
+                                                        !counts(p.loss.targets[c0 + 32 * cb + lane], p.loss.V));
             if (row < q.M) {
               const int64_t at = int64_t(c0 + 32 * cb) * q.ldo + row;
 #pragma unroll
               for (int i = 0; i < 32; i++) {
                 if (32 * cb + i < cols) {
-                  if (q.mode == kDirect) store_as(static_cast<T *>(q.out) + at + i * q.ldo, q.alpha ? q.alpha[c0 + 32 * cb + i] * v[i] : v[i]);
+                  if (q.mode == kDirect) store_as(static_cast<T *>(q.out) + at + i * q.ldo, left_out >> i & 1 ? 0.f : alpha * v[i]);
                   else if (q.mode == kPlane) static_cast<float *>(q.out)[tl.part * q.plane + at + i * q.ldo] = v[i];
                   else red_add(static_cast<float *>(q.out) + tl.part * q.plane + at + i * q.ldo, v[i]);
                 }
@@ -699,6 +705,7 @@ __global__ void __launch_bounds__(Cfg<Ty, EPI, PAIR, RAW>::THREADS, 1) gemm(cons
         }
       } else if (r0 < q.M) {
         const int mode = q.mode;
+        if (PARTS == 1) g = p.alpha && !counts(y, p.loss.V) ? 0.f : alpha;
         const bool direct16 = mode == kDirect && PARTS == 1;
         const int64_t ldo = q.ldo;
         float *out = static_cast<float *>(q.out) + tl.part * q.plane;
